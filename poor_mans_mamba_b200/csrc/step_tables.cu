@@ -1,0 +1,208 @@
+// What surrounds a step of drafted tokens on the cache's side: block tables and the tokens' places built on the device from the
+// requests' lengths, and the kept tokens' keys and values moved into the pages.
+//
+// step_tables, request s with held[s] cached tokens, new[s] tokens in this step and blocks[s] pages of its own:
+//   after = max(blocks, ceil((held + new) / P)),  table[s, blocks .. after) = the next free pages, in the requests' order,
+//   cu = running sums of new,  token i: position held + depth(i), slot = table[s, (held + i) / P] * P + (held + i) % P,
+//   mask bit j = token j of the request is i or one of its ancestors (parents lie in front of their children).
+// Nothing but latency bounds it: a block per request adds up the lengths of the requests in front of it (all loads of a thread
+// go out together; 512 requests are two loads a thread and length) instead of a launch of its own for the sums.
+//
+// keep_accepted: rows[l, plane, cu[s] + path[s, j]] -> pool[l, slot / P, plane, slot % P], slot = slots[cu[s] + j], j < count[s].
+// A copy: a block per (layer and plane, request), every thread's pieces asked for before the first is stored.
+//
+// What these kernels write, later launches read ahead of their wait (sequence bounds, tables, cached keys): neither lets the
+// launch behind it begin early.
+#include "common.cuh"
+
+namespace pmm {
+
+constexpr int kTablesThreads = 256;
+constexpr int kTablesNodes = 1024;  // parents of a request kept in shared memory
+
+struct StepTablesArgs {
+  const int* held;
+  const int* fresh;       // new tokens
+  const int* blocks;
+  int* table;             // [n, width]
+  int width;
+  const int* free_pages;
+  int n_free, n, page_size, spare;
+  int* cu;
+  int* seq_of;
+  int* positions;
+  int* slots;
+  int cap;                // tokens that the three have room for
+  int* blocks_out;
+  int* taken;
+  const int* parents;     // [cap] or nullptr: chains
+  unsigned long long* masks;
+  int words;
+};
+
+__device__ __forceinline__ int blocks_after(int held, int fresh, int blocks, int page_size) {
+  return max(blocks, static_cast<int>((static_cast<long long>(held) + fresh + page_size - 1) / page_size));
+}
+
+__global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(const StepTablesArgs a) {
+  __shared__ int s_sum[2][kTablesThreads / 32];
+  __shared__ int s_up[kTablesNodes];
+  pdl_wait();
+  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int held = max(a.held[s], 0), fresh = max(a.fresh[s], 0), blocks = max(a.blocks[s], 0);
+  int tokens = 0, pages = 0;  // of the requests in front of this one
+  for (int i = tid; i < s; i += kTablesThreads) {
+    const int f = max(a.fresh[i], 0), b = max(a.blocks[i], 0);
+    tokens += f;
+    pages += blocks_after(max(a.held[i], 0), f, b, a.page_size) - b;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
+    pages += __shfl_xor_sync(0xffffffffu, pages, o);
+  }
+  if (lane == 0) {
+    s_sum[0][warp] = tokens;
+    s_sum[1][warp] = pages;
+  }
+  __syncthreads();
+  int t0 = 0, g0 = 0;
+#pragma unroll
+  for (int w = 0; w < kTablesThreads / 32; ++w) {
+    t0 += s_sum[0][w];
+    g0 += s_sum[1][w];
+  }
+  const int after = blocks_after(held, fresh, blocks, a.page_size);
+  if (tid == 0) {
+    a.cu[s] = t0;
+    a.blocks_out[s] = after;
+    if (s == a.n - 1) {
+      a.cu[a.n] = t0 + fresh;
+      a.taken[0] = g0 + after - blocks;
+    }
+  }
+  int* row = a.table + static_cast<size_t>(s) * a.width;
+  // block b's page: one of the request's own, or the next free one
+  auto page_of = [&](int b) {
+    if (b >= a.width) return a.spare;
+    if (b < blocks) return row[b];
+    const int i = g0 + b - blocks;
+    return i < a.n_free ? a.free_pages[i] : a.spare;
+  };
+  for (int b = blocks + tid; b < a.width; b += kTablesThreads) row[b] = b < after ? page_of(b) : a.spare;
+
+  const int n = min(fresh, a.cap - t0);  // (t0 <= cap unless the lengths do not fit the step)
+  const bool cached = n <= kTablesNodes;
+  if (a.parents != nullptr && cached) {
+    for (int i = tid; i < n; i += kTablesThreads) s_up[i] = a.parents[t0 + i];
+    __syncthreads();
+  }
+  for (int i = tid; i < n; i += kTablesThreads) {
+    const int t = t0 + i, pos = held + i;
+    const int page = page_of(pos / a.page_size);
+    a.seq_of[t] = s;
+    a.slots[t] = page < 0 || page == a.spare ? -1 : page * a.page_size + pos % a.page_size;
+    int depth = i;
+    if (a.parents != nullptr) {
+      depth = 0;
+      unsigned long long bits[4] = {0ull, 0ull, 0ull, 0ull};
+      for (int j = i;;) {
+        if (j < 64 * a.words) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            if (j >> 6 == w) bits[w] |= 1ull << (j & 63);
+        }
+        const int up = cached ? s_up[j] : a.parents[t0 + j];
+        if (up < 0 || up >= j) break;  // (a parent lies in front of its child: anything else is a root)
+        j = up;
+        ++depth;
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        if (w < a.words) a.masks[static_cast<size_t>(t) * a.words + w] = bits[w];
+    }
+    a.positions[t] = held + depth;
+  }
+}
+
+constexpr int kKeepThreads = 128;
+constexpr int kKeepLoads = 4;  // pieces of a thread in flight
+
+// V: the piece that a thread copies at a time (16 bytes where rows begin on such boundaries).
+template <typename V>
+__global__ void __launch_bounds__(kKeepThreads)
+    keep_accepted_kernel(const V* rows, long long ld_layer, long long ld_plane, long long ld_row, int n_rows, V* pool, long long pages,
+                         int planes, int page_size, int width, const int* slots, const int* cu, const int* path, int path_width,
+                         const int* count) {
+  pdl_wait();
+  const int s = blockIdx.y, tid = threadIdx.x;
+  const int layer = blockIdx.x / planes, plane = blockIdx.x % planes;
+  const int t0 = cu[s], t1 = min(cu[s + 1], n_rows);
+  const int kept = min(min(count[s], path_width), t1 - t0);
+  if (kept <= 0) return;
+  const V* src = rows + layer * ld_layer + plane * ld_plane;
+  V* dst = pool + (static_cast<long long>(layer) * pages * planes + plane) * page_size * width;
+  const long long n_slots = pages * page_size;
+  const long long items = static_cast<long long>(kept) * width;
+  for (long long base = tid; base < items; base += kKeepThreads * kKeepLoads) {
+    V v[kKeepLoads];
+    long long to[kKeepLoads];
+#pragma unroll
+    for (int u = 0; u < kKeepLoads; ++u) {
+      const long long it = base + u * kKeepThreads;
+      to[u] = -1;
+      if (it < items) {
+        const int j = static_cast<int>(it / width), c = static_cast<int>(it - static_cast<long long>(j) * width);
+        const int node = path[static_cast<size_t>(s) * path_width + j], slot = slots[t0 + j];
+        if (node >= 0 && t0 + node < t1 && slot >= 0 && slot < n_slots) {
+          v[u] = src[static_cast<long long>(t0 + node) * ld_row + c];
+          to[u] = (static_cast<long long>(slot / page_size) * planes * page_size + slot % page_size) * width + c;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kKeepLoads; ++u)
+      if (to[u] >= 0) dst[to[u]] = v[u];
+  }
+}
+
+}  // namespace pmm
+
+// parents (with masks [cap, words], 1 to 4 words) or neither; table [n, width] and the lengths [n] contiguous.
+PMM_EXPORT int pmm_step_tables(const int* held, const int* fresh, const int* blocks, int* table, int width, const int* free_pages, int n_free,
+                               int n, int page_size, int spare, int* cu, int* seq_of, int* positions, int* slots, int cap, int* blocks_out,
+                               int* taken, const int* parents, void* masks, int words, cudaStream_t stream) {
+  if (n <= 0) return 0;
+  if (width <= 0 || n_free < 0 || page_size <= 0 || spare < 0 || cap < 0 || (static_cast<long long>(spare) + 1) * page_size > 0x7fffffffll ||
+      (parents == nullptr) != (masks == nullptr) || (parents && (words < 1 || words > 4)))
+    return PMM_ERR_BAD_ARGUMENT;
+  pmm::StepTablesArgs a{held, fresh, blocks, table, width, free_pages, n_free, n, page_size, spare, cu, seq_of, positions, slots, cap, blocks_out,
+                        taken, parents, static_cast<unsigned long long*>(masks), words};
+  pmm::launch_pdl(pmm::step_tables_kernel, dim3(n), dim3(pmm::kTablesThreads), 0, stream, a);
+  return pmm::launch_status();
+}
+
+// rows: strides in elements of `item` bytes; pool [layers, pages, planes, page_size, width] contiguous.
+PMM_EXPORT int pmm_keep_accepted(const void* rows, long long ld_layer, long long ld_plane, long long ld_row, int n_rows, void* pool, int layers,
+                                 long long pages, int planes, int page_size, int width, int item, const int* slots, const int* cu,
+                                 const int* path, int path_width, const int* count, int n, cudaStream_t stream) {
+  if (n <= 0 || layers <= 0 || planes <= 0) return 0;
+  if (pages <= 0 || page_size <= 0 || width <= 0 || path_width <= 0 || n_rows < 0 || n > 65535 || (item != 2 && item != 4) ||
+      static_cast<long long>(layers) * planes > 0x7fffffffll)
+    return PMM_ERR_BAD_ARGUMENT;
+  // the widest piece that every row begins on
+  const long long all = reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(pool) | (ld_layer * item) | (ld_plane * item) |
+                        (ld_row * item) | (static_cast<long long>(width) * item);
+  const dim3 grid(layers * planes, n);
+  auto go = [&](auto zero) {
+    using V = decltype(zero);
+    const int per = static_cast<int>(sizeof(V)) / item;
+    pmm::launch_pdl(pmm::keep_accepted_kernel<V>, grid, dim3(pmm::kKeepThreads), 0, stream, static_cast<const V*>(rows), ld_layer / per,
+                    ld_plane / per, ld_row / per, n_rows, static_cast<V*>(pool), pages, planes, page_size, width / per, slots, cu, path, path_width,
+                    count);
+    return pmm::launch_status();
+  };
+  if (all % 16 == 0) return go(uint4{});
+  if (all % 4 == 0) return go(0u);
+  return go(static_cast<unsigned short>(0));
+}

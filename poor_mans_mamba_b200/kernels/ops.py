@@ -180,6 +180,16 @@ _SIGNATURES = {
                                c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "pmm_relu_squared": [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int, c_void_p],
+    "pmm_step_tables": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                        c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
+    "pmm_keep_accepted": [c_void_p, c_longlong, c_longlong, c_longlong, c_int, c_void_p, c_int, c_longlong, c_int, c_int, c_int,
+                          c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p],
+    "pmm_tree_attention": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p,
+                           c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
+                           c_int, c_int, c_int, c_void_p],
+    "pmm_verify_scratch": [c_longlong, c_int],
+    "pmm_verify_drafts": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                          c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
     "pmm_sample_rows": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                         c_void_p, c_void_p, c_void_p],
 }
@@ -2301,6 +2311,225 @@ def sample_rows(logits: Tensor, temperature: Optional[Tensor], seeds: Optional[T
     slots, tickets = ensure_sample_scratch(logits.device, n)
     _call("pmm_sample_rows", logits.data_ptr(), ld, _ptr(temperature), _ptr(seeds), _ptr(steps),
           out.data_ptr(), n, V, slots.data_ptr(), tickets.data_ptr(), _stream())
+
+
+# ----------------------------------------------------------------------------- steps of drafted tokens
+# A request's tokens of such a step are its last token (the root, token 0) and the drafted ones, each behind its parent.
+TREE_MASK_WORDS = 4  # 64-bit words of a token's mask: trees of up to 256 tokens
+
+
+def _i32vec(t: Tensor, n: int, what: str) -> None:
+    _i32(t, what)
+    if t.numel() != n:
+        raise KernelError(f"{what}: need int32 [{n}], got {tuple(t.shape)}")
+
+
+def _same_device(what: str, *tensors: Optional[Tensor]) -> None:
+    """All on the current CUDA device (the launch goes to the current device's stream)."""
+    _cuda(*tensors)
+    current = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != current:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{current}")
+
+
+def _mask_words(mask: Tensor, rows: int, what: str) -> int:
+    if not (mask.dtype == torch.int64 and mask.dim() == 2 and mask.shape[0] == rows and mask.is_contiguous()
+            and 1 <= mask.shape[1] <= TREE_MASK_WORDS):
+        raise KernelError(f"{what}: masks must be contiguous int64 [tokens, 1..{TREE_MASK_WORDS}]")
+    return mask.shape[1]
+
+
+def step_tables(held: Tensor, new: Tensor, blocks: Tensor, table: Tensor, free_pages: Tensor, page_size: int, spare_page: int,
+                cu: Tensor, seq_of: Tensor, positions: Tensor, slots: Tensor, blocks_out: Tensor, taken: Tensor,
+                parents: Optional[Tensor] = None, masks: Optional[Tensor] = None) -> None:
+    """A step's tables from the requests' lengths, on the device: ``held`` [n] tokens in the cache, ``new`` [n] tokens in this
+    step (0: none), ``blocks`` [n] pages that a request owns already, all int32.
+    ``table`` [n, width] keeps its first ``blocks`` entries; the pages that held + new tokens need beyond them are taken from
+    ``free_pages`` in the requests' order, everything behind is ``spare_page``.  Written: ``cu`` [n + 1], ``blocks_out`` [n]
+    (not ``blocks`` itself), ``taken`` [1] the number of pages that the step needs (more than there are free ones, or a table
+    that is too narrow: the missing pages are the spare page), and per token ``seq_of``, ``positions`` and ``slots`` (page *
+    page_size + offset of the request's i-th token at held + i; -1 where its page is missing).  The three have room for a step
+    of a fixed size: what lies behind the last token is left as it was.
+    ``parents`` [room], with ``masks`` int64 [room, words]: a token's parent as a place among its request's tokens, in front of
+    it (anything else: none, as -1).  ``positions`` are then held + depth, and bit j of a token's mask says that token j of its
+    request is the token itself or above it (64 * words tokens a request; further ones have no bit).  Without: held + i.
+    What it writes, a launch directly behind may read ahead of its wait: this one lets none begin early."""
+    what = "step_tables"
+    _same_device(what, held, new, blocks, table, free_pages, cu, seq_of, positions, slots, blocks_out, taken, parents, masks)
+    n, cap = held.numel(), seq_of.numel()
+    for t, size, name in ((held, n, "held"), (new, n, "new"), (blocks, n, "blocks"), (blocks_out, n, "blocks_out"), (cu, n + 1, "cu"),
+                          (positions, cap, "positions"), (slots, cap, "slots"), (seq_of, cap, "seq_of"), (taken, 1, "taken")):
+        _i32vec(t, size, f"{what}: {name}")
+    _i32(free_pages, f"{what}: free_pages")
+    _i32(table, f"{what}: table")
+    if not (table.dim() == 2 and table.shape[0] == n and table.shape[1] > 0):
+        raise KernelError(f"{what}: table must be int32 [requests, blocks]")
+    if n == 0:
+        raise KernelError(f"{what}: needs a request")
+    if blocks_out.data_ptr() == blocks.data_ptr():
+        raise KernelError(f"{what}: blocks_out must not be blocks (every request reads those in front of it)")
+    if page_size <= 0 or spare_page < 0 or (spare_page + 1) * page_size > 0x7fffffff:
+        raise KernelError(f"{what}: places in the pool do not fit 32 bits")
+    words = 0
+    if (parents is None) != (masks is None):
+        raise KernelError(f"{what}: parents and masks go together")
+    if masks is not None:
+        _i32vec(parents, cap, f"{what}: parents")
+        words = _mask_words(masks, cap, what)
+    _call("pmm_step_tables", held.data_ptr(), new.data_ptr(), blocks.data_ptr(), table.data_ptr(), table.shape[1], free_pages.data_ptr(),
+          free_pages.numel(), n, int(page_size), int(spare_page), cu.data_ptr(), seq_of.data_ptr(), positions.data_ptr(),
+          slots.data_ptr(), cap, blocks_out.data_ptr(), taken.data_ptr(), _ptr(parents), _ptr(masks), words, _stream())
+
+
+def tree_attention_scratch(device) -> Tensor:
+    """What `tree_attention` needs beside its operands: one buffer for any number of calls on one stream at a time (two graphs
+    that may run side by side need one each).  Every call leaves its counters at zero."""
+    return torch.zeros(1, dtype=torch.float32, device=torch.device(device))
+
+
+def _aligned_rows(t: Tensor, width: int, rows: int, what: str) -> int:
+    ld = _rows_view(t, what)
+    if t.shape != (rows, width):
+        raise KernelError(f"{what}: need [{rows}, {width}], got {tuple(t.shape)}")
+    if t.data_ptr() % 16 or (rows > 1 and ld * t.element_size() % 16):
+        raise KernelError(f"{what}: rows must begin on 16-byte boundaries")
+    return ld
+
+
+def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: Tensor, held: Tensor, cu_seqlens: Tensor, out: Tensor,
+                   n_q_heads: int, n_kv_heads: int, head_dim: int, softmax_scale: float, scratch: Tensor,
+                   mask: Optional[Tensor] = None, positions: Optional[Tensor] = None, window: int = 0,
+                   sink: Optional[Tensor] = None) -> None:
+    """Attention of a step's drafted tokens: token t of request s (``cu_seqlens`` int32 [n + 1]) over the request's ``held``
+    [n] cached keys and, of the request's own tokens in this step, those whose bits ``mask`` [T, words] holds (`step_tables`;
+    None: those in front of it and itself).  ``k``/``v`` [T, Hkv*Dh] are the step's keys and values, rotated and scaled as the
+    cache holds them (`qkv_rope_store` without a pool leaves them so); they are not in the cache yet.  ``q``, ``k``, ``v`` may
+    be column slices of wider rows.  ``window`` limits the cached keys as in `paged_attention`, counted from ``positions`` [T];
+    among the step's tokens the mask alone decides.  ``sink``: see `paged_attention`.
+    A row that sees no key is zero; rows behind the last request (cu_seqlens[n] and further) are left as they are."""
+    what = "tree_attention"
+    _same_device(what, q, k, v, pool, block_table, held, cu_seqlens, out, scratch, mask, positions, sink)
+    check_head_dim(head_dim, FLOAT_ATTENTION_MAX_HEAD)
+    if not (n_kv_heads > 0 and n_q_heads > 0 and n_q_heads % n_kv_heads == 0):
+        raise KernelError(f"{what}: query heads must be a multiple of key/value heads")
+    T, n_seq = q.shape[0], held.numel()
+    kv_dim = n_kv_heads * head_dim
+    ldq, ldk, ldv = (_aligned_rows(t, w, T, f"{what}: {name}") for t, w, name in
+                     ((q, n_q_heads * head_dim, "q"), (k, kv_dim, "k"), (v, kv_dim, "v")))
+    if not (q.dtype == k.dtype == v.dtype == pool.dtype == out.dtype):
+        raise KernelError(f"{what}: q, k, v, pool and out must be of one type")
+    if not (out.is_contiguous() and out.shape == (T, n_q_heads * head_dim) and out.data_ptr() % 16 == 0):
+        raise KernelError(f"{what}: out must be contiguous [T, Hq*Dh] on a 16-byte boundary")
+    if not (pool.dim() == 4 and pool.shape[1] == 2 and pool.shape[3] == kv_dim and pool.is_contiguous() and pool.data_ptr() % 16 == 0
+            and pool.shape[0] > 0):
+        raise KernelError(f"{what}: pool must be contiguous [pages, 2, page_size, Hkv*Dh]")
+    _i32(block_table, f"{what}: block_table")
+    _i32vec(held, n_seq, f"{what}: held")
+    _i32vec(cu_seqlens, n_seq + 1, f"{what}: cu_seqlens")
+    if not (block_table.dim() == 2 and block_table.shape[0] == n_seq and n_seq > 0 and block_table.shape[1] > 0):
+        raise KernelError(f"{what}: one row of the block table per request")
+    if not softmax_scale > 0:
+        raise KernelError(f"{what}: the scale must be positive")
+    words = _mask_words(mask, T, what) if mask is not None else 0
+    if window != 0 and positions is None:
+        raise KernelError(f"{what}: a window needs the tokens' positions")
+    if positions is not None:
+        _i32vec(positions, T, f"{what}: positions")
+    _f32vec(sink, n_q_heads, f"{what}: sink")
+    if not (scratch.dtype == torch.float32 and scratch.is_contiguous()):
+        raise KernelError(f"{what}: scratch comes from tree_attention_scratch")
+    _call("pmm_tree_attention", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, pool.data_ptr(), pool.shape[0],
+          block_table.data_ptr(), block_table.shape[1], held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words,
+          _ptr(sink), out.data_ptr(), float(softmax_scale), int(window), pool.shape[2], n_seq, T, n_q_heads, n_kv_heads, head_dim,
+          _dt(q), _stream())
+
+
+def verify_drafts_scratch(n_rows: int, vocab: int, device) -> Tensor:
+    """Scratch of `verify_drafts` for up to ``n_rows`` rows of ``vocab`` entries (contents do not matter)."""
+    f = _fn("pmm_verify_scratch")
+    f.restype = c_longlong
+    return torch.empty(max(16, int(f(int(n_rows), int(vocab)))), dtype=torch.uint8, device=torch.device(device))
+
+
+def verify_drafts(logits: Tensor, tokens: Tensor, cu_seqlens: Tensor, uniforms: Tensor, tokens_out: Tensor, path: Tensor, count: Tensor,
+                  scratch: Tensor, temperature: Optional[Tensor] = None, parents: Optional[Tensor] = None,
+                  draft_logits: Optional[Tensor] = None) -> None:
+    """Which drafted tokens the target keeps.  ``logits`` float32 [T, V]: row t is the target's answer behind token t of the step;
+    ``tokens`` int32 [T]; ``uniforms`` float32 [T] in [0, 1); ``temperature`` [n] per request (None, or not above 0: greedy).
+    With ``draft_logits`` [T, V] (row t: what the draft of the token behind t was drawn from, at the same temperature) the
+    drafts are a chain: token i is kept when u_i q(x_i) < p(x_i) and all before it are, and the next token is drawn from
+    max(p - q, 0) behind the first refusal, else from p, with the root's uniform.  Without, they are fixed proposals, a chain or
+    (``parents``) a tree: every node's next token is drawn from p with its uniform and the walk follows the first child that
+    holds it.  A draw takes the first index whose running sum passes u times the whole, in 64 bits; ties go to the lowest index.
+    Written per request: ``count`` [n] (1 + kept drafts; 0 for a request without tokens), ``tokens_out`` [n, width] the kept
+    tokens and the next one, ``path`` [n, width] the root and the kept tokens' places among the request's, both -1 behind
+    them.  Drafts deeper than the outputs are wide are not looked at.
+    NaN logits count as -inf.  A row that holds nothing else keeps no draft and gives token 0."""
+    what = "verify_drafts"
+    _same_device(what, logits, tokens, cu_seqlens, uniforms, tokens_out, path, count, scratch, temperature, parents, draft_logits)
+    if not (logits.dtype == torch.float32 and logits.dim() == 2):
+        raise KernelError(f"{what}: logits must be float32 [T, V]")
+    ld = _rows_view(logits, f"{what}: logits")
+    T, V = logits.shape
+    n = count.numel()
+    if not (n > 0 and V > 0):
+        raise KernelError(f"{what}: needs a request and a vocabulary")
+    ld_draft = 0
+    if draft_logits is not None:
+        if parents is not None:
+            raise KernelError(f"{what}: drafts that were drawn are a chain (no parents)")
+        if not (draft_logits.dtype == torch.float32 and draft_logits.shape == logits.shape):
+            raise KernelError(f"{what}: draft_logits must be float32 of the logits' shape")
+        ld_draft = _rows_view(draft_logits, f"{what}: draft_logits")
+    _i32vec(tokens, T, f"{what}: tokens")
+    _i32vec(cu_seqlens, n + 1, f"{what}: cu_seqlens")
+    _i32vec(count, n, f"{what}: count")
+    if parents is not None:
+        _i32vec(parents, T, f"{what}: parents")
+    _f32vec(uniforms, T, f"{what}: uniforms")
+    _f32vec(temperature, n, f"{what}: temperature")
+    for t in (tokens_out, path):
+        _i32(t, f"{what}: tokens_out and path")
+        if not (t.dim() == 2 and t.shape[0] == n and t.shape == path.shape and t.shape[1] > 0):
+            raise KernelError(f"{what}: tokens_out and path must be int32 [requests, width]")
+    f = _fn("pmm_verify_scratch")
+    f.restype = c_longlong
+    if not (scratch.is_contiguous() and scratch.data_ptr() % 16 == 0 and scratch.numel() * scratch.element_size() >= f(T, V)):
+        raise KernelError(f"{what}: scratch comes from verify_drafts_scratch for as many rows")
+    _call("pmm_verify_drafts", logits.data_ptr(), ld, _ptr(draft_logits), ld_draft, tokens.data_ptr(), _ptr(parents), cu_seqlens.data_ptr(), n,
+          uniforms.data_ptr(), _ptr(temperature), V, T, scratch.data_ptr(), tokens_out.data_ptr(), path.data_ptr(), path.shape[1],
+          count.data_ptr(), _stream())
+
+
+def keep_accepted(rows: Tensor, pool: Tensor, slots: Tensor, cu_seqlens: Tensor, path: Tensor, count: Tensor) -> None:
+    """The kept tokens' rows into the cache pages: row cu[s] + path[s, j] of ``rows`` [layers, planes, T, width] to place
+    slots[cu[s] + j] of ``pool`` [layers, pages, planes, page_size, width], j < count[s] (`verify_drafts`, `step_tables`; both
+    may also be one layer's, without the first dimension).  Places of -1, and nodes that the request does not have, are left out.
+    ``rows`` may be a slice with strides; a row is contiguous.  What it writes, a launch directly behind may read ahead of its
+    wait: this one lets none begin early."""
+    what = "keep_accepted"
+    _same_device(what, rows, pool, slots, cu_seqlens, path, count)
+    if rows.dim() == 3 and pool.dim() == 4:
+        rows, pool = rows[None], pool[None]
+    if not (rows.dim() == 4 and pool.dim() == 5 and rows.dtype == pool.dtype and pool.is_contiguous() and rows.stride(3) == 1
+            and rows.shape[0] == pool.shape[0] and rows.shape[1] == pool.shape[2] and rows.shape[3] == pool.shape[4]):
+        raise KernelError(f"{what}: rows [layers, planes, T, width] and a contiguous pool [layers, pages, planes, page_size, width] of one type")
+    n, T = count.numel(), rows.shape[2]
+    _dt(rows)
+    _i32vec(count, n, f"{what}: count")
+    _i32vec(cu_seqlens, n + 1, f"{what}: cu_seqlens")
+    _i32(slots, f"{what}: slots")
+    _i32(path, f"{what}: path")
+    if not (slots.numel() >= T and path.dim() == 2 and path.shape[0] == n and path.shape[1] > 0 and n > 0):
+        raise KernelError(f"{what}: a place per token and a path per request")
+    if pool.shape[1] * pool.shape[3] > 0x7fffffff:
+        raise KernelError(f"{what}: places in the pool do not fit 32 bits")
+    if T == 0:
+        return
+    _call("pmm_keep_accepted", rows.data_ptr(), rows.stride(0), rows.stride(1), rows.stride(2), T, pool.data_ptr(), pool.shape[0], pool.shape[1],
+          pool.shape[2], pool.shape[3], pool.shape[4], rows.element_size(), slots.data_ptr(), cu_seqlens.data_ptr(), path.data_ptr(),
+          path.shape[1], count.data_ptr(), n, _stream())
 
 
 def l2_prefetch(tensors: Sequence[Tensor]) -> None:

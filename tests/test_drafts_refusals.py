@@ -1,0 +1,95 @@
+"""What the launchers of a drafted step's operators refuse before they touch a device (no GPU needed), and the plain forms that
+the GPU tests compare with, against formulas of their own."""
+import math
+
+import pytest
+import torch
+
+from plain import drafts_plain as P
+from poor_mans_mamba_b200.kernels import ops as K
+
+BAD = K.PMM_ERR_BAD_ARGUMENT
+A = 1 << 20  # a pointer that nothing follows
+
+
+def refused(name, good, **bad):
+    """The launcher's arguments `good` with some replaced."""
+    args = dict(good)
+    for key, value in bad.items():
+        assert key in args
+        args[key] = value
+    return K._fn(name)(*args.values()) == BAD
+
+
+TABLES = dict(held=A, new=A, blocks=A, table=A, width=8, free=A, n_free=4, n=2, page_size=64, spare=100, cu=A, seq_of=A, positions=A, slots=A,
+              cap=10, blocks_out=A, taken=A, parents=None, masks=None, words=0, stream=None)
+KEEP = dict(rows=A, ld_layer=100, ld_plane=100, ld_row=100, n_rows=4, pool=A, layers=1, pages=4, planes=2, page_size=64, width=64, item=2,
+            slots=A, cu=A, path=A, path_width=4, count=A, n=2, stream=None)
+VERIFY = dict(logits=A, ld=100, draft=None, ld_draft=0, tokens=A, parents=None, cu=A, n=2, uniforms=A, temperature=None, V=100, n_rows=4,
+              scratch=A, tokens_out=A, path=A, width=4, count=A, stream=None)
+
+
+@pytest.mark.parametrize("bad", [dict(width=0), dict(page_size=0), dict(spare=-1), dict(spare=1 << 26), dict(parents=A), dict(masks=A),
+                                 dict(parents=A, masks=A, words=0), dict(parents=A, masks=A, words=5), dict(cap=-1), dict(n_free=-1)])
+def test_step_tables_refuses(bad):
+    assert refused("pmm_step_tables", TABLES, **bad)
+
+
+@pytest.mark.parametrize("bad", [dict(pages=0), dict(page_size=0), dict(width=0), dict(item=1), dict(item=8), dict(path_width=0), dict(n_rows=-1),
+                                 dict(n=70000)])
+def test_keep_accepted_refuses(bad):
+    assert refused("pmm_keep_accepted", KEEP, **bad)
+
+
+@pytest.mark.parametrize("bad", [dict(V=0), dict(V=1 << 30), dict(n_rows=-1), dict(width=0), dict(scratch=None), dict(scratch=A + 8),
+                                 dict(draft=A, parents=A)])
+def test_verify_drafts_refuses(bad):
+    assert refused("pmm_verify_drafts", VERIFY, **bad)
+
+
+def test_tensors_of_the_host_are_refused():
+    i = torch.zeros(2, dtype=torch.int32)
+    f = torch.zeros(2, 16)
+    with pytest.raises(K.KernelError):
+        K.step_tables(i, i, i, i.view(2, 1), i, 64, 1, i, i, i, i, i, i)
+    with pytest.raises(K.KernelError):
+        K.verify_drafts(f, i, i, f[0], i.view(2, 1), i.view(2, 1), i, f)
+    with pytest.raises(K.KernelError):
+        K.keep_accepted(f[None], f.view(1, 1, 2, 16), i, i, i.view(2, 1), i)
+    with pytest.raises(K.KernelError):
+        K.tree_attention(f, f, f, f.view(1, 2, 1, 16), i.view(2, 1), i, i, f, 1, 1, 16, 1.0, f)
+
+
+# ----------------------------------------------------------------------------- the plain forms themselves
+def test_plain_verification_leaves_tokens_distributed_as_the_target():
+    """The first token of a step over many uniforms: chains from a draft and fixed proposals both leave p."""
+    g = torch.Generator().manual_seed(3)
+    V, n = 5, 4000
+    logits, draft = torch.randn(3, V, generator=g), torch.randn(3, V, generator=g)
+    p, q = torch.softmax(logits[0].double() / 0.8, 0), torch.softmax(draft[0].double() / 0.8, 0)
+    for drawn in (True, False):
+        got = torch.zeros(V)
+        for _ in range(n):
+            x = int(torch.multinomial(q, 1, generator=g))
+            u = torch.rand(3, generator=g)
+            r = P.verify(logits, [0, x, 1], [0, 3], u, 3, [0.8], None, draft if drawn else None)
+            got[r["tokens"][0][0]] += 1
+        # (a count of n draws is off by more than five of its standard deviations once in a million)
+        assert ((got / n - p).abs() <= 5 * (p * (1 - p) / n).sqrt()).all()
+
+
+def test_plain_tree_attention_of_a_chain_is_causal_attention():
+    g = torch.Generator().manual_seed(1)
+    k, v, q = torch.randn(9, 2, 16, generator=g), torch.randn(9, 2, 16, generator=g), torch.randn(9, 4, 16, generator=g)
+    out, _, _ = P.tree_attention(q[5:], k[5:], v[5:], k[:5], v[:5], torch.ones(4, 5, dtype=torch.bool), torch.ones(4, 4, dtype=torch.bool).tril(), 0.25)
+    ref = torch.nn.functional.scaled_dot_product_attention(q.double().transpose(0, 1), k.double().transpose(0, 1).repeat_interleave(2, 0),
+                                                           v.double().transpose(0, 1).repeat_interleave(2, 0), is_causal=True, scale=0.25)
+    assert (out - ref.transpose(0, 1)[5:]).abs().max() < 1e-12
+
+
+def test_plain_tables_of_a_small_step():
+    t = P.step_tables([3, 0, 8], [2, 1, 0], [1, 0, 2], [[5, 9], [9, 9], [6, 7]], [1, 2], 4, 9, 5, parents=[-1, 0, -1, -1, -1], words=1)
+    assert t["cu"] == [0, 2, 3, 3] and t["table"] == [[5, 1], [2, 9], [6, 7]] and t["blocks"] == [2, 1, 2] and t["taken"] == [2]
+    assert t["seq_of"] == [0, 0, 1, -7, -7] and t["positions"] == [3, 4, 0, -7, -7] and t["slots"] == [5 * 4 + 3, 1 * 4, 2 * 4, -7, -7]
+    assert t["masks"] == [[1], [3], [1], [-7], [-7]]
+    assert math.isclose(sum(t["cu"]), 8)
