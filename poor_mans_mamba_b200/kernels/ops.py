@@ -187,6 +187,11 @@ _SIGNATURES = {
     "pmm_tree_attention": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p,
                            c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
                            c_int, c_int, c_int, c_void_p],
+    "pmm_tree_attention_tc_supported": [c_int, c_int, c_int, c_int, c_longlong, c_int],
+    "pmm_tree_attention_scratch": [c_int],
+    "pmm_tree_attention_tc": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p,
+                              c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
+                              c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
     "pmm_verify_scratch": [c_longlong, c_int],
     "pmm_verify_drafts": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
                           c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
@@ -1647,7 +1652,7 @@ def _tc_status(device: torch.device) -> Tensor:
 
 def tc_gemm_status(device) -> int:
     """0 unless a bounded wait inside a tensor-core kernel gave up (tc_gemm: 1 producer, 2 MMA
-    issuer, 3 epilogue; attention_tc: 11..15; skinny_tc: 21..24; decode attention: 31..33).  Reading it waits for the device."""
+    issuer, 3 epilogue; attention_tc: 11..15; skinny_tc: 21..24; decode attention: 31..33; tree_attention: 41..45).  Reading it waits for the device."""
     return int(_tc_status(torch.device(device)).item())
 
 
@@ -2384,8 +2389,28 @@ def step_tables(held: Tensor, new: Tensor, blocks: Tensor, table: Tensor, free_p
 
 def tree_attention_scratch(device) -> Tensor:
     """What `tree_attention` needs beside its operands: one buffer for any number of calls on one stream at a time (two graphs
-    that may run side by side need one each).  Every call leaves its counters at zero."""
-    return torch.zeros(1, dtype=torch.float32, device=torch.device(device))
+    that may run side by side need one each); its contents do not matter."""
+    device = torch.device(device)
+    f = _fn("pmm_tree_attention_scratch")
+    f.restype = c_longlong
+    return torch.empty(int(f(_sm_count(device))), dtype=torch.float32, device=device)
+
+
+_SMS: Dict[int, int] = {}
+
+
+def _sm_count(device: torch.device) -> int:
+    index = torch.cuda.current_device() if device.index is None else device.index
+    if index not in _SMS:
+        _SMS[index] = torch.cuda.get_device_properties(index).multi_processor_count
+    return _SMS[index]
+
+
+def _tree_rows(n_q_heads: int, n_kv_heads: int, head_dim: int, T: int, n_seq: int) -> int:
+    """Rows (token, query head of a group) of a unit of the tensor-core kernel: 128 where the requests bring more than 64 on
+    average (the cached keys are then read once for twice the rows) and the head size leaves room for one block a
+    multiprocessor only; else 64."""
+    return 128 if head_dim == 128 and T * (n_q_heads // n_kv_heads) > 64 * n_seq else 64
 
 
 def _aligned_rows(t: Tensor, width: int, rows: int, what: str) -> int:
@@ -2437,8 +2462,17 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: T
     if positions is not None:
         _i32vec(positions, T, f"{what}: positions")
     _f32vec(sink, n_q_heads, f"{what}: sink")
-    if not (scratch.dtype == torch.float32 and scratch.is_contiguous()):
+    sms = _sm_count(q.device)
+    f = _fn("pmm_tree_attention_scratch")
+    f.restype = c_longlong
+    if not (scratch.dtype == torch.float32 and scratch.is_contiguous() and scratch.data_ptr() % 16 == 0 and scratch.numel() >= f(sms)):
         raise KernelError(f"{what}: scratch comes from tree_attention_scratch")
+    if q.dtype == torch.bfloat16 and _fn("pmm_tree_attention_tc_supported")(n_q_heads, n_kv_heads, head_dim, pool.shape[2], pool.shape[0], n_seq):
+        _call("pmm_tree_attention_tc", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, pool.data_ptr(), pool.shape[0],
+              block_table.data_ptr(), block_table.shape[1], held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words,
+              _ptr(sink), out.data_ptr(), float(softmax_scale), int(window), pool.shape[2], n_seq, T, n_q_heads, n_kv_heads, head_dim,
+              _tree_rows(n_q_heads, n_kv_heads, head_dim, T, n_seq), scratch.data_ptr(), sms, _tc_status(q.device).data_ptr(), _stream())
+        return
     _call("pmm_tree_attention", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, pool.data_ptr(), pool.shape[0],
           block_table.data_ptr(), block_table.shape[1], held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words,
           _ptr(sink), out.data_ptr(), float(softmax_scale), int(window), pool.shape[2], n_seq, T, n_q_heads, n_kv_heads, head_dim,
