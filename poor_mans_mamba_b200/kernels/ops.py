@@ -191,7 +191,7 @@ _SIGNATURES = {
     "pmm_tree_attention_scratch": [c_int],
     "pmm_tree_attention_tc": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p,
                               c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
-                              c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
+                              c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
     "pmm_verify_scratch": [c_longlong, c_int],
     "pmm_verify_drafts": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
                           c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
@@ -2406,13 +2406,6 @@ def _sm_count(device: torch.device) -> int:
     return _SMS[index]
 
 
-def _tree_rows(n_q_heads: int, n_kv_heads: int, head_dim: int, T: int, n_seq: int) -> int:
-    """Rows (token, query head of a group) of a unit of the tensor-core kernel: 128 where the requests bring more than 64 on
-    average (the cached keys are then read once for twice the rows) and the head size leaves room for one block a
-    multiprocessor only; else 64."""
-    return 128 if head_dim == 128 and T * (n_q_heads // n_kv_heads) > 64 * n_seq else 64
-
-
 def _aligned_rows(t: Tensor, width: int, rows: int, what: str) -> int:
     ld = _rows_view(t, what)
     if t.shape != (rows, width):
@@ -2471,7 +2464,7 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: T
         _call("pmm_tree_attention_tc", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, pool.data_ptr(), pool.shape[0],
               block_table.data_ptr(), block_table.shape[1], held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words,
               _ptr(sink), out.data_ptr(), float(softmax_scale), int(window), pool.shape[2], n_seq, T, n_q_heads, n_kv_heads, head_dim,
-              _tree_rows(n_q_heads, n_kv_heads, head_dim, T, n_seq), scratch.data_ptr(), sms, _tc_status(q.device).data_ptr(), _stream())
+              scratch.data_ptr(), sms, _tc_status(q.device).data_ptr(), _stream())
         return
     _call("pmm_tree_attention", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, pool.data_ptr(), pool.shape[0],
           block_table.data_ptr(), block_table.shape[1], held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words,
