@@ -13,25 +13,29 @@
 // keeps no draft.  Where max(p - q, 0) has no weight left (it has some in exact arithmetic), p is drawn from.
 //
 // The answers are whole numbers behind comparisons of sums over some 10^5 weights: with weights rounded to 32 bits a draw in a
-// thousand would come out differently from the formula, so weights, sums and comparisons are in 64 bits.
-// First launch: a block per (row, 4,096 entries) reads its entries once and leaves their maximum, its place and the sum of
-// exp((l - maximum) / T).  Second launch: a cluster of eight blocks per request.
+// thousand would come out differently from the formula, so weights, sums and comparisons are in 64 bits (vf_exp2: 12 operations
+// a weight, about what the 64-bit units do while the entry comes from memory).
+// First launch: a warp per (row, 1,024 entries) reads its entries once and leaves their maximum, its place and the sum of
+// exp((l - maximum) / T).  Second launch: a cluster of eight blocks per request.  A draw is one block's work: it finds the piece
+// of 1,024 by the pieces' sums and the entry in it, four entries a thread; the nodes of a tree draw side by side.  Only
+// max(p - q, 0) needs a pass over two rows, which the cluster's 64 warps share.
 #include "common.cuh"
 #include <math_constants.h>
 
 namespace pmm {
 
 constexpr int kVfThreads = 256;
-constexpr int kVfEach = 16;
-constexpr int kVfChunk = kVfThreads * kVfEach;
+constexpr int kVfWarps = kVfThreads / 32;
+constexpr int kVfEach = 32;
+constexpr int kVfChunk = 32 * kVfEach;
 constexpr int kVfCluster = 8;
-constexpr int kVfChunksMax = 1024;  // chunk sums of a row in shared memory
-constexpr int kVfStride = kVfEach + 1;  // (a thread's entries of a chunk side by side, threads in different banks)
+constexpr int kVfChunksMax = 2048;  // sums of a row's pieces in shared memory
+constexpr int kVfNodes = 64;        // nodes of a chain whose rows' sums are kept
 
-struct VfChunk {
+struct __align__(16) VfChunk {
   double sum;   // of exp((l - top) / T)
   float top;
-  int at;       // the first index that holds top
+  int at;       // the first index that holds top (only where T <= 0)
 };
 
 struct VerifyArgs {
@@ -54,117 +58,164 @@ struct VerifyArgs {
   int* count;
 };
 
-// The request that row r belongs to: how many end at or before it.  Called by the whole block.
+// 2^(y/32) for y in (-32000, 0], to 3e-15 of itself: 2^(k/32) from a table, k = round(y), times the exponential series of the rest,
+// |y - k| ln 2 / 32 <= 0.0109, up to its fifth power (the scheme of Tang, Table-driven implementation of the exponential
+// function, 1989).  y = 0 gives 1 exactly.
+__device__ __forceinline__ double vf_exp2(double y, const double* table) {
+  constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it leaves the nearest integer in the low bits
+  constexpr double kLn = 0.69314718055994530942 / 32.0;
+  const double t = y + kRound;
+  const int k = __double2loint(t);
+  const double r = y - (t - kRound);
+  double p = kLn * kLn * kLn * kLn * kLn / 120.0;
+  p = fma(p, r, kLn * kLn * kLn * kLn / 24.0);
+  p = fma(p, r, kLn * kLn * kLn / 6.0);
+  p = fma(p, r, kLn * kLn / 2.0);
+  p = fma(p, r, kLn);
+  p = fma(p, r, 1.0);
+  p *= table[k & 31];
+  return __hiloint2double(__double2hiint(p) + ((k << 15) & 0xfff00000), __double2loint(p));
+}
+__device__ __forceinline__ void vf_table(double* table) {
+  if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x * 0.03125);
+}
+// 32 log2(e) / T (temperatures below 1e-36 count as that: no product below leaves its type)
+__device__ __forceinline__ double vf_scale(float temp) { return 32.0 * 1.4426950408889634074 / fmax(static_cast<double>(temp), 1e-36); }
+
+__device__ __forceinline__ float vf_clean(float l) { return l == l ? l : -CUDART_INF_F; }
+
+// exp((l - top) / T) as the formulas above want it at infinities; top is at least l.
+__device__ __forceinline__ double vf_weight(float l, float top, double c, const double* table) {
+  if (top == CUDART_INF_F) return l == top ? 1.0 : 0.0;
+  // (beyond 2^-1000 of the largest a weight counts for nothing; a difference of infinities is no number and does not count either)
+  const bool live = (l - top) * static_cast<float>(c) > -32000.f;
+  const double w = vf_exp2((static_cast<double>(live ? l : top) - static_cast<double>(top)) * c, table);
+  return live ? w : 0.0;
+}
+
+// The request that row r belongs to: how many end at or before it.  Called by a whole warp.
 __device__ __forceinline__ int vf_request(const int* cu, int n, int r) {
   int s = 0;
-  for (int b = 0; b < n; b += kVfThreads) {
-    const int i = b + static_cast<int>(threadIdx.x);
-    const int c = __syncthreads_count(i < n && cu[i + 1] <= r);
+  for (int b = 0; b < n; b += 32) {
+    const int i = b + (threadIdx.x & 31);
+    const int c = __popc(__ballot_sync(0xffffffffu, i < n && cu[i + 1] <= r));
     s += c;
-    if (c < kVfThreads) break;
+    if (c < 32) break;
   }
   return s;
 }
 
-__device__ __forceinline__ float vf_clean(float l) { return l == l ? l : -CUDART_INF_F; }
-
-// exp((l - top) / T) as the formulas above want it at infinities.
-__device__ __forceinline__ double vf_weight(float l, float top, double inv_t) {
-  if (l == top) return top == -CUDART_INF_F ? 0.0 : 1.0;
-  if (l == -CUDART_INF_F || top == CUDART_INF_F) return 0.0;
-  return exp((static_cast<double>(l) - static_cast<double>(top)) * inv_t);
+__device__ __forceinline__ double vf_sum(double x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+// The larger of (top, at) over a warp, the lower place on ties.
+__device__ __forceinline__ void vf_top(float& top, int& at) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float ot = __shfl_xor_sync(0xffffffffu, top, o);
+    const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+    if (ot > top || (ot == top && oa < at)) {
+      top = ot;
+      at = oa;
+    }
+  }
 }
 
-__global__ void __launch_bounds__(kVfThreads) verify_stats_kernel(const VerifyArgs a) {
-  __shared__ float s_top[kVfThreads / 32];
-  __shared__ int s_at[kVfThreads / 32];
-  __shared__ double s_sum[kVfThreads / 32];
+__global__ void __launch_bounds__(kVfThreads, 4) verify_stats_kernel(const VerifyArgs a) {
+  __shared__ double s_table[32];
   pdl_launch_dependents();
+  vf_table(s_table);
+  __syncthreads();
   pdl_wait();
-  const int r = blockIdx.x / a.chunks, c = blockIdx.x % a.chunks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lane = threadIdx.x & 31;
+  const unsigned w = blockIdx.x * kVfWarps + (threadIdx.x >> 5);
+  const int r = static_cast<int>(w / a.chunks), c = static_cast<int>(w % a.chunks);
   const bool of_draft = blockIdx.y == 1;
-  if (r >= a.cu[a.n]) return;
+  if (r >= min(a.cu[a.n], a.n_rows)) return;
   const int s = vf_request(a.cu, a.n, r);
   const float temp = a.temperature ? a.temperature[s] : 0.f;
   const bool greedy = !(temp > 0.f);
   if (of_draft && (greedy || r == a.cu[s + 1] - 1)) return;  // (nothing was drafted behind a chain's last token)
-  const float* row = of_draft ? a.draft + r * a.ld_draft : a.logits + r * a.ld;
-  const int base = c * kVfChunk;
+  const int base = c * kVfChunk + lane;
+  const float* row = (of_draft ? a.draft + r * a.ld_draft : a.logits + r * a.ld) + base;
   float v[kVfEach];
+  if (c * kVfChunk + kVfChunk <= a.V) {
 #pragma unroll
-  for (int k = 0; k < kVfEach; ++k) {
-    const int i = base + k * kVfThreads + tid;
-    v[k] = i < a.V ? vf_clean(row[i]) : -CUDART_INF_F;
+    for (int k = 0; k < kVfEach; ++k) v[k] = row[k * 32];
+  } else {
+#pragma unroll
+    for (int k = 0; k < kVfEach; ++k) v[k] = base + k * 32 < a.V ? row[k * 32] : -CUDART_INF_F;
   }
-  float top = v[0];
-  int at = base + tid;
-#pragma unroll
-  for (int k = 1; k < kVfEach; ++k)
-    if (v[k] > top) {
-      top = v[k];
-      at = base + k * kVfThreads + tid;
-    }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float ot = __shfl_xor_sync(0xffffffffu, top, o);
-    const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-    if (ot > top || (ot == top && oa < at)) {
-      top = ot;
-      at = oa;
-    }
-  }
-  if (lane == 0) {
-    s_top[warp] = top;
-    s_at[warp] = at;
-  }
-  __syncthreads();
-  top = s_top[0];
-  at = s_at[0];
-#pragma unroll
-  for (int w = 1; w < kVfThreads / 32; ++w)
-    if (s_top[w] > top || (s_top[w] == top && s_at[w] < at)) {
-      top = s_top[w];
-      at = s_at[w];
-    }
+  float top = -CUDART_INF_F;
+  int at = base;
   double sum = 0.0;
-  if (!greedy) {
-    const double inv_t = 1.0 / static_cast<double>(temp);
+  if (greedy) {
 #pragma unroll
-    for (int k = 0; k < kVfEach; ++k) sum += vf_weight(v[k], top, inv_t);
+    for (int k = 0; k < kVfEach; ++k)
+      if (v[k] > top) {  // (never true of NaN)
+        top = v[k];
+        at = base + k * 32;
+      }
+    vf_top(top, at);
+  } else {
+    float low = CUDART_INF_F;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s_sum[warp] = sum;
-    __syncthreads();
-    sum = 0.0;
+    for (int k = 0; k < kVfEach; ++k) {
+      top = fmaxf(top, v[k]);  // (NaN gives way)
+      low = fminf(low, v[k]);
+    }
+    top = warp_max(top);
+    const double scale = vf_scale(temp);
+    float nan = 0.f;
 #pragma unroll
-    for (int w = 0; w < kVfThreads / 32; ++w) sum += s_sum[w];
+    for (int k = 0; k < kVfEach; ++k) nan += v[k] * 0.f;  // NaN where an entry is NaN or infinite
+    double part[2] = {0.0, 0.0};
+    if (__all_sync(0xffffffffu, nan == 0.f && (low - top) * static_cast<float>(scale) > -32000.f)) {  // every weight counts
+#pragma unroll
+      for (int k = 0; k < kVfEach; ++k)
+        part[k & 1] += vf_exp2((static_cast<double>(v[k]) - static_cast<double>(top)) * scale, s_table);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kVfEach; ++k) part[k & 1] += vf_weight(vf_clean(v[k]), top, scale, s_table);
+    }
+    sum = vf_sum(part[0] + part[1]);
   }
-  if (tid == 0) a.stats[(static_cast<size_t>(of_draft ? a.n_rows : 0) + r) * a.chunks + c] = VfChunk{sum, top, at};
+  if (lane == 0) a.stats[(static_cast<size_t>(of_draft ? a.n_rows : 0) + r) * a.chunks + c] = VfChunk{sum, top, at};
 }
 
-// A row's maximum (and its first place), and the sum of exp((l - maximum) / T) over the row, by one warp.
-__device__ __forceinline__ void vf_row(const VfChunk* st, int chunks, double inv_t, float& top, int& at, double& sum) {
+// A row's maximum (and its first place, of a greedy row), and the sum of exp((l - maximum) / T) over the row, by one warp.
+struct VfRow {
+  float top;
+  int at;
+  double sum;
+};
+__device__ __forceinline__ VfRow vf_row(const VfChunk* st, int chunks, double scale, bool greedy, const double* table) {
   const int lane = threadIdx.x & 31;
-  top = -CUDART_INF_F;
-  at = 0;
-  for (int c = lane; c < chunks; c += 32)
-    if (st[c].top > top) {
-      top = st[c].top;
-      at = st[c].at;
-    }
+  VfRow r{-CUDART_INF_F, 0, 0.0};
+  for (int b = lane; b < chunks; b += 128) {  // four loads in flight
+    VfChunk x[4];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float ot = __shfl_xor_sync(0xffffffffu, top, o);
-    const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-    if (ot > top || (ot == top && oa < at)) {
-      top = ot;
-      at = oa;
-    }
+    for (int u = 0; u < 4; ++u) x[u] = st[min(b + 32 * u, chunks - 1)];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (x[u].top > r.top) {
+        r.top = x[u].top;
+        r.at = x[u].at;
+      }
   }
-  sum = 0.0;
-  for (int c = lane; c < chunks; c += 32) sum += st[c].sum * vf_weight(st[c].top, top, inv_t);
+  vf_top(r.top, r.at);
+  if (greedy) return r;
+  for (int b = lane; b < chunks; b += 128) {
+    VfChunk x[4];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int u = 0; u < 4; ++u) x[u] = st[min(b + 32 * u, chunks - 1)];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) r.sum += b + 32 * u < chunks ? x[u].sum * vf_weight(x[u].top, r.top, scale, table) : 0.0;
+  }
+  r.sum = vf_sum(r.sum);
+  return r;
 }
 
 __device__ __forceinline__ void cluster_sync() {
@@ -172,89 +223,120 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 
-// The first index of a chunk whose running sum of weight(i) passes `target` (the last with any weight where rounding leaves none).
-// Called by the whole block; w: shared memory for the chunk's weights, scan for a double per warp.
-template <typename W>
-__device__ __forceinline__ int vf_pick(int base, int V, double target, W weight, double* w, double* scan, int* s_pick) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-#pragma unroll
-  for (int k = 0; k < kVfEach; ++k) {
-    const int i = base + k * kVfThreads + tid;
-    const int e = k * kVfThreads + tid;
-    w[e / kVfEach * kVfStride + e % kVfEach] = i < V ? weight(i) : 0.0;
-  }
-  if (tid == 0) {
-    s_pick[0] = 0x7fffffff;
-    s_pick[1] = -1;
-  }
+struct VfShared {
+  double table[32], scan[kVfWarps], left;
+  int pick, last;
+};
+
+// The whole block: sum of x.
+__device__ __forceinline__ double vf_block_sum(double x, VfShared& sh) {
+  x = vf_sum(x);
   __syncthreads();
-  double own = 0.0;
-  int last = -1;
+  if ((threadIdx.x & 31) == 0) sh.scan[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = 0.0;
 #pragma unroll
-  for (int k = 0; k < kVfEach; ++k) {
-    const double x = w[tid * kVfStride + k];
-    own += x;
-    if (x > 0.0) last = tid * kVfEach + k;
-  }
-  double run = own;
+  for (int w = 0; w < kVfWarps; ++w) x += sh.scan[w];
+  return x;
+}
+// The whole block: the first thread at which the running sum of x passes `target` (the last with any weight where rounding leaves
+// none); `target` becomes what is left of it there.
+__device__ __forceinline__ int vf_block_find(double x, double& target, VfShared& sh) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  double run = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const double up = __shfl_up_sync(0xffffffffu, run, o);
     if (lane >= o) run += up;
   }
-  if (lane == 31) scan[warp] = run;
   __syncthreads();
-  double before = run - own;
-  for (int i = 0; i < warp; ++i) before += scan[i];
-  int found = 0x7fffffff;
-  double at = before;
-  for (int k = 0; k < kVfEach; ++k) {
-    const double x = w[tid * kVfStride + k];
-    at += x;
-    if (x > 0.0 && at > target && found == 0x7fffffff) found = tid * kVfEach + k;
+  if (lane == 31) sh.scan[warp] = run;
+  if (tid == 0) {
+    sh.pick = 0x7fffffff;
+    sh.last = 0;
   }
-  if (found != 0x7fffffff) atomicMin(&s_pick[0], found);
-  if (last >= 0) atomicMax(&s_pick[1], last);
   __syncthreads();
-  return base + (s_pick[0] != 0x7fffffff ? s_pick[0] : max(s_pick[1], 0));
+  double before = 0.0;
+#pragma unroll
+  for (int w = 0; w < kVfWarps; ++w)
+    if (w < warp) before += sh.scan[w];
+  const unsigned hit = __ballot_sync(0xffffffffu, x > 0.0 && before + run > target), any = __ballot_sync(0xffffffffu, x > 0.0);
+  if (lane == 0) {
+    if (hit) atomicMin(&sh.pick, warp * 32 + __ffs(hit) - 1);
+    if (any) atomicMax(&sh.last, warp * 32 + 31 - __clz(any));
+  }
+  __syncthreads();
+  const int pick = sh.pick != 0x7fffffff ? sh.pick : sh.last;
+  if (tid == pick) sh.left = target - (before + run - x);
+  __syncthreads();
+  target = sh.left;
+  return pick;
 }
-
-// The chunk in which the running sum of part[0 .. chunks) passes `target` (the last with any weight where rounding leaves none),
-// and what of the target is left in it.  Every thread walks by itself.
-__device__ __forceinline__ int vf_chunk(const double* part, int chunks, double& target) {
-  double run = 0.0;
-  int last = 0;
-  double before_last = 0.0;
-  for (int c = 0; c < chunks; ++c) {
-    if (part[c] > 0.0) {
-      if (run + part[c] > target) {
-        target -= run;
-        return c;
-      }
-      last = c;
-      before_last = run;
+// The whole block: the first of n values part(i) (of n entries at most 256 * `each`) whose running sum passes `target`.
+template <typename P>
+__device__ __forceinline__ int vf_block_place(int n, double& target, VfShared& sh, P part) {
+  const int each = (n + kVfThreads - 1) / kVfThreads, first = static_cast<int>(threadIdx.x) * each;
+  double own = 0.0;
+  for (int i = first; i < min(n, first + each); ++i) own += part(i);
+  const int who = vf_block_find(own, target, sh);
+  if (each == 1) return who;
+  double run = 0.0, left = target;
+  int at = who * each;
+  for (int i = who * each; i < min(n, who * each + each); ++i) {  // (every thread walks them)
+    const double x = part(i);
+    if (x > 0.0) {
+      at = i;
+      left = target - run;
+      if (run + x > target) break;
     }
-    run += part[c];
+    run += x;
   }
-  target -= before_last;
-  return last;
+  target = left;
+  return at;
+}
+// The whole block: the entry of piece c whose running sum of weight(i) passes `target`.
+template <typename W>
+__device__ __forceinline__ int vf_block_entry(int c, int V, double target, VfShared& sh, W weight) {
+  constexpr int kFour = kVfChunk / kVfThreads;
+  const int first = c * kVfChunk + static_cast<int>(threadIdx.x) * kFour;
+  double x[kFour], own = 0.0;
+#pragma unroll
+  for (int k = 0; k < kFour; ++k) x[k] = first + k < V ? weight(first + k) : 0.0;
+#pragma unroll
+  for (int k = 0; k < kFour; ++k) own += x[k];
+  const int who = vf_block_find(own, target, sh);
+  if (static_cast<int>(threadIdx.x) == who) {
+    double run = 0.0;
+    int at = 0;
+    bool found = false;
+#pragma unroll
+    for (int k = 0; k < kFour; ++k) {
+      if (x[k] > 0.0 && !found) {
+        at = k;
+        found = run + x[k] > target;
+      }
+      run += x[k];
+    }
+    sh.pick = first + at;
+  }
+  __syncthreads();
+  return sh.pick;
 }
 
 __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1) verify_walk_kernel(const VerifyArgs a) {
-  __shared__ double s_w[kVfThreads * kVfStride];
   __shared__ double s_part[kVfChunksMax];
-  __shared__ double s_scan[kVfThreads / 32];
-  __shared__ int s_pick[2];
-  __shared__ float s_top[2];
-  __shared__ double s_total[2];
-  __shared__ int s_best, s_kept;
+  __shared__ VfShared sh;
+  __shared__ VfRow s_row[2][kVfNodes], s_one;
+  __shared__ int s_kept;
+  vf_table(sh.table);
+  __syncthreads();
   pdl_wait();
   const int s = blockIdx.x / kVfCluster, rank = blockIdx.x % kVfCluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int t0 = a.cu[s], t1 = min(a.cu[s + 1], a.n_rows);
   const int nodes = t1 - t0;
   const float temp = a.temperature ? a.temperature[s] : 0.f;
   const bool greedy = !(temp > 0.f);
-  const double inv_t = greedy ? 1.0 : 1.0 / static_cast<double>(temp);
+  const double scale = greedy ? 0.0 : vf_scale(temp);
   int* out = a.tokens_out + static_cast<size_t>(s) * a.width;
   int* path = a.path + static_cast<size_t>(s) * a.width;
   if (nodes <= 0) {  // (the same for the whole cluster)
@@ -265,45 +347,26 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
     return;
   }
   auto stats = [&](int r, bool of_draft) { return a.stats + (static_cast<size_t>(of_draft ? a.n_rows : 0) + r) * a.chunks; };
-  // a row's chunk sums against its maximum into s_part, maximum and total into place `k`, the place of the maximum into s_best
-  auto row_parts = [&](int r, bool of_draft, int k, bool parts) {
-    const VfChunk* st = stats(r, of_draft);
-    if (warp == 0) {
-      float top;
-      int at;
-      double sum;
-      vf_row(st, a.chunks, inv_t, top, at, sum);
-      if (lane == 0) {
-        s_top[k] = top;
-        s_total[k] = sum;
-        if (k == 0) s_best = at;
-      }
-    }
-    __syncthreads();
-    if (parts)
-      for (int c = tid; c < a.chunks; c += kVfThreads) s_part[c] = st[c].sum * vf_weight(st[c].top, s_top[k], inv_t);
-    __syncthreads();
-  };
-  // a draw from p of row r with u, by one block (-1: no token has any weight)
+  // a draw from p of row r with u, by the whole block (-1: no token has any weight)
   auto draw = [&](int r, float u) {
-    row_parts(r, false, 0, !greedy);
-    int got = s_best;
-    if (!greedy && s_total[0] > 0.0) {
-      double whole = 0.0;
-      for (int c = 0; c < a.chunks; ++c) whole += s_part[c];
-      double target = static_cast<double>(u) * whole;
-      const int c = vf_chunk(s_part, a.chunks, target);
-      const float* row = a.logits + r * a.ld;
-      const float top = s_top[0];
-      got = vf_pick(c * kVfChunk, a.V, target, [&](int i) { return vf_weight(vf_clean(row[i]), top, inv_t); }, s_w, s_scan, s_pick);
-    }
-    if (s_top[0] == -CUDART_INF_F) got = -1;
+    const VfChunk* st = stats(r, false);
     __syncthreads();
-    return got;
+    if (warp == 0) {
+      const VfRow got = vf_row(st, a.chunks, scale, greedy, sh.table);
+      if (lane == 0) s_one = got;
+    }
+    __syncthreads();
+    const VfRow one = s_one;
+    if (one.top == -CUDART_INF_F) return -1;
+    if (greedy) return one.at;
+    double target = static_cast<double>(u) * one.sum;
+    const int c = vf_block_place(a.chunks, target, sh, [&](int i) { return st[i].sum * vf_weight(st[i].top, one.top, scale, sh.table); });
+    const float* row = a.logits + r * a.ld;
+    return vf_block_entry(c, a.V, target, sh, [&](int i) { return vf_weight(vf_clean(row[i]), one.top, scale, sh.table); });
   };
 
   if (a.draft == nullptr) {
-    // ---- fixed proposals: every node's draw, the blocks of the cluster side by side; then the walk
+    // ---- fixed proposals: every node's draw, a block each; then the walk
     for (int i = rank; i < nodes; i += kVfCluster) {
       const int got = draw(t0 + i, a.uniforms[t0 + i]);
       if (tid == 0) a.drawn[t0 + i] = got;
@@ -339,75 +402,84 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
 
   // ---- a chain from a draft's distribution: which tokens are kept (every block of the cluster finds out for itself)
   const int drafted = min(nodes, a.width) - 1;
-  if (tid == 0) s_kept = drafted;
-  __syncthreads();
-  for (int i = 1 + warp; i <= drafted; i += kVfThreads / 32) {
-    const int r = t0 + i - 1, x = a.tokens[t0 + i];
-    float top, top_q = 0.f;
-    int at, at_q;
-    double sum, sum_q = 0.0;
-    vf_row(stats(r, false), a.chunks, inv_t, top, at, sum);
-    bool ok = false;
-    if (greedy) {
-      ok = at == x && top > -CUDART_INF_F;
-    } else if (x >= 0 && x < a.V) {
-      vf_row(stats(r, true), a.chunks, inv_t, top_q, at_q, sum_q);
-      const double p = vf_weight(vf_clean(a.logits[r * a.ld + x]), top, inv_t), q = vf_weight(vf_clean(a.draft[r * a.ld_draft + x]), top_q, inv_t);
-      // u q / sum_q < p / sum (a draft without weight anywhere proposes nothing that could be kept)
-      ok = sum > 0.0 && sum_q > 0.0 && static_cast<double>(a.uniforms[t0 + i]) * (q / sum_q) < p / sum;
-    }
-    if (!ok && lane == 0) atomicMin(&s_kept, i - 1);
-  }
-  __syncthreads();
-  const int kept = s_kept;
-  const int r = t0 + kept;
-  const float u = a.uniforms[t0];
-  const bool rest = !greedy && kept < drafted;   // a draft was refused: what p has more than q
-  int got = -1;
-  if (rest) {
-    row_parts(r, false, 0, false);
-    row_parts(r, true, 1, false);
-    const float* row = a.logits + r * a.ld;
-    const float* row_q = a.draft + r * a.ld_draft;
-    const float top = s_top[0], top_q = s_top[1];
-    const double inv = s_total[0] > 0.0 ? 1.0 / s_total[0] : 0.0, inv_q = s_total[1] > 0.0 ? 1.0 / s_total[1] : 0.0;
-    auto weight = [&](int i) {
-      const double p = vf_weight(vf_clean(row[i]), top, inv_t) * inv, q = vf_weight(vf_clean(row_q[i]), top_q, inv_t) * inv_q;
-      return fmax(p - q, 0.0);
-    };
-    cluster_sync();  // (every block of the cluster is there: its shared memory may be written)
-    for (int c = rank; c < a.chunks; c += kVfCluster) {
-      double sum = 0.0;
-#pragma unroll 4
-      for (int k = 0; k < kVfEach; ++k) {
-        const int i = c * kVfChunk + k * kVfThreads + tid;
-        if (i < a.V) sum += weight(i);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) s_scan[warp] = sum;
-      __syncthreads();
-      if (tid < kVfCluster) {  // the chunk's sum to every block of the cluster
-        sum = 0.0;
-        for (int w = 0; w < kVfThreads / 32; ++w) sum += s_scan[w];
-        unsigned dst;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(dst) : "r"(static_cast<unsigned>(__cvta_generic_to_shared(&s_part[c]))), "r"(tid));
-        asm volatile("st.shared::cluster.f64 [%0], %1;\n" ::"r"(dst), "d"(sum) : "memory");
-      }
-      __syncthreads();
-    }
-    cluster_sync();
-    double whole = 0.0;
-    for (int c = 0; c < a.chunks; ++c) whole += s_part[c];
-    if (whole > 0.0) {
-      double target = static_cast<double>(u) * whole;
-      const int c = vf_chunk(s_part, a.chunks, target);
-      if (c % kVfCluster != rank) return;
-      got = vf_pick(c * kVfChunk, a.V, target, weight, s_w, s_scan, s_pick);
-    } else if (rank != 0) {
-      return;
+  int kept = 0;
+  for (int first = 1; first <= drafted && kept == first - 1; first += kVfNodes) {  // (kVfNodes at a time, while all before are kept)
+    const int n = min(kVfNodes, drafted - first + 1);
+    __syncthreads();
+    if (tid == 0) s_kept = first - 1 + n;
+    // a warp a row: the target's rows and the draft's
+    for (int j = warp; j < 2 * n; j += kVfWarps) {
+      const int i = first + (j >> 1);
+      if ((j & 1) && greedy) continue;
+      const VfRow got = vf_row(stats(t0 + i - 1, j & 1), a.chunks, scale, greedy, sh.table);
+      if (lane == 0) s_row[j & 1][i - first] = got;
     }
     __syncthreads();
+    if (tid < n) {
+      const int i = first + tid, r = t0 + i - 1, x = a.tokens[t0 + i];
+      const VfRow of_p = s_row[0][tid];
+      bool ok = false;
+      if (greedy) {
+        ok = of_p.at == x && of_p.top > -CUDART_INF_F;
+      } else if (x >= 0 && x < a.V) {
+        const VfRow of_q = s_row[1][tid];
+        const double p = vf_weight(vf_clean(a.logits[r * a.ld + x]), of_p.top, scale, sh.table);
+        const double q = vf_weight(vf_clean(a.draft[r * a.ld_draft + x]), of_q.top, scale, sh.table);
+        // (a draft without weight anywhere proposes nothing that could be kept)
+        ok = of_p.sum > 0.0 && of_q.sum > 0.0 && static_cast<double>(a.uniforms[t0 + i]) * (q / of_q.sum) < p / of_p.sum;
+      }
+      if (!ok) atomicMin(&s_kept, i - 1);
+    }
+    __syncthreads();
+    kept = s_kept;
+    if (kept < first - 1 + n) break;
+  }
+  const int r = t0 + kept;
+  const float u = a.uniforms[t0];
+  int got = -1;
+  if (!greedy && kept < drafted) {  // a draft was refused: what p has more than q
+    const int j = kept % kVfNodes;  // (the refused token's place among the last ones looked at: kept + 1 = first + j)
+    const VfRow of_p = s_row[0][j], of_q = s_row[1][j];
+    const double inv = of_p.sum > 0.0 ? 1.0 / of_p.sum : 0.0, inv_q = of_q.sum > 0.0 ? 1.0 / of_q.sum : 0.0;
+    const float* row = a.logits + r * a.ld;
+    const float* row_q = a.draft + r * a.ld_draft;
+    auto more = [&](float l, float l_q) {
+      return fmax(vf_weight(vf_clean(l), of_p.top, scale, sh.table) * inv - vf_weight(vf_clean(l_q), of_q.top, scale, sh.table) * inv_q, 0.0);
+    };
+    cluster_sync();  // (every block of the cluster is there: its shared memory may be written)
+    for (int c = rank + kVfCluster * warp; c < a.chunks; c += kVfCluster * kVfWarps) {
+      double part = 0.0;
+      const int base = c * kVfChunk + lane;
+#pragma unroll
+      for (int k0 = 0; k0 < kVfEach; k0 += 16) {
+        float v[16], v_q[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const int i = base + (k0 + k) * 32;
+          v[k] = i < a.V ? row[i] : -CUDART_INF_F;
+          v_q[k] = i < a.V ? row_q[i] : -CUDART_INF_F;
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (base + (k0 + k) * 32 < a.V) part += more(v[k], v_q[k]);
+      }
+      part = vf_sum(part);
+      if (lane < kVfCluster) {  // the piece's sum to every block of the cluster
+        unsigned dst;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(dst) : "r"(static_cast<unsigned>(__cvta_generic_to_shared(&s_part[c]))), "r"(lane));
+        asm volatile("st.shared::cluster.f64 [%0], %1;\n" ::"r"(dst), "d"(part) : "memory");
+      }
+    }
+    cluster_sync();
+    if (rank != 0) return;
+    double whole = 0.0;
+    for (int c = tid; c < a.chunks; c += kVfThreads) whole += s_part[c];
+    whole = vf_block_sum(whole, sh);
+    if (whole > 0.0) {
+      double target = static_cast<double>(u) * whole;
+      const int c = vf_block_place(a.chunks, target, sh, [&](int i) { return s_part[i]; });
+      got = vf_block_entry(c, a.V, target, sh, [&](int i) { return more(row[i], row_q[i]); });
+    }
   } else if (rank != 0) {
     return;
   }
@@ -456,7 +528,7 @@ PMM_EXPORT int pmm_verify_drafts(const float* logits, long long ld, const float*
   a.width = width;
   a.count = count;
   if (n_rows > 0)
-    pmm::launch_pdl(pmm::verify_stats_kernel, dim3(chunks * n_rows, draft ? 2 : 1), dim3(pmm::kVfThreads), 0, stream, a);
+    pmm::launch_pdl(pmm::verify_stats_kernel, dim3((static_cast<unsigned>(chunks) * n_rows + pmm::kVfWarps - 1) / pmm::kVfWarps, draft ? 2 : 1), dim3(pmm::kVfThreads), 0, stream, a);
   pmm::launch_pdl(pmm::verify_walk_kernel, dim3(n * pmm::kVfCluster), dim3(pmm::kVfThreads), 0, stream, a);
   return pmm::launch_status();
 }

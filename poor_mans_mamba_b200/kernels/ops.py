@@ -2323,19 +2323,25 @@ def sample_rows(logits: Tensor, temperature: Optional[Tensor], seeds: Optional[T
 TREE_MASK_WORDS = 4  # 64-bit words of a token's mask: trees of up to 256 tokens
 
 
-def _i32vec(t: Tensor, n: int, what: str) -> None:
-    _i32(t, what)
-    if t.numel() != n:
-        raise KernelError(f"{what}: need int32 [{n}], got {tuple(t.shape)}")
+def _ints(what: str, *checks) -> None:
+    """Every (name, tensor, entries or None): contiguous int32.  (No message is put together for a call that is in order: a step
+    makes these calls layer after layer.)"""
+    for name, t, n in checks:
+        if t.dtype is not torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n):
+            raise KernelError(f"{what}: {name} must be contiguous int32" + (f" [{n}]" if n is not None else "") + f", got {t.dtype} {tuple(t.shape)}")
 
 
-def _same_device(what: str, *tensors: Optional[Tensor]) -> None:
-    """All on the current CUDA device (the launch goes to the current device's stream)."""
-    _cuda(*tensors)
-    current = torch.cuda.current_device()
+def _launch_stream(what: str, *tensors: Optional[Tensor]) -> int:
+    """The current stream's handle, all tensors being on its device."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device.index != current:
-            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{current}")
+        if t is not None and t.get_device() != index or index < 0:
+            _cuda(t)
+            raise KernelError(f"{what}: tensors are on cuda:{index} and {t.device}")
+    current = torch.cuda.current_device()
+    if index != current:
+        raise KernelError(f"{what}: the tensors are on cuda:{index}, the current device is cuda:{current}")
+    return _RAW_STREAM(index) if _RAW_STREAM is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _mask_words(mask: Tensor, rows: int, what: str) -> int:
@@ -2361,17 +2367,13 @@ def step_tables(held: Tensor, new: Tensor, blocks: Tensor, table: Tensor, free_p
     request is the token itself or above it (64 * words tokens a request; further ones have no bit).  Without: held + i.
     What it writes, a launch directly behind may read ahead of its wait: this one lets none begin early."""
     what = "step_tables"
-    _same_device(what, held, new, blocks, table, free_pages, cu, seq_of, positions, slots, blocks_out, taken, parents, masks)
+    stream = _launch_stream(what, held, new, blocks, table, free_pages, cu, seq_of, positions, slots, blocks_out, taken, parents, masks)
     n, cap = held.numel(), seq_of.numel()
-    for t, size, name in ((held, n, "held"), (new, n, "new"), (blocks, n, "blocks"), (blocks_out, n, "blocks_out"), (cu, n + 1, "cu"),
-                          (positions, cap, "positions"), (slots, cap, "slots"), (seq_of, cap, "seq_of"), (taken, 1, "taken")):
-        _i32vec(t, size, f"{what}: {name}")
-    _i32(free_pages, f"{what}: free_pages")
-    _i32(table, f"{what}: table")
-    if not (table.dim() == 2 and table.shape[0] == n and table.shape[1] > 0):
-        raise KernelError(f"{what}: table must be int32 [requests, blocks]")
-    if n == 0:
-        raise KernelError(f"{what}: needs a request")
+    _ints(what, ("held", held, n), ("new", new, n), ("blocks", blocks, n), ("blocks_out", blocks_out, n), ("cu", cu, n + 1),
+          ("seq_of", seq_of, cap), ("positions", positions, cap), ("slots", slots, cap), ("taken", taken, 1), ("free_pages", free_pages, None),
+          ("table", table, None))
+    if n == 0 or table.dim() != 2 or table.shape[0] != n or table.shape[1] == 0:
+        raise KernelError(f"{what}: table must be int32 [requests, blocks], and there must be a request")
     if blocks_out.data_ptr() == blocks.data_ptr():
         raise KernelError(f"{what}: blocks_out must not be blocks (every request reads those in front of it)")
     if page_size <= 0 or spare_page < 0 or (spare_page + 1) * page_size > 0x7fffffff:
@@ -2380,20 +2382,25 @@ def step_tables(held: Tensor, new: Tensor, blocks: Tensor, table: Tensor, free_p
     if (parents is None) != (masks is None):
         raise KernelError(f"{what}: parents and masks go together")
     if masks is not None:
-        _i32vec(parents, cap, f"{what}: parents")
+        _ints(what, ("parents", parents, cap))
         words = _mask_words(masks, cap, what)
     _call("pmm_step_tables", held.data_ptr(), new.data_ptr(), blocks.data_ptr(), table.data_ptr(), table.shape[1], free_pages.data_ptr(),
-          free_pages.numel(), n, int(page_size), int(spare_page), cu.data_ptr(), seq_of.data_ptr(), positions.data_ptr(),
-          slots.data_ptr(), cap, blocks_out.data_ptr(), taken.data_ptr(), _ptr(parents), _ptr(masks), words, _stream())
+          free_pages.numel(), n, page_size, spare_page, cu.data_ptr(), seq_of.data_ptr(), positions.data_ptr(),
+          slots.data_ptr(), cap, blocks_out.data_ptr(), taken.data_ptr(), _ptr(parents), _ptr(masks), words, stream)
 
 
 def tree_attention_scratch(device) -> Tensor:
     """What `tree_attention` needs beside its operands: one buffer for any number of calls on one stream at a time (two graphs
     that may run side by side need one each); its contents do not matter."""
     device = torch.device(device)
-    f = _fn("pmm_tree_attention_scratch")
+    return torch.empty(_sized("pmm_tree_attention_scratch", _sm_count(device)), dtype=torch.float32, device=device)
+
+
+def _sized(name: str, *args: int) -> int:
+    """What a function of the library that counts scratch says."""
+    f = _fn(name)
     f.restype = c_longlong
-    return torch.empty(int(f(_sm_count(device))), dtype=torch.float32, device=device)
+    return f(*args)
 
 
 _SMS: Dict[int, int] = {}
@@ -2406,12 +2413,13 @@ def _sm_count(device: torch.device) -> int:
     return _SMS[index]
 
 
-def _aligned_rows(t: Tensor, width: int, rows: int, what: str) -> int:
-    ld = _rows_view(t, what)
-    if t.shape != (rows, width):
-        raise KernelError(f"{what}: need [{rows}, {width}], got {tuple(t.shape)}")
+def _aligned_rows(what: str, name: str, t: Tensor, rows: int, width: int) -> int:
+    """Row stride of a [rows, width] view whose rows begin on 16-byte boundaries."""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+        raise KernelError(f"{what}: {name} must be [{rows}, {width}] with unit column stride, got {tuple(t.shape)}")
+    ld = t.stride(0)
     if t.data_ptr() % 16 or (rows > 1 and ld * t.element_size() % 16):
-        raise KernelError(f"{what}: rows must begin on 16-byte boundaries")
+        raise KernelError(f"{what}: the rows of {name} must begin on 16-byte boundaries")
     return ld
 
 
@@ -2427,56 +2435,50 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: T
     among the step's tokens the mask alone decides.  ``sink``: see `paged_attention`.
     A row that sees no key is zero; rows behind the last request (cu_seqlens[n] and further) are left as they are."""
     what = "tree_attention"
-    _same_device(what, q, k, v, pool, block_table, held, cu_seqlens, out, scratch, mask, positions, sink)
+    stream = _launch_stream(what, q, k, v, pool, block_table, held, cu_seqlens, out, scratch, mask, positions, sink)
     check_head_dim(head_dim, FLOAT_ATTENTION_MAX_HEAD)
-    if not (n_kv_heads > 0 and n_q_heads > 0 and n_q_heads % n_kv_heads == 0):
+    if n_kv_heads <= 0 or n_q_heads <= 0 or n_q_heads % n_kv_heads:
         raise KernelError(f"{what}: query heads must be a multiple of key/value heads")
-    T, n_seq = q.shape[0], held.numel()
+    T, n_seq, dtype = q.shape[0], held.numel(), q.dtype
     kv_dim = n_kv_heads * head_dim
-    ldq, ldk, ldv = (_aligned_rows(t, w, T, f"{what}: {name}") for t, w, name in
-                     ((q, n_q_heads * head_dim, "q"), (k, kv_dim, "k"), (v, kv_dim, "v")))
-    if not (q.dtype == k.dtype == v.dtype == pool.dtype == out.dtype):
+    ldq = _aligned_rows(what, "q", q, T, n_q_heads * head_dim)
+    ldk = _aligned_rows(what, "k", k, T, kv_dim)
+    ldv = _aligned_rows(what, "v", v, T, kv_dim)
+    if k.dtype is not dtype or v.dtype is not dtype or pool.dtype is not dtype or out.dtype is not dtype:
         raise KernelError(f"{what}: q, k, v, pool and out must be of one type")
-    if not (out.is_contiguous() and out.shape == (T, n_q_heads * head_dim) and out.data_ptr() % 16 == 0):
+    if not out.is_contiguous() or out.shape != q.shape or out.data_ptr() % 16:
         raise KernelError(f"{what}: out must be contiguous [T, Hq*Dh] on a 16-byte boundary")
     if not (pool.dim() == 4 and pool.shape[1] == 2 and pool.shape[3] == kv_dim and pool.is_contiguous() and pool.data_ptr() % 16 == 0
             and pool.shape[0] > 0):
         raise KernelError(f"{what}: pool must be contiguous [pages, 2, page_size, Hkv*Dh]")
-    _i32(block_table, f"{what}: block_table")
-    _i32vec(held, n_seq, f"{what}: held")
-    _i32vec(cu_seqlens, n_seq + 1, f"{what}: cu_seqlens")
+    _ints(what, ("block_table", block_table, None), ("held", held, None), ("cu_seqlens", cu_seqlens, n_seq + 1))
     if not (block_table.dim() == 2 and block_table.shape[0] == n_seq and n_seq > 0 and block_table.shape[1] > 0):
         raise KernelError(f"{what}: one row of the block table per request")
     if not softmax_scale > 0:
         raise KernelError(f"{what}: the scale must be positive")
     words = _mask_words(mask, T, what) if mask is not None else 0
-    if window != 0 and positions is None:
-        raise KernelError(f"{what}: a window needs the tokens' positions")
     if positions is not None:
-        _i32vec(positions, T, f"{what}: positions")
-    _f32vec(sink, n_q_heads, f"{what}: sink")
+        _ints(what, ("positions", positions, T))
+    elif window != 0:
+        raise KernelError(f"{what}: a window needs the tokens' positions")
+    if sink is not None:
+        _f32vec(sink, n_q_heads, "tree_attention: sink")
     sms = _sm_count(q.device)
-    f = _fn("pmm_tree_attention_scratch")
-    f.restype = c_longlong
-    if not (scratch.dtype == torch.float32 and scratch.is_contiguous() and scratch.data_ptr() % 16 == 0 and scratch.numel() >= f(sms)):
+    if not (scratch.dtype is torch.float32 and scratch.is_contiguous() and scratch.data_ptr() % 16 == 0
+            and scratch.numel() >= _sized("pmm_tree_attention_scratch", sms)):
         raise KernelError(f"{what}: scratch comes from tree_attention_scratch")
-    if q.dtype == torch.bfloat16 and _fn("pmm_tree_attention_tc_supported")(n_q_heads, n_kv_heads, head_dim, pool.shape[2], pool.shape[0], n_seq):
-        _call("pmm_tree_attention_tc", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, pool.data_ptr(), pool.shape[0],
-              block_table.data_ptr(), block_table.shape[1], held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words,
-              _ptr(sink), out.data_ptr(), float(softmax_scale), int(window), pool.shape[2], n_seq, T, n_q_heads, n_kv_heads, head_dim,
-              scratch.data_ptr(), sms, _tc_status(q.device).data_ptr(), _stream())
-        return
-    _call("pmm_tree_attention", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, pool.data_ptr(), pool.shape[0],
-          block_table.data_ptr(), block_table.shape[1], held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words,
-          _ptr(sink), out.data_ptr(), float(softmax_scale), int(window), pool.shape[2], n_seq, T, n_q_heads, n_kv_heads, head_dim,
-          _dt(q), _stream())
+    args = (q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, pool.data_ptr(), pool.shape[0], block_table.data_ptr(), block_table.shape[1],
+            held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words, _ptr(sink), out.data_ptr(), softmax_scale, window,
+            pool.shape[2], n_seq, T, n_q_heads, n_kv_heads, head_dim)
+    if dtype is torch.bfloat16 and _fn("pmm_tree_attention_tc_supported")(n_q_heads, n_kv_heads, head_dim, pool.shape[2], pool.shape[0], n_seq):
+        _call("pmm_tree_attention_tc", *args, scratch.data_ptr(), sms, _tc_status(q.device).data_ptr(), stream)
+    else:
+        _call("pmm_tree_attention", *args, _dt(q), stream)
 
 
 def verify_drafts_scratch(n_rows: int, vocab: int, device) -> Tensor:
     """Scratch of `verify_drafts` for up to ``n_rows`` rows of ``vocab`` entries (contents do not matter)."""
-    f = _fn("pmm_verify_scratch")
-    f.restype = c_longlong
-    return torch.empty(max(16, int(f(int(n_rows), int(vocab)))), dtype=torch.uint8, device=torch.device(device))
+    return torch.empty(max(16, _sized("pmm_verify_scratch", int(n_rows), int(vocab))), dtype=torch.uint8, device=torch.device(device))
 
 
 def verify_drafts(logits: Tensor, tokens: Tensor, cu_seqlens: Tensor, uniforms: Tensor, tokens_out: Tensor, path: Tensor, count: Tensor,
@@ -2494,39 +2496,35 @@ def verify_drafts(logits: Tensor, tokens: Tensor, cu_seqlens: Tensor, uniforms: 
     them.  Drafts deeper than the outputs are wide are not looked at.
     NaN logits count as -inf.  A row that holds nothing else keeps no draft and gives token 0."""
     what = "verify_drafts"
-    _same_device(what, logits, tokens, cu_seqlens, uniforms, tokens_out, path, count, scratch, temperature, parents, draft_logits)
-    if not (logits.dtype == torch.float32 and logits.dim() == 2):
-        raise KernelError(f"{what}: logits must be float32 [T, V]")
-    ld = _rows_view(logits, f"{what}: logits")
+    stream = _launch_stream(what, logits, tokens, cu_seqlens, uniforms, tokens_out, path, count, scratch, temperature, parents, draft_logits)
+    if not (logits.dtype is torch.float32 and logits.dim() == 2 and logits.stride(1) == 1):
+        raise KernelError(f"{what}: logits must be float32 [T, V] with unit column stride")
     T, V = logits.shape
     n = count.numel()
-    if not (n > 0 and V > 0):
+    if n == 0 or V == 0:
         raise KernelError(f"{what}: needs a request and a vocabulary")
     ld_draft = 0
     if draft_logits is not None:
         if parents is not None:
             raise KernelError(f"{what}: drafts that were drawn are a chain (no parents)")
-        if not (draft_logits.dtype == torch.float32 and draft_logits.shape == logits.shape):
-            raise KernelError(f"{what}: draft_logits must be float32 of the logits' shape")
-        ld_draft = _rows_view(draft_logits, f"{what}: draft_logits")
-    _i32vec(tokens, T, f"{what}: tokens")
-    _i32vec(cu_seqlens, n + 1, f"{what}: cu_seqlens")
-    _i32vec(count, n, f"{what}: count")
+        if not (draft_logits.dtype is torch.float32 and draft_logits.shape == logits.shape and draft_logits.stride(1) == 1):
+            raise KernelError(f"{what}: draft_logits must be float32 of the logits' shape with unit column stride")
+        ld_draft = draft_logits.stride(0)
+    _ints(what, ("tokens", tokens, T), ("cu_seqlens", cu_seqlens, n + 1), ("count", count, n), ("tokens_out", tokens_out, None), ("path", path, None))
     if parents is not None:
-        _i32vec(parents, T, f"{what}: parents")
-    _f32vec(uniforms, T, f"{what}: uniforms")
-    _f32vec(temperature, n, f"{what}: temperature")
-    for t in (tokens_out, path):
-        _i32(t, f"{what}: tokens_out and path")
-        if not (t.dim() == 2 and t.shape[0] == n and t.shape == path.shape and t.shape[1] > 0):
-            raise KernelError(f"{what}: tokens_out and path must be int32 [requests, width]")
-    f = _fn("pmm_verify_scratch")
-    f.restype = c_longlong
-    if not (scratch.is_contiguous() and scratch.data_ptr() % 16 == 0 and scratch.numel() * scratch.element_size() >= f(T, V)):
+        _ints(what, ("parents", parents, T))
+    if not (uniforms.dtype is torch.float32 and uniforms.is_contiguous() and uniforms.numel() == T):
+        raise KernelError(f"{what}: uniforms must be contiguous float32 [{T}]")
+    if temperature is not None and not (temperature.dtype is torch.float32 and temperature.is_contiguous() and temperature.numel() == n):
+        raise KernelError(f"{what}: temperature must be contiguous float32 [{n}]")
+    if not (path.dim() == 2 and path.shape[0] == n and path.shape[1] > 0 and tokens_out.shape == path.shape):
+        raise KernelError(f"{what}: tokens_out and path must be int32 [requests, width]")
+    if not (scratch.is_contiguous() and scratch.data_ptr() % 16 == 0
+            and scratch.numel() * scratch.element_size() >= _sized("pmm_verify_scratch", T, V)):
         raise KernelError(f"{what}: scratch comes from verify_drafts_scratch for as many rows")
-    _call("pmm_verify_drafts", logits.data_ptr(), ld, _ptr(draft_logits), ld_draft, tokens.data_ptr(), _ptr(parents), cu_seqlens.data_ptr(), n,
-          uniforms.data_ptr(), _ptr(temperature), V, T, scratch.data_ptr(), tokens_out.data_ptr(), path.data_ptr(), path.shape[1],
-          count.data_ptr(), _stream())
+    _call("pmm_verify_drafts", logits.data_ptr(), logits.stride(0), _ptr(draft_logits), ld_draft, tokens.data_ptr(), _ptr(parents),
+          cu_seqlens.data_ptr(), n, uniforms.data_ptr(), _ptr(temperature), V, T, scratch.data_ptr(), tokens_out.data_ptr(), path.data_ptr(),
+          path.shape[1], count.data_ptr(), stream)
 
 
 def keep_accepted(rows: Tensor, pool: Tensor, slots: Tensor, cu_seqlens: Tensor, path: Tensor, count: Tensor) -> None:
@@ -2536,27 +2534,26 @@ def keep_accepted(rows: Tensor, pool: Tensor, slots: Tensor, cu_seqlens: Tensor,
     ``rows`` may be a slice with strides; a row is contiguous.  What it writes, a launch directly behind may read ahead of its
     wait: this one lets none begin early."""
     what = "keep_accepted"
-    _same_device(what, rows, pool, slots, cu_seqlens, path, count)
+    stream = _launch_stream(what, rows, pool, slots, cu_seqlens, path, count)
     if rows.dim() == 3 and pool.dim() == 4:
         rows, pool = rows[None], pool[None]
-    if not (rows.dim() == 4 and pool.dim() == 5 and rows.dtype == pool.dtype and pool.is_contiguous() and rows.stride(3) == 1
-            and rows.shape[0] == pool.shape[0] and rows.shape[1] == pool.shape[2] and rows.shape[3] == pool.shape[4]):
+    if not (rows.dim() == 4 and pool.dim() == 5 and rows.dtype is pool.dtype and pool.is_contiguous()
+            and rows.shape[0] == pool.shape[0] and rows.shape[1] == pool.shape[2] and rows.shape[3] == pool.shape[4]
+            and (rows.shape[3] == 1 or rows.stride(3) == 1)):
         raise KernelError(f"{what}: rows [layers, planes, T, width] and a contiguous pool [layers, pages, planes, page_size, width] of one type")
-    n, T = count.numel(), rows.shape[2]
     _dt(rows)
-    _i32vec(count, n, f"{what}: count")
-    _i32vec(cu_seqlens, n + 1, f"{what}: cu_seqlens")
-    _i32(slots, f"{what}: slots")
-    _i32(path, f"{what}: path")
+    n, T = count.numel(), rows.shape[2]
+    _ints(what, ("count", count, None), ("cu_seqlens", cu_seqlens, n + 1), ("slots", slots, None), ("path", path, None))
     if not (slots.numel() >= T and path.dim() == 2 and path.shape[0] == n and path.shape[1] > 0 and n > 0):
         raise KernelError(f"{what}: a place per token and a path per request")
     if pool.shape[1] * pool.shape[3] > 0x7fffffff:
         raise KernelError(f"{what}: places in the pool do not fit 32 bits")
     if T == 0:
         return
-    _call("pmm_keep_accepted", rows.data_ptr(), rows.stride(0), rows.stride(1), rows.stride(2), T, pool.data_ptr(), pool.shape[0], pool.shape[1],
-          pool.shape[2], pool.shape[3], pool.shape[4], rows.element_size(), slots.data_ptr(), cu_seqlens.data_ptr(), path.data_ptr(),
-          path.shape[1], count.data_ptr(), n, _stream())
+    sl, sp, sr, _ = rows.stride()
+    layers, pages, planes, page_size, width = pool.shape
+    _call("pmm_keep_accepted", rows.data_ptr(), sl, sp, sr, T, pool.data_ptr(), layers, pages, planes, page_size, width, rows.element_size(),
+          slots.data_ptr(), cu_seqlens.data_ptr(), path.data_ptr(), path.shape[1], count.data_ptr(), n, stream)
 
 
 def l2_prefetch(tensors: Sequence[Tensor]) -> None:
