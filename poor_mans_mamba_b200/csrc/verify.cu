@@ -13,12 +13,15 @@
 // keeps no draft.  Where max(p - q, 0) has no weight left (it has some in exact arithmetic), p is drawn from.
 //
 // The answers are whole numbers behind comparisons of sums over some 10^5 weights: with weights rounded to 32 bits a draw in a
-// thousand would come out differently from the formula, so weights, sums and comparisons are in 64 bits (vf_exp2: 12 operations
-// a weight, about what the 64-bit units do while the entry comes from memory).
-// First launch: a warp per (row, 1,024 entries) reads its entries once and leaves their maximum, its place and the sum of
-// exp((l - maximum) / T).  Second launch: a cluster of eight blocks per request.  A draw is one block's work: it finds the piece
-// of 1,024 by the pieces' sums and the entry in it, four entries a thread; the nodes of a tree draw side by side.  Only
-// max(p - q, 0) needs a pass over two rows, which the cluster's 64 warps share.
+// hundred would come out differently from the formula, so what decides is in 64 bits (vf_exp2).  The 64-bit units do not keep
+// pace with memory (32 clocks a weight and warp against 23 for the bytes), so not every row goes through them:
+// First launch: a warp per (row, 1,024 entries) reads its entries once and leaves their maximum and the sum of
+// exp((l - maximum) / T); for drafts with a distribution in 32 bits (the sums are off by less than 2^-17 of themselves), for
+// fixed proposals, each node of which draws, in 64.
+// Second launch: a cluster of eight blocks per request.  With a draft's distribution, u q(x) < p(x) is decided from the first
+// launch's sums where the sides are 2^-14 apart or more, else (hardly ever) from exact sums of the two rows; then the row
+// that the next token is drawn from, and the draft's behind it, go once through the cluster's 64 warps.  A draw is one block's work:
+// it finds the piece of 1,024 by the pieces' sums and the entry in it, four entries a thread; a tree's nodes draw side by side.
 #include "common.cuh"
 #include <math_constants.h>
 
@@ -30,6 +33,7 @@ constexpr int kVfEach = 32;
 constexpr int kVfChunk = 32 * kVfEach;
 constexpr int kVfCluster = 8;
 constexpr int kVfChunksMax = 2048;  // sums of a row's pieces in shared memory
+constexpr int kVfNear = 4;          // places that a lane remembers
 constexpr int kVfNodes = 64;        // nodes of a chain whose rows' sums are kept
 
 struct __align__(16) VfChunk {
@@ -73,11 +77,21 @@ __device__ __forceinline__ double vf_exp2(double y, const double* table) {
   p = fma(p, r, kLn * kLn / 2.0);
   p = fma(p, r, kLn);
   p = fma(p, r, 1.0);
-  p *= table[k & 31];
-  return __hiloint2double(__double2hiint(p) + ((k << 15) & 0xfff00000), __double2loint(p));
+  const double power = table[k & 31];  // 2^(k % 32 / 32), less k % 32 in the place to which k is added
+  return p * __hiloint2double(__double2hiint(power) + (k << 15), __double2loint(power));
 }
+__constant__ double kVfPowers[32] = {  // 2^(k/32)
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
 __device__ __forceinline__ void vf_table(double* table) {
-  if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x * 0.03125);
+  const int j = threadIdx.x;
+  if (j < 32) table[j] = __hiloint2double(__double2hiint(kVfPowers[j]) - (j << 15), __double2loint(kVfPowers[j]));
 }
 // 32 log2(e) / T (temperatures below 1e-36 count as that: no product below leaves its type)
 __device__ __forceinline__ double vf_scale(float temp) { return 32.0 * 1.4426950408889634074 / fmax(static_cast<double>(temp), 1e-36); }
@@ -123,11 +137,27 @@ __device__ __forceinline__ void vf_top(float& top, int& at) {
   }
 }
 
+// Whether all of a lane's N entries are numbers whose weights against `top` count.
+template <int N>
+__device__ __forceinline__ bool vf_counts(const float (&v)[N], float top, float scale) {
+  float low = CUDART_INF_F, nan = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    low = fminf(low, v[k]);
+    nan = fmaf(v[k], 0.f, nan);  // NaN where an entry is NaN or infinite
+  }
+  return nan == 0.f && (low - top) * scale > -32000.f;
+}
+
+// EXACT: sums in 64 bits.
+template <bool EXACT>
 __global__ void __launch_bounds__(kVfThreads, 4) verify_stats_kernel(const VerifyArgs a) {
   __shared__ double s_table[32];
   pdl_launch_dependents();
-  vf_table(s_table);
-  __syncthreads();
+  if (EXACT) {
+    vf_table(s_table);
+    __syncthreads();
+  }
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const unsigned w = blockIdx.x * kVfWarps + (threadIdx.x >> 5);
@@ -160,27 +190,34 @@ __global__ void __launch_bounds__(kVfThreads, 4) verify_stats_kernel(const Verif
       }
     vf_top(top, at);
   } else {
-    float low = CUDART_INF_F;
 #pragma unroll
-    for (int k = 0; k < kVfEach; ++k) {
-      top = fmaxf(top, v[k]);  // (NaN gives way)
-      low = fminf(low, v[k]);
-    }
+    for (int k = 0; k < kVfEach; ++k) top = fmaxf(top, v[k]);  // (NaN gives way)
     top = warp_max(top);
     const double scale = vf_scale(temp);
-    float nan = 0.f;
+    if (top == CUDART_INF_F) {  // the infinite ones share the weight
 #pragma unroll
-    for (int k = 0; k < kVfEach; ++k) nan += v[k] * 0.f;  // NaN where an entry is NaN or infinite
-    double part[2] = {0.0, 0.0};
-    if (__all_sync(0xffffffffu, nan == 0.f && (low - top) * static_cast<float>(scale) > -32000.f)) {  // every weight counts
+      for (int k = 0; k < kVfEach; ++k) sum += v[k] == top ? 1.0 : 0.0;
+    } else if (top > -CUDART_INF_F) {
+      if (EXACT) {
+        // (what counts for nothing, NaN among it, is held where its weight, 2^-1000, leaves a sum of 1 and more as it is)
+        const float low = top - 31900.f / static_cast<float>(scale);
+        double part[2] = {0.0, 0.0};
 #pragma unroll
-      for (int k = 0; k < kVfEach; ++k)
-        part[k & 1] += vf_exp2((static_cast<double>(v[k]) - static_cast<double>(top)) * scale, s_table);
-    } else {
+        for (int k = 0; k < kVfEach; ++k)
+          part[k & 1] += vf_exp2((static_cast<double>(fmaxf(v[k], low)) - static_cast<double>(top)) * scale, s_table);
+        sum = part[0] + part[1];
+      } else {
+        const float c2 = static_cast<float>(scale * 0.03125);
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < kVfEach; ++k) part[k & 1] += vf_weight(vf_clean(v[k]), top, scale, s_table);
+        for (int k = 0; k < kVfEach; ++k) {
+          const float x = (v[k] - top) * c2;
+          part[k & 3] += x == x ? exp2f(x) : 0.f;
+        }
+        sum = (static_cast<double>(part[0]) + part[1]) + (static_cast<double>(part[2]) + part[3]);
+      }
     }
-    sum = vf_sum(part[0] + part[1]);
+    sum = vf_sum(sum);
   }
   if (lane == 0) a.stats[(static_cast<size_t>(of_draft ? a.n_rows : 0) + r) * a.chunks + c] = VfChunk{sum, top, at};
 }
@@ -191,7 +228,7 @@ struct VfRow {
   int at;
   double sum;
 };
-__device__ __forceinline__ VfRow vf_row(const VfChunk* st, int chunks, double scale, bool greedy, const double* table) {
+__device__ __noinline__ VfRow vf_row(const VfChunk* st, int chunks, double scale, bool greedy, const double* table) {
   const int lane = threadIdx.x & 31;
   VfRow r{-CUDART_INF_F, 0, 0.0};
   for (int b = lane; b < chunks; b += 128) {  // four loads in flight
@@ -241,7 +278,7 @@ __device__ __forceinline__ double vf_block_sum(double x, VfShared& sh) {
 }
 // The whole block: the first thread at which the running sum of x passes `target` (the last with any weight where rounding leaves
 // none); `target` becomes what is left of it there.
-__device__ __forceinline__ int vf_block_find(double x, double& target, VfShared& sh) {
+__device__ __noinline__ int vf_block_find(double x, double& target, VfShared& sh) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   double run = x;
 #pragma unroll
@@ -324,10 +361,10 @@ __device__ __forceinline__ int vf_block_entry(int c, int V, double target, VfSha
 }
 
 __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1) verify_walk_kernel(const VerifyArgs a) {
-  __shared__ double s_part[kVfChunksMax];
+  extern __shared__ double s_part[];  // [4][chunks]: a piece's weight in p and in q, and the same of the entries with more in p than in q
   __shared__ VfShared sh;
   __shared__ VfRow s_row[2][kVfNodes], s_one;
-  __shared__ int s_kept;
+  __shared__ int s_kept, s_ok[kVfNodes];
   vf_table(sh.table);
   __syncthreads();
   pdl_wait();
@@ -401,6 +438,126 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
   }
 
   // ---- a chain from a draft's distribution: which tokens are kept (every block of the cluster finds out for itself)
+  // Row r of the target (and the draft's, `both`) once through all warps of the cluster: the pieces' weights in s_part of every block,
+  // and the weights of the entries with more in p than in q in s_part of the block that took the piece.  The sums at hand tell which
+  // those are but for the entries where p and q are within 2^-15 of one another: a lane remembers their places (`settle`).
+  int near[kVfNear], n_near = 0;
+  auto send = [&](int which, int c, double x) {  // to block lane % 8 of the cluster
+    unsigned dst;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n"
+                 : "=r"(dst)
+                 : "r"(static_cast<unsigned>(__cvta_generic_to_shared(s_part + which * a.chunks + c))), "r"(lane & (kVfCluster - 1)));
+    asm volatile("st.shared::cluster.f64 [%0], %1;\n" ::"r"(dst), "d"(x) : "memory");
+  };
+  auto pass = [&](int r, const VfRow of_p, const VfRow of_q, bool both) {
+    const float* row = a.logits + r * a.ld;
+    const float* row_q = a.draft + r * a.ld_draft;
+    const float scale_f = static_cast<float>(scale);
+    const double inv = of_p.sum > 0.0 ? 1.0 / of_p.sum : 0.0, inv_q = of_q.sum > 0.0 ? 1.0 / of_q.sum : 0.0;
+    n_near = 0;
+    cluster_sync();  // (every block of the cluster is there, and done with what it held)
+    for (int c = rank + kVfCluster * warp; c < a.chunks; c += kVfCluster * kVfWarps) {
+      double sum_p = 0.0, sum_q = 0.0, more_p = 0.0, more_q = 0.0;
+      const int base = c * kVfChunk + lane;
+      float v[8], v_q[8], w[8], w_q[8];  // eight entries of both rows, and the next eight on their way
+      auto fetch = [&](int k0, float (&x)[8], float (&y)[8]) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int i = base + (k0 + k) * 32;
+          x[k] = i < a.V ? row[i] : -CUDART_INF_F;
+          y[k] = both && i < a.V ? row_q[i] : -CUDART_INF_F;
+        }
+      };
+      auto add = [&](int i, double p, double q) {
+        sum_p += p;
+        sum_q += q;
+        const double in_p = p * inv, more = in_p - q * inv_q;
+        if (fabs(more) < 0x1p-15 * in_p) {
+#pragma unroll
+          for (int u = kVfNear - 1; u > 0; --u) near[u] = near[u - 1];
+          near[0] = i;
+          ++n_near;
+        } else if (more > 0.0) {
+          more_p += p;
+          more_q += q;
+        }
+      };
+      auto take = [&](int k0, const float (&x)[8], const float (&y)[8]) {
+        const bool fine = vf_counts<8>(x, of_p.top, scale_f) && (!both || vf_counts<8>(y, of_q.top, scale_f));
+        if (!__all_sync(0xffffffffu, fine)) {
+#pragma unroll 1
+          for (int i = base + k0 * 32; i < min(a.V, base + (k0 + 8) * 32); i += 32)
+            add(i, vf_weight(vf_clean(row[i]), of_p.top, scale, sh.table), both ? vf_weight(vf_clean(row_q[i]), of_q.top, scale, sh.table) : 0.0);
+        } else if (both) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            add(base + (k0 + k) * 32, vf_exp2((static_cast<double>(x[k]) - static_cast<double>(of_p.top)) * scale, sh.table),
+                vf_exp2((static_cast<double>(y[k]) - static_cast<double>(of_q.top)) * scale, sh.table));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sum_p += vf_exp2((static_cast<double>(x[k]) - static_cast<double>(of_p.top)) * scale, sh.table);
+        }
+      };
+      fetch(0, v, v_q);
+#pragma unroll 1
+      for (int k0 = 0; k0 < kVfEach; k0 += 16) {
+        fetch(k0 + 8, w, w_q);
+        take(k0, v, v_q);
+        if (k0 + 16 < kVfEach) fetch(k0 + 16, v, v_q);
+        take(k0 + 8, w, w_q);
+      }
+      sum_p = vf_sum(sum_p);
+      if (both) {
+        sum_q = vf_sum(sum_q);
+        more_p = vf_sum(more_p);
+        more_q = vf_sum(more_q);
+      }
+      if (lane < 2 * kVfCluster) send(lane / kVfCluster, c, lane / kVfCluster == 0 ? sum_p : sum_q);
+      if (lane == 0) {
+        s_part[2 * a.chunks + c] = more_p;
+        s_part[3 * a.chunks + c] = more_q;
+      }
+    }
+    cluster_sync();
+  };
+  // The entries that were too near to tell, with the exact sums behind inv and inv_q; then the last two of s_part are in every block.
+  auto settle = [&](int r, const VfRow of_p, const VfRow of_q, double inv, double inv_q) {
+    const float* row = a.logits + r * a.ld;
+    const float* row_q = a.draft + r * a.ld_draft;
+    const bool lost = __any_sync(0xffffffffu, n_near > kVfNear);  // (more places than a lane remembers: the pieces once more)
+    for (int c = rank + kVfCluster * warp; c < a.chunks; c += kVfCluster * kVfWarps) {
+      double more_p = 0.0, more_q = 0.0;
+      auto add = [&](int i) {
+        const double p = vf_weight(vf_clean(row[i]), of_p.top, scale, sh.table), q = vf_weight(vf_clean(row_q[i]), of_q.top, scale, sh.table);
+        if (p * inv > q * inv_q) {
+          more_p += p;
+          more_q += q;
+        }
+      };
+      if (lost) {
+#pragma unroll 1
+        for (int i = c * kVfChunk + lane; i < min(a.V, c * kVfChunk + kVfChunk); i += 32) add(i);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kVfNear; ++u)
+          if (u < n_near && near[u] / kVfChunk == c) add(near[u]);
+      }
+      more_p = vf_sum(more_p);
+      more_q = vf_sum(more_q);
+      if (!lost) {
+        more_p += s_part[2 * a.chunks + c];
+        more_q += s_part[3 * a.chunks + c];
+      }
+      __syncwarp();
+      if (lane < 2 * kVfCluster) send(2 + lane / kVfCluster, c, lane / kVfCluster == 0 ? more_p : more_q);
+    }
+    cluster_sync();
+  };
+  auto total = [&](int which) {
+    double x = 0.0;
+    for (int c = tid; c < a.chunks; c += kVfThreads) x += s_part[which * a.chunks + c];
+    return vf_block_sum(x, sh);
+  };
   const int drafted = min(nodes, a.width) - 1;
   int kept = 0;
   for (int first = 1; first <= drafted && kept == first - 1; first += kVfNodes) {  // (kVfNodes at a time, while all before are kept)
@@ -418,7 +575,7 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
     if (tid < n) {
       const int i = first + tid, r = t0 + i - 1, x = a.tokens[t0 + i];
       const VfRow of_p = s_row[0][tid];
-      bool ok = false;
+      int ok = 0;
       if (greedy) {
         ok = of_p.at == x && of_p.top > -CUDART_INF_F;
       } else if (x >= 0 && x < a.V) {
@@ -426,64 +583,86 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
         const double p = vf_weight(vf_clean(a.logits[r * a.ld + x]), of_p.top, scale, sh.table);
         const double q = vf_weight(vf_clean(a.draft[r * a.ld_draft + x]), of_q.top, scale, sh.table);
         // (a draft without weight anywhere proposes nothing that could be kept)
-        ok = of_p.sum > 0.0 && of_q.sum > 0.0 && static_cast<double>(a.uniforms[t0 + i]) * (q / of_q.sum) < p / of_p.sum;
+        if (of_p.sum > 0.0 && of_q.sum > 0.0) {
+          const double left = static_cast<double>(a.uniforms[t0 + i]) * q * of_p.sum, right = p * of_q.sum;
+          ok = left < right;
+          if (fabs(left - right) <= 0x1p-14 * right) ok = 2;
+        }
       }
-      if (!ok) atomicMin(&s_kept, i - 1);
+      s_ok[tid] = ok;
+      if (ok != 1) atomicMin(&s_kept, i - 1);
     }
     __syncthreads();
     kept = s_kept;
+    while (kept < first - 1 + n && s_ok[kept + 1 - first] == 2) {  // too near to tell: by exact sums (the same for the whole cluster)
+      const int j = kept + 1 - first, r = t0 + kept, x = a.tokens[t0 + kept + 1];
+      pass(r, s_row[0][j], s_row[1][j], true);
+      const double p = vf_weight(vf_clean(a.logits[r * a.ld + x]), s_row[0][j].top, scale, sh.table);
+      const double q = vf_weight(vf_clean(a.draft[r * a.ld_draft + x]), s_row[1][j].top, scale, sh.table);
+      if (!(static_cast<double>(a.uniforms[t0 + kept + 1]) * q * total(0) < p * total(1))) break;
+      do ++kept;
+      while (kept < first - 1 + n && s_ok[kept + 1 - first] == 1);
+    }
     if (kept < first - 1 + n) break;
   }
   const int r = t0 + kept;
-  const float u = a.uniforms[t0];
   int got = -1;
-  if (!greedy && kept < drafted) {  // a draft was refused: what p has more than q
-    const int j = kept % kVfNodes;  // (the refused token's place among the last ones looked at: kept + 1 = first + j)
-    const VfRow of_p = s_row[0][j], of_q = s_row[1][j];
-    const double inv = of_p.sum > 0.0 ? 1.0 / of_p.sum : 0.0, inv_q = of_q.sum > 0.0 ? 1.0 / of_q.sum : 0.0;
+  if (greedy) {
+    if (rank != 0) return;
+    if (warp == 0) {
+      const VfRow one = vf_row(stats(r, false), a.chunks, scale, true, sh.table);
+      if (lane == 0) s_one = one;
+    }
+    __syncthreads();
+    got = s_one.at;
+  } else {
+    const bool rest = kept < drafted;  // a draft was refused: what p has more than q
+    VfRow of_p, of_q{};
+    if (rest) {
+      of_p = s_row[0][kept % kVfNodes];  // (the refused token's place among the last ones looked at)
+      of_q = s_row[1][kept % kVfNodes];
+    } else {
+      __syncthreads();
+      if (warp == 0) {
+        const VfRow one = vf_row(stats(r, false), a.chunks, scale, false, sh.table);
+        if (lane == 0) s_one = one;
+      }
+      __syncthreads();
+      of_p = s_one;
+    }
+    pass(r, of_p, of_q, rest);
+    const double sum = total(0);
+    double inv = 0.0, inv_q = 0.0;
+    if (rest) {
+      const double sum_q = total(1);
+      inv = sum > 0.0 ? 1.0 / sum : 0.0;
+      inv_q = sum_q > 0.0 ? 1.0 / sum_q : 0.0;
+      settle(r, of_p, of_q, inv, inv_q);
+    }
+    if (rank != 0) return;
     const float* row = a.logits + r * a.ld;
     const float* row_q = a.draft + r * a.ld_draft;
-    auto more = [&](float l, float l_q) {
-      return fmax(vf_weight(vf_clean(l), of_p.top, scale, sh.table) * inv - vf_weight(vf_clean(l_q), of_q.top, scale, sh.table) * inv_q, 0.0);
-    };
-    cluster_sync();  // (every block of the cluster is there: its shared memory may be written)
-    for (int c = rank + kVfCluster * warp; c < a.chunks; c += kVfCluster * kVfWarps) {
-      double part = 0.0;
-      const int base = c * kVfChunk + lane;
-#pragma unroll
-      for (int k0 = 0; k0 < kVfEach; k0 += 16) {
-        float v[16], v_q[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const int i = base + (k0 + k) * 32;
-          v[k] = i < a.V ? row[i] : -CUDART_INF_F;
-          v_q[k] = i < a.V ? row_q[i] : -CUDART_INF_F;
-        }
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (base + (k0 + k) * 32 < a.V) part += more(v[k], v_q[k]);
-      }
-      part = vf_sum(part);
-      if (lane < kVfCluster) {  // the piece's sum to every block of the cluster
-        unsigned dst;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(dst) : "r"(static_cast<unsigned>(__cvta_generic_to_shared(&s_part[c]))), "r"(lane));
-        asm volatile("st.shared::cluster.f64 [%0], %1;\n" ::"r"(dst), "d"(part) : "memory");
+    const double u = static_cast<double>(a.uniforms[t0]);
+    if (rest) {
+      auto piece = [&](int c) { return fmax(s_part[2 * a.chunks + c] * inv - s_part[3 * a.chunks + c] * inv_q, 0.0); };
+      double whole = 0.0;
+      for (int c = tid; c < a.chunks; c += kVfThreads) whole += piece(c);
+      whole = vf_block_sum(whole, sh);
+      if (whole > 0.0) {
+        double target = u * whole;
+        const int c = vf_block_place(a.chunks, target, sh, piece);
+        got = vf_block_entry(c, a.V, target, sh, [&](int i) {
+          return fmax(vf_weight(vf_clean(row[i]), of_p.top, scale, sh.table) * inv - vf_weight(vf_clean(row_q[i]), of_q.top, scale, sh.table) * inv_q, 0.0);
+        });
       }
     }
-    cluster_sync();
-    if (rank != 0) return;
-    double whole = 0.0;
-    for (int c = tid; c < a.chunks; c += kVfThreads) whole += s_part[c];
-    whole = vf_block_sum(whole, sh);
-    if (whole > 0.0) {
-      double target = static_cast<double>(u) * whole;
+    if (got < 0 && sum > 0.0) {
+      double target = u * sum;
       const int c = vf_block_place(a.chunks, target, sh, [&](int i) { return s_part[i]; });
-      got = vf_block_entry(c, a.V, target, sh, [&](int i) { return more(row[i], row_q[i]); });
+      got = vf_block_entry(c, a.V, target, sh, [&](int i) { return vf_weight(vf_clean(row[i]), of_p.top, scale, sh.table); });
     }
-  } else if (rank != 0) {
-    return;
+    got = max(got, 0);
   }
-  if (got < 0) got = max(draw(r, u), 0);
   for (int j = tid; j < a.width; j += kVfThreads) {
     out[j] = j < kept ? a.tokens[t0 + j + 1] : j == kept ? got : -1;
     path[j] = j <= kept ? j : -1;
@@ -504,7 +683,7 @@ PMM_EXPORT int pmm_verify_drafts(const float* logits, long long ld, const float*
                                  int* tokens_out, int* path, int width, int* count, cudaStream_t stream) {
   if (n <= 0) return 0;
   const int chunks = V > 0 ? (V + pmm::kVfChunk - 1) / pmm::kVfChunk : 0;
-  if (V <= 0 || chunks > pmm::kVfChunksMax || n_rows < 0 || static_cast<long long>(n_rows) * chunks > 0x7fffffffll || width <= 0 || !scratch || reinterpret_cast<uintptr_t>(scratch) % 16 ||
+  if (V <= 0 || chunks > pmm::kVfChunksMax || n_rows < 0 || static_cast<long long>(n_rows) * chunks > 0x3fffffffll || width <= 0 || !scratch || reinterpret_cast<uintptr_t>(scratch) % 16 ||
       (draft && parents) || n > 0x7fffffff / pmm::kVfCluster)
     return PMM_ERR_BAD_ARGUMENT;
   pmm::VerifyArgs a{};
@@ -527,8 +706,14 @@ PMM_EXPORT int pmm_verify_drafts(const float* logits, long long ld, const float*
   a.path = path;
   a.width = width;
   a.count = count;
+  const unsigned blocks = (static_cast<unsigned>(chunks) * n_rows + pmm::kVfWarps - 1) / pmm::kVfWarps;
   if (n_rows > 0)
-    pmm::launch_pdl(pmm::verify_stats_kernel, dim3((static_cast<unsigned>(chunks) * n_rows + pmm::kVfWarps - 1) / pmm::kVfWarps, draft ? 2 : 1), dim3(pmm::kVfThreads), 0, stream, a);
-  pmm::launch_pdl(pmm::verify_walk_kernel, dim3(n * pmm::kVfCluster), dim3(pmm::kVfThreads), 0, stream, a);
+    pmm::launch_pdl(draft ? pmm::verify_stats_kernel<false> : pmm::verify_stats_kernel<true>, dim3(blocks, draft ? 2 : 1), dim3(pmm::kVfThreads), 0, stream, a);
+  const size_t smem = draft ? 4 * static_cast<size_t>(chunks) * sizeof(double) : 0;
+  if (smem > 16 * 1024) {  // (a vocabulary of half a million; attributes hold for the current device: set at every call)
+    const cudaError_t e = cudaFuncSetAttribute(pmm::verify_walk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  pmm::launch_pdl(pmm::verify_walk_kernel, dim3(n * pmm::kVfCluster), dim3(pmm::kVfThreads), smem, stream, a);
   return pmm::launch_status();
 }

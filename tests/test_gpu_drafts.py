@@ -449,6 +449,30 @@ def test_verify_drafts_borders():
     assert verify(logits, [0, 9, 9, 9], [4], torch.full((T,), 2.0 ** -14), 4, [1.0], None, draft)["count"] == [4]
 
 
+@pytest.mark.parametrize("near", [0.0, 1e-7, 1e-5, 1e-3])
+@pytest.mark.parametrize("bump", [0.0, 1e-6, 0.05, 3.0])
+def test_verify_drafts_of_a_draft_that_is_almost_the_target(near, bump):
+    """p and q apart by less than their sums are known to at first, at all entries or at a few, with and without tokens that one
+    of them likes better; drafted tokens that p likes less, and uniforms close to the border of being kept."""
+    V, lens, temps = 20000, [3, 3, 3, 3, 3, 3], [1.0, 0.7, 1.0, 1.5, 1.0, 0.9]
+    g = torch.Generator().manual_seed(7)
+    T = sum(lens)
+    logits = torch.randn(T, V, generator=g) * 2
+    draft = logits + near * torch.randn(T, V, generator=g)
+    logits[:, 17::1000] += bump
+    draft[:, [5, 11000]] += bump
+    tokens = [5, 11000, 17] * 6
+    p, q = (torch.softmax(x.double() / torch.tensor(temps, dtype=torch.float64).repeat_interleave(3)[:, None], 1) for x in (logits, draft))
+    u = torch.rand(T, generator=g)
+    for t in range(T):
+        if t % 3:  # on the border of p / q, a float32 step or two to either side
+            ratio = float(p[t - 1, tokens[t]] / q[t - 1, tokens[t]])
+            u[t] = min(max(ratio + (t % 5 - 2) * 6e-8, 0.0), 1 - 2.0 ** -24)
+    verify(logits.to(DEV), tokens, lens, u, 3, temps, None, draft.to(DEV))
+    u[1::3] = 1 - 2.0 ** -24
+    verify(logits.to(DEV), tokens, lens, u, 3, temps, None, draft.to(DEV))
+
+
 @pytest.mark.parametrize("mode", ["chain", "drawn", "tree"])
 @pytest.mark.parametrize("V", [50, 9000])
 def test_verify_drafts_infinities(mode, V):
