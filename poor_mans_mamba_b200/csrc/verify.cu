@@ -18,7 +18,7 @@
 // First launch: a warp per (row, 1,024 entries) reads its entries once and leaves their maximum and the sum of
 // exp((l - maximum) / T); for drafts with a distribution in 32 bits (the sums are off by less than 2^-17 of themselves), for
 // fixed proposals, each node of which draws, in 64.
-// Second launch: a cluster of eight blocks per request.  With a draft's distribution, u q(x) < p(x) is decided from the first
+// Second launch: a cluster of up to eight blocks per request.  With a draft's distribution, u q(x) < p(x) is decided from the first
 // launch's sums where the sides are 2^-14 apart or more, else (hardly ever) from exact sums of the two rows; then the row
 // that the next token is drawn from, and the draft's behind it, go once through the cluster's 64 warps.  A draw is one block's work:
 // it finds the piece of 1,024 by the pieces' sums and the entry in it, four entries a thread; a tree's nodes draw side by side.
@@ -31,8 +31,9 @@ constexpr int kVfThreads = 256;
 constexpr int kVfWarps = kVfThreads / 32;
 constexpr int kVfEach = 32;
 constexpr int kVfChunk = 32 * kVfEach;
-constexpr int kVfCluster = 8;
+constexpr int kVfCluster = 8;       // blocks of a cluster at most
 constexpr int kVfChunksMax = 2048;  // sums of a row's pieces in shared memory
+constexpr int kVfStep = 4;          // entries of a row that a lane takes at a time in the second launch
 constexpr int kVfNear = 4;          // places that a lane remembers
 constexpr int kVfNodes = 64;        // nodes of a chain whose rows' sums are kept
 
@@ -60,6 +61,7 @@ struct VerifyArgs {
   int* path;
   int width;
   int* count;
+  int cluster;              // blocks that share a request
 };
 
 // 2^(y/32) for y in (-32000, 0], to 3e-15 of itself: 2^(k/32) from a table, k = round(y), times the exponential series of the rest,
@@ -98,13 +100,13 @@ __device__ __forceinline__ double vf_scale(float temp) { return 32.0 * 1.4426950
 
 __device__ __forceinline__ float vf_clean(float l) { return l == l ? l : -CUDART_INF_F; }
 
-// exp((l - top) / T) as the formulas above want it at infinities; top is at least l.
+// exp((l - top) / T) as the formulas above want it at infinities; top is at least l.  (No branches: several of them run side by
+// side, a chain of dependent 64-bit operations each.)
 __device__ __forceinline__ double vf_weight(float l, float top, double c, const double* table) {
-  if (top == CUDART_INF_F) return l == top ? 1.0 : 0.0;
   // (beyond 2^-1000 of the largest a weight counts for nothing; a difference of infinities is no number and does not count either)
   const bool live = (l - top) * static_cast<float>(c) > -32000.f;
-  const double w = vf_exp2((static_cast<double>(live ? l : top) - static_cast<double>(top)) * c, table);
-  return live ? w : 0.0;
+  const double w = vf_exp2((static_cast<double>(live ? l : 0.f) - static_cast<double>(live ? top : 0.f)) * c, table);
+  return live ? w : top == CUDART_INF_F && l == top ? 1.0 : 0.0;
 }
 
 // The request that row r belongs to: how many end at or before it.  Called by a whole warp.
@@ -360,7 +362,7 @@ __device__ __forceinline__ int vf_block_entry(int c, int V, double target, VfSha
   return sh.pick;
 }
 
-__global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1) verify_walk_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kVfThreads, 2) verify_walk_kernel(const VerifyArgs a) {
   extern __shared__ double s_part[];  // [4][chunks]: a piece's weight in p and in q, and the same of the entries with more in p than in q
   __shared__ VfShared sh;
   __shared__ VfRow s_row[2][kVfNodes], s_one;
@@ -368,7 +370,7 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
   vf_table(sh.table);
   __syncthreads();
   pdl_wait();
-  const int s = blockIdx.x / kVfCluster, rank = blockIdx.x % kVfCluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int cluster = a.cluster, s = blockIdx.x / cluster, rank = blockIdx.x % cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int t0 = a.cu[s], t1 = min(a.cu[s + 1], a.n_rows);
   const int nodes = t1 - t0;
   const float temp = a.temperature ? a.temperature[s] : 0.f;
@@ -404,7 +406,7 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
 
   if (a.draft == nullptr) {
     // ---- fixed proposals: every node's draw, a block each; then the walk
-    for (int i = rank; i < nodes; i += kVfCluster) {
+    for (int i = rank; i < nodes; i += cluster) {
       const int got = draw(t0 + i, a.uniforms[t0 + i]);
       if (tid == 0) a.drawn[t0 + i] = got;
     }
@@ -442,11 +444,11 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
   // and the weights of the entries with more in p than in q in s_part of the block that took the piece.  The sums at hand tell which
   // those are but for the entries where p and q are within 2^-15 of one another: a lane remembers their places (`settle`).
   int near[kVfNear], n_near = 0;
-  auto send = [&](int which, int c, double x) {  // to block lane % 8 of the cluster
+  auto send = [&](int which, int c, double x) {  // to block lane % cluster
     unsigned dst;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n"
                  : "=r"(dst)
-                 : "r"(static_cast<unsigned>(__cvta_generic_to_shared(s_part + which * a.chunks + c))), "r"(lane & (kVfCluster - 1)));
+                 : "r"(static_cast<unsigned>(__cvta_generic_to_shared(s_part + which * a.chunks + c))), "r"(lane % cluster));
     asm volatile("st.shared::cluster.f64 [%0], %1;\n" ::"r"(dst), "d"(x) : "memory");
   };
   auto pass = [&](int r, const VfRow of_p, const VfRow of_q, bool both) {
@@ -456,55 +458,85 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
     const double inv = of_p.sum > 0.0 ? 1.0 / of_p.sum : 0.0, inv_q = of_q.sum > 0.0 ? 1.0 / of_q.sum : 0.0;
     n_near = 0;
     cluster_sync();  // (every block of the cluster is there, and done with what it held)
-    for (int c = rank + kVfCluster * warp; c < a.chunks; c += kVfCluster * kVfWarps) {
+    for (int c = rank + cluster * warp; c < a.chunks; c += cluster * kVfWarps) {
       double sum_p = 0.0, sum_q = 0.0, more_p = 0.0, more_q = 0.0;
       const int base = c * kVfChunk + lane;
-      float v[8], v_q[8], w[8], w_q[8];  // eight entries of both rows, and the next eight on their way
-      auto fetch = [&](int k0, float (&x)[8], float (&y)[8]) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int i = base + (k0 + k) * 32;
-          x[k] = i < a.V ? row[i] : -CUDART_INF_F;
-          y[k] = both && i < a.V ? row_q[i] : -CUDART_INF_F;
-        }
-      };
-      auto add = [&](int i, double p, double q) {
+      // what an entry adds; whether p and q are too near to tell which is more there
+      auto add = [&](double p, double q) {
         sum_p += p;
         sum_q += q;
-        const double in_p = p * inv, more = in_p - q * inv_q;
-        if (fabs(more) < 0x1p-15 * in_p) {
-#pragma unroll
-          for (int u = kVfNear - 1; u > 0; --u) near[u] = near[u - 1];
-          near[0] = i;
-          ++n_near;
-        } else if (more > 0.0) {
-          more_p += p;
-          more_q += q;
-        }
+        const double in_p = p * inv, more = fma(-q, inv_q, in_p);
+        // |more| < 2^-15 in_p, by the halves that hold the exponents
+        const bool tied = (__double2hiint(more) & 0x7fffffff) < __double2hiint(in_p) - (15 << 20);
+        const bool take = !tied && __double2hiint(more) > 0;
+        more_p += take ? p : 0.0;
+        more_q += take ? q : 0.0;
+        return tied;
       };
-      auto take = [&](int k0, const float (&x)[8], const float (&y)[8]) {
-        const bool fine = vf_counts<8>(x, of_p.top, scale_f) && (!both || vf_counts<8>(y, of_q.top, scale_f));
-        if (!__all_sync(0xffffffffu, fine)) {
-#pragma unroll 1
-          for (int i = base + k0 * 32; i < min(a.V, base + (k0 + 8) * 32); i += 32)
-            add(i, vf_weight(vf_clean(row[i]), of_p.top, scale, sh.table), both ? vf_weight(vf_clean(row_q[i]), of_q.top, scale, sh.table) : 0.0);
-        } else if (both) {
+      auto remember = [&](int i) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            add(base + (k0 + k) * 32, vf_exp2((static_cast<double>(x[k]) - static_cast<double>(of_p.top)) * scale, sh.table),
-                vf_exp2((static_cast<double>(y[k]) - static_cast<double>(of_q.top)) * scale, sh.table));
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) sum_p += vf_exp2((static_cast<double>(x[k]) - static_cast<double>(of_p.top)) * scale, sh.table);
-        }
+        for (int u = kVfNear - 1; u > 0; --u) near[u] = near[u - 1];
+        near[0] = i;
+        ++n_near;
       };
-      fetch(0, v, v_q);
+      auto slow = [&](int first, int n) {
 #pragma unroll 1
-      for (int k0 = 0; k0 < kVfEach; k0 += 16) {
-        fetch(k0 + 8, w, w_q);
-        take(k0, v, v_q);
-        if (k0 + 16 < kVfEach) fetch(k0 + 16, v, v_q);
-        take(k0 + 8, w, w_q);
+        for (int i = first; i < min(a.V, first + n * 32); i += 32)
+          if (add(vf_weight(vf_clean(row[i]), of_p.top, scale, sh.table), both ? vf_weight(vf_clean(row_q[i]), of_q.top, scale, sh.table) : 0.0)) remember(i);
+      };
+      if (c * kVfChunk + kVfChunk > a.V) {
+        slow(base, kVfEach);
+      } else {
+        const float *at = row + base, *at_q = row_q + base;
+        const double top_p = of_p.top, top_q = of_q.top;
+        float v[kVfStep], v_q[kVfStep], w[kVfStep], w_q[kVfStep];  // some entries of both rows, and the next ones on their way
+        auto fetch = [&](int k0, float (&x)[kVfStep], float (&y)[kVfStep]) {
+#pragma unroll
+          for (int k = 0; k < kVfStep; ++k) x[k] = at[(k0 + k) * 32];
+          if (both) {
+#pragma unroll
+            for (int k = 0; k < kVfStep; ++k) y[k] = at_q[(k0 + k) * 32];
+          }
+        };
+        auto take = [&](int i0, const float (&x)[kVfStep], const float (&y)[kVfStep]) {
+          const bool fine = vf_counts<kVfStep>(x, of_p.top, scale_f) && (!both || vf_counts<kVfStep>(y, of_q.top, scale_f));
+          if (!__all_sync(0xffffffffu, fine)) {
+            slow(i0, kVfStep);
+          } else if (both) {
+            double p[kVfStep], q[kVfStep];
+#pragma unroll
+            for (int k = 0; k < kVfStep; ++k) {
+              p[k] = vf_exp2((static_cast<double>(x[k]) - top_p) * scale, sh.table);
+              q[k] = vf_exp2((static_cast<double>(y[k]) - top_q) * scale, sh.table);
+            }
+            unsigned tied = 0u;
+#pragma unroll
+            for (int k = 0; k < kVfStep; ++k) tied |= add(p[k], q[k]) ? 1u << k : 0u;
+            if (tied) {
+#pragma unroll
+              for (int k = 0; k < kVfStep; ++k)
+                if (tied >> k & 1u) remember(i0 + k * 32);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < kVfStep; ++k) {
+              const double p = vf_exp2((static_cast<double>(x[k]) - top_p) * scale, sh.table);
+              (k & 1 ? sum_q : sum_p) += p;  // (two chains; one sum in the end)
+            }
+          }
+        };
+        fetch(0, v, v_q);
+#pragma unroll 1
+        for (int k0 = 0; k0 < kVfEach; k0 += 2 * kVfStep, at += 2 * kVfStep * 32, at_q += 2 * kVfStep * 32) {
+          fetch(kVfStep, w, w_q);
+          take(base + k0 * 32, v, v_q);
+          if (k0 + 2 * kVfStep < kVfEach) fetch(2 * kVfStep, v, v_q);
+          take(base + (k0 + kVfStep) * 32, w, w_q);
+        }
+      }
+      if (!both) {
+        sum_p += sum_q;
+        sum_q = 0.0;
       }
       sum_p = vf_sum(sum_p);
       if (both) {
@@ -512,7 +544,7 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
         more_p = vf_sum(more_p);
         more_q = vf_sum(more_q);
       }
-      if (lane < 2 * kVfCluster) send(lane / kVfCluster, c, lane / kVfCluster == 0 ? sum_p : sum_q);
+      if (lane < 2 * cluster) send(lane / cluster, c, lane / cluster == 0 ? sum_p : sum_q);
       if (lane == 0) {
         s_part[2 * a.chunks + c] = more_p;
         s_part[3 * a.chunks + c] = more_q;
@@ -525,7 +557,7 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
     const float* row = a.logits + r * a.ld;
     const float* row_q = a.draft + r * a.ld_draft;
     const bool lost = __any_sync(0xffffffffu, n_near > kVfNear);  // (more places than a lane remembers: the pieces once more)
-    for (int c = rank + kVfCluster * warp; c < a.chunks; c += kVfCluster * kVfWarps) {
+    for (int c = rank + cluster * warp; c < a.chunks; c += cluster * kVfWarps) {
       double more_p = 0.0, more_q = 0.0;
       auto add = [&](int i) {
         const double p = vf_weight(vf_clean(row[i]), of_p.top, scale, sh.table), q = vf_weight(vf_clean(row_q[i]), of_q.top, scale, sh.table);
@@ -549,7 +581,7 @@ __global__ void __launch_bounds__(kVfThreads) __cluster_dims__(kVfCluster, 1, 1)
         more_q += s_part[3 * a.chunks + c];
       }
       __syncwarp();
-      if (lane < 2 * kVfCluster) send(2 + lane / kVfCluster, c, lane / kVfCluster == 0 ? more_p : more_q);
+      if (lane < 2 * cluster) send(2 + lane / cluster, c, lane / cluster == 0 ? more_p : more_q);
     }
     cluster_sync();
   };
@@ -680,10 +712,10 @@ PMM_EXPORT long long pmm_verify_scratch(long long rows, int V) {
 
 PMM_EXPORT int pmm_verify_drafts(const float* logits, long long ld, const float* draft, long long ld_draft, const int* tokens, const int* parents,
                                  const int* cu, int n, const float* uniforms, const float* temperature, int V, int n_rows, void* scratch,
-                                 int* tokens_out, int* path, int width, int* count, cudaStream_t stream) {
+                                 int* tokens_out, int* path, int width, int* count, int sms, cudaStream_t stream) {
   if (n <= 0) return 0;
   const int chunks = V > 0 ? (V + pmm::kVfChunk - 1) / pmm::kVfChunk : 0;
-  if (V <= 0 || chunks > pmm::kVfChunksMax || n_rows < 0 || static_cast<long long>(n_rows) * chunks > 0x3fffffffll || width <= 0 || !scratch || reinterpret_cast<uintptr_t>(scratch) % 16 ||
+  if (V <= 0 || sms < 1 || chunks > pmm::kVfChunksMax || n_rows < 0 || static_cast<long long>(n_rows) * chunks > 0x3fffffffll || width <= 0 || !scratch || reinterpret_cast<uintptr_t>(scratch) % 16 ||
       (draft && parents) || n > 0x7fffffff / pmm::kVfCluster)
     return PMM_ERR_BAD_ARGUMENT;
   pmm::VerifyArgs a{};
@@ -714,6 +746,24 @@ PMM_EXPORT int pmm_verify_drafts(const float* logits, long long ld, const float*
     const cudaError_t e = cudaFuncSetAttribute(pmm::verify_walk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  pmm::launch_pdl(pmm::verify_walk_kernel, dim3(n * pmm::kVfCluster), dim3(pmm::kVfThreads), smem, stream, a);
+  // as many blocks a request as are on the device at once (two a multiprocessor), up to eight: 64 chains at 130,049 take 106 us with
+  // four, 113 with eight
+  a.cluster = pmm::kVfCluster;
+  while (a.cluster > 1 && static_cast<long long>(n) * a.cluster > 2ll * sms) a.cluster /= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(n) * a.cluster);
+  cfg.blockDim = dim3(pmm::kVfThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = a.cluster;
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, pmm::verify_walk_kernel, a);
   return pmm::launch_status();
 }

@@ -194,7 +194,7 @@ _SIGNATURES = {
                               c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
     "pmm_verify_scratch": [c_longlong, c_int],
     "pmm_verify_drafts": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
-                          c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
+                          c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p],
     "pmm_sample_rows": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                         c_void_p, c_void_p, c_void_p],
 }
@@ -2524,7 +2524,7 @@ def verify_drafts(logits: Tensor, tokens: Tensor, cu_seqlens: Tensor, uniforms: 
         raise KernelError(f"{what}: scratch comes from verify_drafts_scratch for as many rows")
     _call("pmm_verify_drafts", logits.data_ptr(), logits.stride(0), _ptr(draft_logits), ld_draft, tokens.data_ptr(), _ptr(parents),
           cu_seqlens.data_ptr(), n, uniforms.data_ptr(), _ptr(temperature), V, T, scratch.data_ptr(), tokens_out.data_ptr(), path.data_ptr(),
-          path.shape[1], count.data_ptr(), stream)
+          path.shape[1], count.data_ptr(), _sm_count(logits.device), stream)
 
 
 def keep_accepted(rows: Tensor, pool: Tensor, slots: Tensor, cu_seqlens: Tensor, path: Tensor, count: Tensor) -> None:

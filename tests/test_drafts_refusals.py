@@ -26,7 +26,7 @@ TABLES = dict(held=A, new=A, blocks=A, table=A, width=8, free=A, n_free=4, n=2, 
 KEEP = dict(rows=A, ld_layer=100, ld_plane=100, ld_row=100, n_rows=4, pool=A, layers=1, pages=4, planes=2, page_size=64, width=64, item=2,
             slots=A, cu=A, path=A, path_width=4, count=A, n=2, stream=None)
 VERIFY = dict(logits=A, ld=100, draft=None, ld_draft=0, tokens=A, parents=None, cu=A, n=2, uniforms=A, temperature=None, V=100, n_rows=4,
-              scratch=A, tokens_out=A, path=A, width=4, count=A, stream=None)
+              scratch=A, tokens_out=A, path=A, width=4, count=A, sms=148, stream=None)
 
 
 @pytest.mark.parametrize("bad", [dict(width=0), dict(page_size=0), dict(spare=-1), dict(spare=1 << 26), dict(parents=A), dict(masks=A),
@@ -41,7 +41,7 @@ def test_keep_accepted_refuses(bad):
     assert refused("pmm_keep_accepted", KEEP, **bad)
 
 
-@pytest.mark.parametrize("bad", [dict(V=0), dict(V=1 << 30), dict(n_rows=-1), dict(width=0), dict(scratch=None), dict(scratch=A + 8),
+@pytest.mark.parametrize("bad", [dict(V=0), dict(V=1 << 30), dict(n_rows=-1), dict(width=0), dict(scratch=None), dict(scratch=A + 8), dict(sms=0),
                                  dict(draft=A, parents=A)])
 def test_verify_drafts_refuses(bad):
     assert refused("pmm_verify_drafts", VERIFY, **bad)
