@@ -1,22 +1,23 @@
 // Attention of drafted tokens over a paged cache on the fifth-generation tensor cores (the formulas of tree_attention.cu;
-// bfloat16, head size 64 or 128, pages of a multiple of 16 positions).
+// bfloat16, head size 64 or 128, pages of a multiple of 8 positions).
 //
-// A unit of work is up to 128 rows (a row: a token and a query head of the group) of ONE request and ONE key/value head; its
-// keys are tiles of 128, first the request's cached keys, then its own tokens of this step.  The number of tiles of all units
-// is only known on the device (lengths are tensors, contexts are ragged), so every block adds it up and takes an equal share
-// of the tiles, one behind the other (148 SMs stay busy to the end whatever the batch).  A unit that lies within one share is
-// finished by its block; of a unit that shares cut, every block leaves (maximum, sum, unnormalised result) in scratch and a
-// second launch merges them in the order of the keys, so results do not depend on which block came first.
+// A unit of work is up to 128 rows, or 256 (a row: a token and a query head of the group), of ONE request and ONE key/value
+// head; its keys are tiles of 128, first the request's cached keys, then its own tokens of this step.  The number of tiles of
+// all units is only known on the device (lengths are tensors, contexts are ragged), so every block adds it up and takes an
+// equal share of the tiles, one behind the other (148 SMs stay busy to the end whatever the batch).  A unit that lies within one
+// share is finished by its block; of a unit that shares cut, every block leaves (maximum, sum, unnormalised result) in scratch
+// and a second launch merges them in the order of the keys, so results do not depend on which block came first.
 // Within a block warp 0 brings K and V tiles by TMA (cached keys in boxes that lie inside a page, the step's own from k and
-// v) into a ring, warp 1 issues S = Q K^T and O += P V, a warp per 16 rows turns S into P with four threads per row.  The ring
-// and the products run on across units: while a unit's result is written the next one's tiles travel, and its queries are
-// put in place before.
-// Q and P are operands in tensor memory (Q, S, O and two tiles of P: 448 columns of 512): with both in shared memory a tile
-// moves 64 KB in, 128 KB out to the products and 32 KB of P, 1,800 clocks at 128 bytes a clock, where the products take 1,026
-// (eight of 128 x 128 x 16 each, 64 clocks; with half as many rows they take as long, so a unit has 128).  From tensor
-// memory the products read K and V alone.  What thread k of a row's four holds of S are columns 4 i + k; as an operand, P has two
-// neighbouring keys in a word.  So a K tile lies in shared memory with its even keys first and its odd keys behind them (two
-// tensor maps of every other row): columns i and i + 16 of a thread are neighbouring keys, and no word changes threads.
+// v) into a ring; two sets of four warps turn S = Q K^T into P, a thread a row, all 128 of its scores in registers, so that
+// maximum and sum need no other thread; and for each set a warp issues S and O += P V.  Units of 128 rows: the sets take the
+// tiles in turn, and their results are joined when the unit ends.  Units of 256: every set has 128 rows, and K and V are brought
+// once for both.  Each set has its S, running maximum and sum, and its O in tensor memory (4 x 128 columns); P takes the place
+// of the S that it is made from.  A set's products are executed in order: its S is complete only when its P V before is.
+// The ring and the products run on across units.
+// What bounds a tile of 128 rows and 128 keys, clocks: products 1,026 (16 of 128 x 128 x 16, 64 each; half as many rows take as
+// long), exponentials 1,024 (16 a clock), shared memory 1,250 (64 KB in, 96 KB read by the products, 128 bytes a clock), 64 KB from
+// memory 2,800 where it comes from there.  A warp that issues spends 1,400 clocks a tile on barriers, and the products behind
+// one another in its queue do not cover that: hence a warp a set.
 // Of a tile's values only the 16 keys at a time that hold a valid one are multiplied; rows behind the last valid one (stale
 // places of a page, other requests' tokens) are set to zero first, for 0 * NaN is NaN.  Where a tile's keys are not seen by
 // all rows alike (the step's own tokens, a window's edge) values that are not finite are taken out of the product and added
@@ -28,13 +29,19 @@
 namespace pmm {
 
 constexpr int kTtSeqs = 1024;  // requests whose lengths fit shared memory
-constexpr int kTtRows = 128;   // rows of a unit
-constexpr int kTtWarps = kTtRows / 16;
-constexpr int kTtThreads = 64 + kTtWarps * 32;
-// tensor memory: S, O, Q and two tiles of P (operands: two bfloat16 a column)
-constexpr unsigned kTtO = 128, kTtQ = 256, kTtP = 320, kTtCols = 512;
-__host__ __device__ constexpr int tree_ring(int dh) { return dh == 64 ? 11 : 6; }  // tiles in flight (16 or 32 KB each)
-__host__ __device__ constexpr size_t tree_smem(int dh) { return static_cast<size_t>(tree_ring(dh)) * (dh / kAtDhBlock) * kAtKvSub + 1024 /*alignment*/; }
+constexpr int kTtRows = 128;   // rows of a set
+constexpr int kTtThreads = 12 * 32;  // copies, two warps that issue, one without work, two sets of four
+// tensor memory: S (and P) of the two sets of warps, O of the two
+constexpr unsigned kTtO = 256, kTtCols = 512;
+__host__ __device__ constexpr int tree_q_sub() { return kTtRows * kAtDhBlock * 2; }        // a sub-tile of Q: 64 head-size columns
+// tiles in flight (16 or 32 KB each): what the queries leave of shared memory
+// K_j is copy 2 j, V_j copy 2 j + 1 of the block, in slot (copy % ring).  The ring is a multiple of 4, so that all copies of a slot are of one
+// kind and, where the sets take the tiles in turn, of one set: who waits for a slot has seen the copy before in it land (a barrier
+// tells a copy only from the one before, and a wait that skips one may take the last but one for its own).
+__host__ __device__ constexpr int tree_ring(int dh) { return dh == 64 ? 8 : 4; }
+__host__ __device__ constexpr size_t tree_smem(int dh, bool wide) {
+  return static_cast<size_t>(dh / kAtDhBlock) * ((wide ? 2 : 1) * tree_q_sub() + tree_ring(dh) * kAtKvSub) + 1024 /*alignment*/;
+}
 
 // S = Q K^T: both K-major; O += P V: V as it lies in the cache (MN-major), all DH columns at once.
 constexpr unsigned kTtIdescS = at_idesc_s(kTtRows);
@@ -52,26 +59,31 @@ __device__ __forceinline__ void umma_ts_lead(unsigned tmem_d, unsigned tmem_a, u
       : "r"(tmem_d), "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
       : "memory");
 }
-// The store that mirrors at_tmem_ld: 16 lanes of tensor memory x 64 columns.
-__device__ __forceinline__ void tree_tmem_st(unsigned taddr, const unsigned* r) {
+
+// 32 lanes of tensor memory x 16 columns, a lane a row.
+__device__ __forceinline__ void tree_tmem_ld16(unsigned taddr, unsigned* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tree_tmem_st16(unsigned taddr, const unsigned* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n"
       :
       : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 
-// Tensor maps, two-dimensional with boxes of 64 columns: the pool's rows as they are (values), its even and its odd rows (keys), the
-// step's values, the even and the odd rows of its keys.
+// Tensor maps, two-dimensional with boxes of 64 columns: the pool's rows, the step's keys and values.
 struct TreeMaps {
-  CUtensorMap pool_v, pool_k[2], own_v, own_k[2];
+  CUtensorMap pool, own_k, own_v;
 };
-
 struct TreeTcArgs {
   const bf16* q;
   long long ldq;
@@ -87,10 +99,11 @@ struct TreeTcArgs {
   int words;
   const float* sink;
   bf16* out;
-  float* part_o;        // [2 * blocks][M][DH]
-  float2* part_ml;      // [2 * blocks][M]
+  float* part_o;        // [2 * blocks][rows][DH]
+  float2* part_ml;      // [2 * blocks][rows]
   float scale_log2;
   int window, page_size, box, n_seq, T, Hq, Hkv, shares, min_tiles;
+  int rows;             // of a unit: 128 or 256
   int* status;
 };
 
@@ -106,44 +119,63 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeTcArgs& a, int t0, int t1,
   s.held = held;
   s.first = first;
   const int G = a.Hq / a.Hkv;
-  s.n_rt = (s.n_new * G + kTtRows - 1) / kTtRows;
+  s.n_rt = (s.n_new * G + a.rows - 1) / a.rows;
   s.ctx_tiles = held > first ? (held - first + kAtKeys - 1) / kAtKeys : 0;
   s.nt = s.ctx_tiles + (s.n_new + kAtKeys - 1) / kAtKeys;
   return s;
 }
 
-// The lengths of all requests in shared memory, and the running sum of their tiles.
+// The lengths of all requests in shared memory, and the running sum of their tiles.  The order of the units: where all requests have as
+// many row tiles, row tile by row tile over all requests, so that the blocks that read the same keys do so at the same time
+// (one behind the other every row tile brought them from memory anew: the wide trees' 0.6 GB became 2.1); else request by request.
 struct TreePlan {
-  int* pre;    // [n_seq + 1] tiles in front of a request
+  int* pre;    // [n_seq + 1] tiles in front of a request, in the first row tile's round or in all
   int* cu;     // [n_seq + 1]
   int* held;   // [n_seq]
   int* first;  // [n_seq]
+  int rounds;  // row tiles of every request, or 0: requests differ
+  int total;
 };
 __host__ __device__ constexpr size_t tree_plan_bytes(int n_seq) { return (4 * static_cast<size_t>(n_seq) + 2) * sizeof(int); }
 
 // Called by all THREADS threads of the block; red: shared memory for 32 ints.
 template <int THREADS>
-__device__ __forceinline__ void tree_plan(const TreeTcArgs& a, const TreePlan& p, int* red) {
+__device__ __forceinline__ void tree_plan(const TreeTcArgs& a, TreePlan& p, int* red) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) red[31] = 0;
+  __syncthreads();
+  int same = -1;
+  bool differ = false;
+  for (int s = tid; s < a.n_seq; s += THREADS) {
+    const int t0 = min(max(a.cu[s], 0), a.T), t1 = min(max(a.cu[s + 1], t0), a.T);
+    const int held = max(0, static_cast<int>(min(static_cast<long long>(a.held[s]), static_cast<long long>(a.max_blocks) * a.page_size)));
+    int first = 0;
+    if (a.window != 0) {  // the first key that any of the request's tokens may see
+      int pos = 0x7fffffff;
+      for (int t = t0; t < t1; ++t) pos = min(pos, a.positions[t]);
+      first = t1 > t0 ? min(first_visible(pos, a.window), held) / a.box * a.box : 0;
+    }
+    p.cu[s] = t0;
+    if (s == a.n_seq - 1) p.cu[s + 1] = t1;
+    p.held[s] = held;
+    p.first[s] = first;
+    const int n_rt = tree_seq(a, t0, t1, held, first).n_rt;
+    if (n_rt > 0) {
+      differ |= same > 0 && n_rt != same;
+      same = n_rt;
+    }
+  }
+  if (same > 0) atomicMax(&red[31], same);
+  const int any_differs = __syncthreads_or(differ);
+  const int most = red[31];
+  p.rounds = __syncthreads_or(any_differs || (same > 0 && same != most)) ? 0 : most;
   int total = 0;
   for (int base = 0; base < a.n_seq; base += THREADS) {
     const int s = base + tid;
     int tiles = 0;
     if (s < a.n_seq) {
-      const int t0 = min(max(a.cu[s], 0), a.T), t1 = min(max(a.cu[s + 1], t0), a.T);
-      const int held = max(0, static_cast<int>(min(static_cast<long long>(a.held[s]), static_cast<long long>(a.max_blocks) * a.page_size)));
-      int first = 0;
-      if (a.window != 0) {  // the first key that any of the request's tokens may see
-        int pos = 0x7fffffff;
-        for (int t = t0; t < t1; ++t) pos = min(pos, a.positions[t]);
-        first = t1 > t0 ? min(first_visible(pos, a.window), held) / a.box * a.box : 0;
-      }
-      p.cu[s] = t0;
-      if (s == a.n_seq - 1) p.cu[s + 1] = t1;
-      p.held[s] = held;
-      p.first[s] = first;
-      const TreeSeq q = tree_seq(a, t0, t1, held, first);
-      tiles = q.nt * q.n_rt * a.Hkv;
+      const TreeSeq q = tree_seq(a, p.cu[s], p.cu[s + 1], p.held[s], p.first[s]);
+      tiles = q.n_rt > 0 ? q.nt * a.Hkv * (p.rounds > 0 ? 1 : q.n_rt) : 0;
     }
     int run = tiles;
 #pragma unroll
@@ -164,6 +196,7 @@ __device__ __forceinline__ void tree_plan(const TreeTcArgs& a, const TreePlan& p
   }
   if (tid == 0) p.pre[a.n_seq] = total;
   __syncthreads();
+  p.total = total * max(p.rounds, 1);
 }
 
 // How many blocks share `total` tiles, the tile at which block b's share begins, and the block in whose share tile x lies.
@@ -182,10 +215,11 @@ struct TreeSeg {
 };
 // The stretch that begins at tile `at` and ends with its unit or at `end`.
 __device__ __forceinline__ TreeSeg tree_seg(const TreeTcArgs& a, const TreePlan& p, int at, int end) {
-  int lo = 0, hi = a.n_seq - 1;  // the last request that begins at or before `at` (behind requests without tiles)
+  const int round = p.pre[a.n_seq], rt = p.rounds > 0 ? at / round : 0, in_round = at - rt * round;
+  int lo = 0, hi = a.n_seq - 1;  // the last request that begins at or before (behind requests without tiles)
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (p.pre[mid] <= at)
+    if (p.pre[mid] <= in_round)
       lo = mid;
     else
       hi = mid - 1;
@@ -193,9 +227,14 @@ __device__ __forceinline__ TreeSeg tree_seg(const TreeTcArgs& a, const TreePlan&
   TreeSeg g;
   g.seq = lo;
   g.s = tree_seq(a, p.cu[lo], p.cu[lo + 1], p.held[lo], p.first[lo]);
-  const int off = at - p.pre[lo], u = off / g.s.nt;
-  g.hk = u / g.s.n_rt;
-  g.rt = u - g.hk * g.s.n_rt;
+  const int off = in_round - p.pre[lo], u = off / g.s.nt;
+  if (p.rounds > 0) {
+    g.hk = u;
+    g.rt = rt;
+  } else {
+    g.hk = u / g.s.n_rt;
+    g.rt = u - g.hk * g.s.n_rt;
+  }
   g.unit = at - (off - u * g.s.nt);
   g.j0 = at - g.unit;
   g.j1 = min(g.s.nt, end - g.unit);
@@ -206,17 +245,23 @@ __device__ __forceinline__ int tree_valid(const TreeSeq& s, int j) {
   return j < s.ctx_tiles ? min(kAtKeys, s.held - s.first - j * kAtKeys) : min(kAtKeys, s.n_new - (j - s.ctx_tiles) * kAtKeys);
 }
 
-template <int DH>
+template <int DH, bool WIDE>
 __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const __grid_constant__ TreeMaps maps, const __grid_constant__ TreeTcArgs a) {
   constexpr int NSUB = DH / kAtDhBlock;
   constexpr int kRing = tree_ring(DH);
+  constexpr int kRows = WIDE ? 2 * kTtRows : kTtRows;  // of a unit
   constexpr int kSlot = NSUB * kAtKvSub;
+  constexpr int kQSub = tree_q_sub();
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) unsigned long long bar_q, bar_full[kRing], bar_empty[kRing], bar_s, bar_sfree, bar_p[2], bar_pv[2];
+  // the queries are in place / have been read by a unit's last S; a slot is full / empty; a set's S and P are there; a unit's last
+  // products are done; both sets' maxima and sums are there; both have read their O; it is a set's turn to make its exponentials
+  __shared__ __align__(8) unsigned long long bar_q, bar_qfree, bar_full[kRing], bar_empty[kRing], bar_s[2], bar_p[2], bar_turn[2], bar_done, bar_ml, bar_read;
+  __shared__ float2 s_ml[2][2][kTtRows];  // (of two stretches in turn: one set may be a stretch ahead)
   __shared__ unsigned s_tmem_base;
   __shared__ int s_abort, s_red[32], s_bad[2];
 
-  unsigned char* sRing = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* sQ = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* sRing = sQ + (WIDE ? 2 : 1) * NSUB * kQSub;
   TreePlan plan;
   plan.pre = reinterpret_cast<int*>(sRing + kRing * kSlot);
   plan.cu = plan.pre + a.n_seq + 1;
@@ -227,28 +272,31 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int G = a.Hq / a.Hkv;
   if (tid == 0) {
-    mbar_init(&bar_q, kTtWarps);
+    mbar_init(&bar_q, 8);
+    mbar_init(&bar_qfree, 2);
 #pragma unroll
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&bar_full[i], 1);
-      mbar_init(&bar_empty[i], 1);
+      mbar_init(&bar_empty[i], WIDE ? 2 : 1);
     }
-    mbar_init(&bar_s, 1);
-    mbar_init(&bar_sfree, kTtWarps);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar_p[i], kTtWarps);
-      mbar_init(&bar_pv[i], 1);
+      mbar_init(&bar_s[i], 1);
+      mbar_init(&bar_p[i], 4);
+      mbar_init(&bar_turn[i], 4);
     }
+    mbar_init(&bar_done, 2);
+    mbar_init(&bar_ml, 8);
+    mbar_init(&bar_read, 8);
     s_abort = 0;
     s_bad[0] = s_bad[1] = -1;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-    asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<unsigned long long>(&maps.pool_v)) : "memory");
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<unsigned long long>(&maps.pool)) : "memory");
   }
   pdl_wait();
   pdl_launch_dependents();  // (behind the wait: the merge reads the lengths ahead of its own)
   tree_plan<kTtThreads>(a, plan, s_red);
-  const int total = plan.pre[a.n_seq];
+  const int total = plan.total;
   const int shares = tree_shares(a, total);
   if (static_cast<int>(blockIdx.x) >= shares || total == 0) return;
   const int begin = tree_begin(blockIdx.x, total, shares), end = tree_begin(blockIdx.x + 1, total, shares);
@@ -267,18 +315,22 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
     s_abort = 1;
   };
 
+  // The block is launched with 168 registers a thread, 64,512 in all: 96 for the first four warps, 200 for the softmax warps, whose 128
+  // scores a thread do not fit otherwise (128 * 96 + 256 * 200 = 63,488).
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer (the whole warp walks, a lane a box)
     const int page_size = a.page_size;
     const int per = kAtKeys / a.box;  // boxes of a tile of cached keys
-    int item = 0;
+    int n_k = 0, n_v = 0;             // copies requested
     bool ok = true;
     struct Tile {
       int row, valid, hk;  // row of the pool (of k and v) at which this lane's box begins, keys of the tile
       bool own;            // the step's own tokens
     };
     auto request = [&](const Tile& t, bool is_v) {
-      const int slot = item % kRing;
+      const int item = is_v ? 2 * n_v + 1 : 2 * n_k, slot = item % kRing;
       if (item >= kRing && ok) {
         int got = 1;
         if (lane == 0) got = mbar_wait(&bar_empty[slot], (item / kRing - 1) & 1, abort_flag) ? 1 : 0;
@@ -290,19 +342,12 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
       const int boxes = (t.valid + keys - 1) / keys;
       if (lane == 0) mbar_expect_tx(&bar_full[slot], static_cast<unsigned>(boxes * keys * NSUB * 128));
       __syncwarp();
-      // a lane a copy: box, sub-tile of 64 columns and, of keys, even or odd rows
-      const int d = lane % NSUB, e = is_v ? 0 : lane / NSUB & 1, b = lane / (is_v ? NSUB : 2 * NSUB);
+      const int d = lane % NSUB, b = lane / NSUB;  // a lane a copy: sub-tile of 64 columns, box
       const int row = __shfl_sync(0xffffffffu, t.row, b);
-      if (b < boxes) {
-        unsigned char* dst = sRing + slot * kSlot + d * kAtKvSub;
-        const int col = t.hk * DH + d * kAtDhBlock;
-        if (is_v)
-          tma_load_2d(dst + b * keys * 128, t.own ? &maps.own_v : &maps.pool_v, col, row + (t.own ? 0 : page_size), &bar_full[slot]);
-        else  // key 2 m + e of the tile to row 64 e + m
-          tma_load_2d(dst + (64 * e + b * keys / 2) * 128, t.own ? &maps.own_k[(row + e) & 1] : &maps.pool_k[e], col, (row + (t.own ? e : 0)) >> 1,
-                      &bar_full[slot]);
-      }
-      ++item;
+      if (b < boxes)
+        tma_load_2d(sRing + slot * kSlot + d * kAtKvSub + b * keys * 128, t.own ? (is_v ? &maps.own_v : &maps.own_k) : &maps.pool,
+                    t.hk * DH + d * kAtDhBlock, row + (is_v && !t.own ? page_size : 0), &bar_full[slot]);
+      ++(is_v ? n_v : n_k);
     };
     Tile prev{};
     for (int at = begin; at < end && ok;) {
@@ -337,217 +382,231 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
     __syncwarp();
     if (lane == 0 && s_abort) {
       // copies already requested still write into this block's shared memory: wait for them
-      for (int it = max(0, item - kRing); it < item; ++it)
+      for (int u = 0; u < kRing; ++u) {  // the last copy of every slot
+        const int last = (u & 1) ? 2 * (n_v - 1) + 1 : 2 * (n_k - 1), it = last - (last - u + kRing) % kRing;
+        if (it < 0) continue;
         for (unsigned i = 0; i < kSpinLimit && !mbar_try_wait(&bar_full[it % kRing], (it / kRing) & 1); ++i) {
         }
+      }
     }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer (the whole warp walks, one lane issues)
-    // (what the products are issued with is known to be the same in the whole warp: it stays in uniform registers)
-    auto uniform = [](auto x) { return __shfl_sync(0xffffffffu, x, 0); };
+  } else if (warp == 1 || warp == 2) {
+    // ---------------------------------------------------------------- MMA issuers, one a set (the whole warp walks, one lane issues)
+    const int set = warp - 1;
+    // What the products are issued with, and everything that decides whether they are, comes out of a reduction or a vote: it is known to
+    // be the same in the whole warp and stays in uniform registers (130 to 180 clocks a product where it is not, 64 where it is).
+    auto uniform = [](unsigned x) { return static_cast<int>(__reduce_max_sync(0xffffffffu, x)); };
     const int n = uniform(n_tiles), items = 2 * n;
-    const unsigned tmem = uniform(tmem_base);
+    const unsigned tmem = uniform(tmem_base), s_tmem = tmem + kAtKeys * set, o_tmem = tmem + kTtO + 128 * set;
     const unsigned lead = lane == 0 ? 1u : 0u;
-    const unsigned long long ring_desc = umma_desc(sRing);
+    const unsigned long long q_desc = umma_desc(sQ + (WIDE ? set * NSUB * kQSub : 0)), ring_desc = umma_desc(sRing);
     // (of a V tile: 64 columns further lie one sub-tile further)
     const unsigned long long v_ring = (ring_desc & ~(0x3fffull << 16)) | (static_cast<unsigned long long>(kAtKvSub >> 4) << 16);
     auto wait = [&](unsigned long long* bar, unsigned parity) {
-      const bool got = mbar_wait(bar, parity, abort_flag);
-      __syncwarp();  // (no lane may fall a phase behind)
-      return got;
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;  // (no lane may fall a phase behind)
     };
     auto full = [&](int it) { return wait(&bar_full[it % kRing], (it / kRing) & 1); };
-    auto issue_s = [&](int j) {  // S_j = Q K_j^T
-      const int slot = at_k_item(j) % kRing;
-      const unsigned long long k_desc = ring_desc + static_cast<unsigned>(slot * (kSlot >> 4));
-#pragma unroll
-      for (int k = 0; k < DH / 16; ++k)
-        umma_ts_lead(tmem, tmem + kTtQ + 8 * k, k_desc + (k >> 2) * (kAtKvSub >> 4) + 2 * (k & 3), kTtIdescS, k > 0 ? 1u : 0u, lead);
-      umma_commit_lead(&bar_s, lead);
-      if (at_k_item(j) + kRing < items) umma_commit_lead(&bar_empty[slot], lead);
+    // a slot's copy has been used (nobody waits for the last copies' slots); by a set without rows, at once
+    auto used = [&](int it, bool rows) {
+      if (it + kRing < items) {
+        if (rows)
+          umma_commit_lead(&bar_empty[it % kRing], lead);
+        else if (lane == 0)
+          mbar_arrive(&bar_empty[it % kRing]);
+      }
     };
-    int code = 0, segs = 0;
-    TreeSeg g = tree_seg(a, plan, begin, end);
-    if (wait(&bar_q, 0) && full(0)) {
-      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-      issue_s(0);
-    } else {
-      code = 43;
-    }
-    for (int j = 0; j < n && code == 0; ++j) {
-      const int own = begin + j - g.unit;  // this tile within its unit
-      const int steps = uniform((tree_valid(g.s, own) + 15) / 16);
-      const unsigned more = uniform(own > g.j0 ? 1u : 0u);  // 0 in the first tile of a stretch: O begins anew
-      if (own + 1 == g.j1) {               // the next tile is another unit's
-        ++segs;
-        if (j + 1 < n) g = tree_seg(a, plan, begin + j + 1, end);
+    constexpr int kStep = WIDE ? 1 : 2;
+    // The set's tiles, stretch by stretch.  Two walks over them: of the S products and, a tile behind, of the P V.  (A set has tiles in
+    // every stretch but those of one tile, and no two of those without one follow one another.)  Tiles are counted within the block.
+    struct Walk {
+      int seg, t, end;               // the stretch's number, the next tile, the stretch's end
+      int live, in, rows;            // in: its queries are in place; rows: the set has some (of 256, the second may have none)
+      int own, last;                 // the unit's first tile of the step's own tokens, its last tile
+      int ctx_steps, last_steps;     // sixteens of keys in the last tile of cached keys, and in the last of all
+    };
+    auto load = [&](Walk& w, int at) {
+      const TreeSeg g = tree_seg(a, plan, at, end);
+      w.end = uniform(g.unit + g.j1 - begin);
+      w.rows = uniform(!WIDE || g.s.n_new * G - g.rt * kRows > set * kTtRows ? 1u : 0u);
+      // (negative where the unit began in an earlier block: moved up by 2^30 to be compared as unsigned)
+      w.own = uniform(g.unit + g.s.ctx_tiles - begin + (1 << 30)) - (1 << 30);
+      w.last = uniform(g.unit + g.s.nt - 1 - begin + (1 << 30)) - (1 << 30);
+      w.ctx_steps = uniform(g.s.ctx_tiles > 0 ? (tree_valid(g.s, g.s.ctx_tiles - 1) + 15) / 16 : 0);
+      w.last_steps = uniform((tree_valid(g.s, g.s.nt - 1) + 15) / 16);
+    };
+    auto leave = [&](Walk& w) {
+      w.in = 0;
+      w.live = w.end < n;
+      if (w.live) {
+        load(w, begin + w.end);
+        ++w.seg;
       }
-      if (j + 1 < n) {
-        // the softmax threads hold S_j in registers: the next S may overwrite it, and the tensor core works on it while they compute
-        if (!full(at_k_item(j + 1)) || !wait(&bar_sfree, j & 1) || (begin + j + 1 == g.unit + g.j0 && !wait(&bar_q, segs & 1))) {
-          code = 43;
-          break;
-        }
+    };
+    Walk ws;
+    ws.seg = ws.in = 0;
+    ws.t = WIDE ? 0 : set;
+    ws.live = 1;
+    load(ws, begin);
+    Walk wp = ws;
+    auto enter = [&]() {
+      if (!ws.in) ws.in = wait(&bar_q, ws.seg & 1);
+      return ws.in != 0;
+    };
+    auto issue_s = [&]() {  // the next S, where there is one
+      while (ws.live && ws.t >= ws.end) {  // (a stretch without a tile of this set)
+        if (!enter()) return false;
+        umma_commit_lead(&bar_qfree, lead);
+        leave(ws);
+      }
+      if (!ws.live) return true;
+      const int item = 2 * ws.t, slot = item % kRing;
+      if (!enter() || !full(item)) return false;
+      if (ws.rows) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        issue_s(j + 1);
+        const unsigned long long k_desc = ring_desc + static_cast<unsigned>(slot * (kSlot >> 4));
+#pragma unroll
+        for (int k = 0; k < DH / 16; ++k)
+          umma_f16_lead(s_tmem, q_desc + (k >> 2) * (kQSub >> 4) + 2 * (k & 3), k_desc + (k >> 2) * (kAtKvSub >> 4) + 2 * (k & 3), kTtIdescS,
+                        k > 0 ? 1u : 0u, lead);
+        umma_commit_lead(&bar_s[set], lead);
       }
-      const int v_item = at_v_item(j, n);
-      if (!full(v_item) || !wait(&bar_p[j & 1], (j >> 1) & 1)) {
+      used(item, ws.rows);
+      ws.t += kStep;
+      if (ws.t >= ws.end) {  // the stretch's last of this set: its queries may make way
+        umma_commit_lead(&bar_qfree, lead);
+        leave(ws);
+      }
+      return true;
+    };
+    int code = issue_s() ? 0 : 43, n_p = 0;  // tiles of P used
+    int more = 0, told = 0;                  // O goes on; the stretch's end has been told
+    while (code == 0 && wp.live) {
+      if (wp.t >= wp.end) {
+        if (!told) umma_commit_lead(&bar_done, lead);
+        told = more = 0;
+        const int left = wp.seg;
+        leave(wp);
+        if (wp.live && !wait(&bar_read, left & 1)) code = 44;  // (its O has been read)
+        continue;
+      }
+      const int item = 2 * wp.t + 1, slot = item % kRing;
+      if (!full(item) || (wp.rows && !wait(&bar_p[set], n_p & 1))) {
         code = 44;
         break;
       }
-      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-      const int slot = v_item % kRing;
-      const unsigned long long v_desc = v_ring + static_cast<unsigned>(slot * (kSlot >> 4));
-      const unsigned p_tmem = tmem + kTtP + 64 * (j & 1);
-      auto product = [&](int k) {  // 16 keys: 16 rows of 128 bytes of every sub-tile
-        umma_ts_lead(tmem + kTtO, p_tmem + 8 * k, v_desc + ((k * 16 * 128) >> 4), tree_idesc_o(DH), k > 0 ? 1u : more, lead);
-      };
-      if (steps == kAtKeys / 16) {
+      if (wp.rows) {
+        ++n_p;
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const int steps = wp.t == wp.own - 1 ? wp.ctx_steps : wp.t == wp.last ? wp.last_steps : kAtKeys / 16;
+        const unsigned long long v_desc = v_ring + static_cast<unsigned>(slot * (kSlot >> 4));
+        auto product = [&](int k) {  // 16 keys: 16 rows of 128 bytes of every sub-tile
+          umma_ts_lead(o_tmem, s_tmem + 8 * k, v_desc + ((k * 16 * 128) >> 4), tree_idesc_o(DH), k > 0 ? 1u : static_cast<unsigned>(more), lead);
+        };
+        if (steps == kAtKeys / 16) {
 #pragma unroll
-        for (int k = 0; k < kAtKeys / 16; ++k) product(k);
-      } else {
-        for (int k = 0; k < steps; ++k) product(k);
+          for (int k = 0; k < kAtKeys / 16; ++k) product(k);
+        } else {
+          for (int k = 0; k < steps; ++k) product(k);
+        }
       }
-      umma_commit_lead(&bar_pv[j & 1], lead);
-      if (v_item + kRing < items) umma_commit_lead(&bar_empty[slot], lead);
+      used(item, wp.rows);
+      more = 1;
+      wp.t += kStep;
+      if (wp.t >= wp.end) {
+        umma_commit_lead(&bar_done, lead);
+        told = 1;
+      }
+      if (!issue_s()) code = 43;  // (into the S whose P has just been used: products run in order)
     }
     if (code != 0) give_up(code);
+  }
   } else {
-    // ---------------------------------------------------------------- softmax and output (a warp per 16 rows)
-    // groups of 16 rows go round the four quarters of tensor memory (and of the multiprocessor): few rows, too, use all of it
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const int base_row = (half * 4 + quarter) * 16;
-    const unsigned lane_base = tmem_base + (static_cast<unsigned>(quarter * 32 + half * 16) << 16);
-    const int k4 = lane & 3;                              // this thread's columns: 4 i + k4
-    const int row0 = base_row + (lane >> 2);
-    const int soft_tid = tid - 64;                        // among the softmax threads
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
+    // ---------------------------------------------------------------- softmax and output (a thread a row, two sets of warps)
+    const int set = (warp - 4) >> 2, quarter = warp & 3;
+    const int row = (WIDE ? set * kTtRows : 0) + quarter * 32 + lane;  // of the unit (quarter * 32 + lane: its lane of tensor memory)
+    const unsigned lane_base = tmem_base + (static_cast<unsigned>(quarter * 32) << 16);
+    const unsigned s_tmem = lane_base + kAtKeys * set, o_tmem = lane_base + kTtO + 128 * set;
+    const int soft_tid = tid - 128, set_tid = soft_tid & 127;  // among the softmax threads, the set's
     bool alive = true;
-    int gt = 0;                                           // tiles so far
-    auto product_done = [&](int i) { return mbar_wait(&bar_pv[i & 1], (i >> 1) & 1, abort_flag); };  // O += P V of tile i
-    // the stretch's query rows -> tensor memory (rows beyond the unit are zero)
-    auto queries = [&](const TreeSeg& g) {
-      const int n_rows = min(kTtRows, g.s.n_new * G - g.rt * kTtRows);
-      unsigned w[DH / 4];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = row0 + 8 * r, gr = g.rt * kTtRows + row, tk = gr / G;
-        const bool there = row < n_rows;
-        const unsigned* src = reinterpret_cast<const unsigned*>(a.q + (g.s.t0 + (there ? tk : 0)) * a.ldq + (g.hk * G + (there ? gr - tk * G : 0)) * DH) + k4;
-#pragma unroll
-        for (int i = 0; i < DH / 8; ++i) w[2 * i + r] = there ? src[4 * i] : 0u;
+    auto wait = [&](unsigned long long* bar, unsigned parity) {
+      const bool got = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+      if (!got) {
+        if (lane == 0) give_up(45);
+        alive = false;
       }
+      return got;
+    };
+    // the stretch's query rows -> shared memory, swizzled (rows beyond the unit are zero)
+    auto queries = [&](const TreeSeg& g) {
+      const int n_rows = min(kRows, g.s.n_new * G - g.rt * kRows);
+      constexpr int kPieces = DH / 8;
+      for (int p0 = soft_tid; p0 < kRows * kPieces; p0 += 1024) {  // neighbouring lanes take neighbouring pieces
+        uint4 x[4];
 #pragma unroll
-      for (int c = 0; c < DH / 64; ++c) at_tmem_st32(lane_base + kTtQ + 32 * c, w + 16 * c);
-      asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-      asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        for (int i = 0; i < 4; ++i) {
+          const int p = p0 + 256 * i, r = p / kPieces, c = p % kPieces;
+          const int gr = g.rt * kRows + r, tk = gr / G;
+          x[i] = r < n_rows ? *reinterpret_cast<const uint4*>(a.q + (g.s.t0 + tk) * a.ldq + (g.hk * G + (gr - tk * G)) * DH + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int p = p0 + 256 * i, r = p / kPieces, c = p % kPieces;
+          *reinterpret_cast<uint4*>(sQ + ((r >> 7) * NSUB + (c >> 3)) * kQSub + at_swizzled(r & 127, c & 7)) = x[i];
+        }
+      }
+      fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar_q);
+    };
+    int n_s = 0;                                          // tiles of S that this set has taken
+    // The sets make their exponentials in turn, the first set first: side by side they share the units, and both then wait for their
+    // products at the same time (5,850 clocks a tile of both sets; in turn XX).
+    int n_turn = 0;
+    auto my_turn = [&]() {
+      if (set == 1 || n_turn > 0) {
+        if (!wait(&bar_turn[set], (set == 1 ? n_turn : n_turn - 1) & 1)) return false;
+      }
+      ++n_turn;
+      return true;
+    };
+    auto pass_turn = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_turn[set ^ 1]);
     };
     TreeSeg g = tree_seg(a, plan, begin, end);
     queries(g);
     for (int seg = 0, at = begin; at < end && alive; ++seg) {
-      const int n_rows = min(kTtRows, g.s.n_new * G - g.rt * kTtRows);
-      const bool idle = base_row >= n_rows;               // (the whole warp: none of its rows exists)
-      int my_tok[2], my_lo[2];                            // of this thread's rows: token of the request, first cached key
-      float m_run[2], l_run[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = row0 + 8 * r;
-        my_tok[r] = row < n_rows ? (g.rt * kTtRows + row) / G : 0;
-        my_lo[r] = a.window != 0 ? first_visible(a.positions[g.s.t0 + my_tok[r]], a.window) : 0;
-        m_run[r] = -CUDART_INF_F;
-        l_run[r] = 0.f;
-      }
-      float sum[2] = {0.f, 0.f}, alpha[2] = {1.f, 1.f};
-      auto take_sums = [&]() {
-        float t0 = sum[0] + __shfl_xor_sync(0xffffffffu, sum[0], 1), t1 = sum[1] + __shfl_xor_sync(0xffffffffu, sum[1], 1);
-        t0 += __shfl_xor_sync(0xffffffffu, t0, 2);
-        t1 += __shfl_xor_sync(0xffffffffu, t1, 2);
-        l_run[0] = l_run[0] * alpha[0] + t0;
-        l_run[1] = l_run[1] * alpha[1] + t1;
-      };
-      // the bits of a row's visible keys among the 128 of tile j of the step's own tokens
-      auto own_bits = [&](int r, int j, unsigned long long (&w)[2]) {
-        const int k0 = (j - g.s.ctx_tiles) * kAtKeys, valid = tree_valid(g.s, j);
-        const int upto = a.mask ? valid : min(valid, my_tok[r] + 1 - k0);  // without masks: up to the token itself
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int n = upto - 64 * h;
-          w[h] = n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull;
-          if (a.mask) {
-            const int at_word = k0 / 64 + h;
-            w[h] &= at_word < a.words ? a.mask[static_cast<size_t>(g.s.t0 + my_tok[r]) * a.words + at_word] : 0ull;
-          }
-        }
-      };
+      const int n_rows = min(kRows, g.s.n_new * G - g.rt * kRows);
+      const bool idle = (WIDE ? set * kTtRows : 0) + quarter * 32 >= n_rows;           // (the whole warp: none of its rows exists)
+      const int my_tok = row < n_rows ? (g.rt * kRows + row) / G : 0;   // the row's token, of the request
+      const int my_lo = a.window != 0 ? first_visible(a.positions[g.s.t0 + my_tok], a.window) : 0;  // its first cached key
+      float m_run = -CUDART_INF_F, l_run = 0.f;           // maximum in use (exponent's unit), sum against it
       int edge = 0;                                       // behind it every row of the unit sees all cached keys
       if (a.window != 0) {
-        const int last = (g.rt * kTtRows + n_rows - 1) / G;
-        for (int tk = g.rt * kTtRows / G + lane; tk <= last; tk += 32) edge = max(edge, first_visible(a.positions[g.s.t0 + tk], a.window));
+        const int last = (g.rt * kRows + n_rows - 1) / G;
+        for (int tk = g.rt * kRows / G + lane; tk <= last; tk += 32) edge = max(edge, first_visible(a.positions[g.s.t0 + tk], a.window));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) edge = max(edge, __shfl_xor_sync(0xffffffffu, edge, o));
       }
       // whether the rows may see tile j's keys differently: the step's own tokens, and in front of the windows' last edge
       auto mixed = [&](const TreeSeg& of, int j) { return j >= of.s.ctx_tiles || of.s.first + j * kAtKeys < edge; };
-      for (int j = g.j0; j < g.j1; ++j, ++gt, ++at) {
+      // the set's tiles: all of them, where it has rows, or every second, over all units
+      const int first = WIDE ? (n_rows > set * kTtRows ? at : g.unit + g.j1) : at + ((at - begin + set) & 1);
+      for (int t = first; t < g.unit + g.j1; t += WIDE ? 1 : 2) {
+        const int j = t - g.unit, gt = t - begin;         // within the unit, of the block
         const bool own = j >= g.s.ctx_tiles;
         const int base = g.s.first + j * kAtKeys;         // (cached keys)
         const int valid = tree_valid(g.s, j);
-        bool ok = mbar_wait(&bar_s, gt & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {
-          if (lane == 0) give_up(45);
-          alive = false;
-          break;
-        }
+        if (!wait(&bar_s[set], n_s++ & 1)) break;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        unsigned v[kAtKeys / 2];
-        if (!idle) {
-          at_tmem_ld(lane_base, v);
-          at_tmem_ld(lane_base + 64, v + 32);
-          if (j > g.j0) take_sums();  // (of the tile before, while these travel)
-          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-        }
-        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_sfree);
-        if (!idle) {
-          if (own) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              unsigned long long w[2];
-              own_bits(r, j, w);
-              w[0] >>= 2 * k4;
-              w[1] >>= 2 * k4;
-#pragma unroll
-              for (int i = 0; i < kAtKeys / 4; ++i)  // keys 8 (i % 16) + 2 k4 + i / 16
-                if (!(w[(i & 15) >> 3] >> (8 * (i & 7) + (i >> 4)) & 1ull)) v[2 * i + r] = __float_as_uint(-CUDART_INF_F);
-            }
-          } else if (valid < kAtKeys || base < max(my_lo[0], my_lo[1])) {
-#pragma unroll
-            for (int i = 0; i < kAtKeys / 4; ++i) {
-              const int key = base + 8 * (i & 15) + 2 * k4 + (i >> 4);
-#pragma unroll
-              for (int r = 0; r < 2; ++r)
-                if (!(key >= my_lo[r] && key < g.s.held)) v[2 * i + r] = __float_as_uint(-CUDART_INF_F);
-            }
-          }
-        }
         if (valid % 16 != 0 || mixed(g, j)) {
           // values that must not meet a probability of zero: rows behind the last valid one become zero; where rows see the
           // keys differently, so do values that are not finite
-          const int item = at_v_item(gt, n_tiles), slot = item % kRing;
-          ok = mbar_wait(&bar_full[slot], (item / kRing) & 1, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) {
-            if (lane == 0) give_up(45);
-            alive = false;
-            break;
-          }
+          const int item = 2 * gt + 1, slot = item % kRing;
+          if (!wait(&bar_full[slot], (item / kRing) & 1)) break;
           unsigned char* sV = sRing + slot * kSlot;
           const int from = mixed(g, j) ? 0 : valid * (DH / 8), to = (valid + 15) / 16 * 16 * (DH / 8);
-          for (int p = from + soft_tid; p < to; p += kTtWarps * 32) {
+          for (int p = from + set_tid; p < to; p += 128) {
             const int r = p / (DH / 8), c = p % (DH / 8);
             uint4* at16 = reinterpret_cast<uint4*>(sV + (c >> 3) * kAtKvSub + at_swizzled(r, c & 7));
             if (r >= valid) {
@@ -576,136 +635,155 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
           fence_proxy_async();
         }
         if (!idle) {
-          float mx[2][2];
+          unsigned v[kAtKeys];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            mx[r][0] = fmaxf(__uint_as_float(v[r]), __uint_as_float(v[2 + r]));
-            mx[r][1] = fmaxf(__uint_as_float(v[4 + r]), __uint_as_float(v[6 + r]));
-          }
+          for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + 32 * c, v + 32 * c);
+          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+          if (own) {
+            // the bits of the row's visible keys among these 128: of its mask, or up to the token itself
+            const int k0 = (j - g.s.ctx_tiles) * kAtKeys;
+            const int upto = a.mask ? valid : min(valid, my_tok + 1 - k0);
 #pragma unroll
-          for (int i = 4; i < kAtKeys / 4; i += 4)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              mx[r][0] = at_max3(mx[r][0], __uint_as_float(v[2 * i + r]), __uint_as_float(v[2 * i + 2 + r]));
-              mx[r][1] = at_max3(mx[r][1], __uint_as_float(v[2 * i + 4 + r]), __uint_as_float(v[2 * i + 6 + r]));
-            }
-          mx[0][0] = fmaxf(mx[0][0], mx[0][1]);
-          mx[1][0] = fmaxf(mx[1][0], mx[1][1]);
-#pragma unroll
-          for (int o = 1; o <= 2; ++o) {
-            const float o0 = __shfl_xor_sync(0xffffffffu, mx[0][0], o), o1 = __shfl_xor_sync(0xffffffffu, mx[1][0], o);
-            mx[0][0] = fmaxf(mx[0][0], o0);
-            mx[1][0] = fmaxf(mx[1][0], o1);
-          }
-          float mu[2];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float m = mx[r][0] * a.scale_log2;  // scale > 0
-            // raise the maximum in use only when the row's maximum has run ahead of it by more than kAtLazy
-            const bool raise = (m > m_run[r] + kAtLazy || m_run[r] == -CUDART_INF_F) && m != -CUDART_INF_F;
-            alpha[r] = raise ? at_ex2(m_run[r] - m) : 1.f;
-            m_run[r] = raise ? m : m_run[r];
-            mu[r] = (m_run[r] == -CUDART_INF_F) ? 0.f : m_run[r];
-          }
-          const bool rescale = j > g.j0 && __any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f);
-          if (gt >= 2 || rescale) {
-            // the product of two tiles ago must have finished: it read the P tile that is written below; the one before
-            // this tile's, too, where its sums are to be scaled (rare)
-            ok = gt < 2 || product_done(gt - 2);
-            if (rescale) ok = ok && product_done(gt - 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) {
-              if (lane == 0) give_up(45);
-              alive = false;
-              break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            if (rescale) {
-#pragma unroll
-              for (int c = 0; c < DH / 32; ++c) {
-                unsigned ov[16];
-                at_tmem_ld32(lane_base + kTtO + c * 32, ov);
-                asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-#pragma unroll
-                for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha[e & 1]);
-                at_tmem_st32(lane_base + kTtO + c * 32, ov);
+            for (int h = 0; h < 4; ++h) {
+              const int nb = upto - 32 * h;
+              unsigned w = nb <= 0 ? 0u : nb >= 32 ? ~0u : (1u << nb) - 1u;
+              if (a.mask) {
+                const int at_word = k0 / 64 + (h >> 1);
+                w &= at_word < a.words
+                         ? static_cast<unsigned>(a.mask[static_cast<size_t>(g.s.t0 + my_tok) * a.words + at_word] >> (32 * (h & 1))) : 0u;
               }
-              asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(w >> i & 1u)) v[32 * h + i] = __float_as_uint(-CUDART_INF_F);
+            }
+          } else if (valid < kAtKeys || base < my_lo) {
+#pragma unroll
+            for (int i = 0; i < kAtKeys; ++i)
+              if (base + i < my_lo || i >= valid) v[i] = __float_as_uint(-CUDART_INF_F);
+          }
+          float mx[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx[u] = fmaxf(__uint_as_float(v[u]), __uint_as_float(v[u + 4]));
+#pragma unroll
+          for (int i = 8; i < kAtKeys; i += 8)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) mx[u] = at_max3(mx[u], __uint_as_float(v[i + u]), __uint_as_float(v[i + u + 4]));
+          const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;  // scale > 0
+          // raise the maximum in use only when the row's maximum has run ahead of it by more than kAtLazy
+          const bool raise = (m > m_run + kAtLazy || m_run == -CUDART_INF_F) && m != -CUDART_INF_F;
+          const float alpha = raise ? at_ex2(m_run - m) : 1.f;
+          m_run = raise ? m : m_run;
+          const float mu = m_run == -CUDART_INF_F ? 0.f : m_run;
+          if (t > first && __any_sync(0xffffffffu, alpha != 1.f)) {
+            // (this set's product before is done: S, which came behind it, is)
+#pragma unroll
+            for (int c = 0; c < DH / 16; ++c) {
+              unsigned o[16];
+              tree_tmem_ld16(o_tmem + 16 * c, o);
+              asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tree_tmem_st16(o_tmem + 16 * c, o);
             }
           }
-          // P, two neighbouring keys a word
-          sum[0] = sum[1] = 0.f;
+          if (!my_turn()) break;
+          // P, two neighbouring keys a word, in the place of S
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float p0 = at_ex2(fmaf(__uint_as_float(v[2 * i + r]), a.scale_log2, -mu[r]));  // masked: ex2(-inf) = 0
-              const float p1 = at_ex2(fmaf(__uint_as_float(v[2 * (i + 16) + r]), a.scale_log2, -mu[r]));
-              sum[r] += p0;
-              sum[r] += p1;
-              v[2 * i + r] = at_pack(p0, p1);
-            }
-          tree_tmem_st(lane_base + kTtP + 64 * (gt & 1), v);
+          for (int i = 0; i < kAtKeys / 2; ++i) {
+            const float p0 = at_ex2(fmaf(__uint_as_float(v[2 * i]), a.scale_log2, -mu));  // masked: ex2(-inf) = 0
+            const float p1 = at_ex2(fmaf(__uint_as_float(v[2 * i + 1]), a.scale_log2, -mu));
+            sum[2 * (i & 1)] += p0;
+            sum[2 * (i & 1) + 1] += p1;
+            v[i] = at_pack(p0, p1);
+            if (i % 32 == 31) tmem_st32(s_tmem + i / 32 * 32, v + i / 32 * 32);
+          }
+          pass_turn();
+          l_run = l_run * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
           asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-        } else if (gt >= 2) {
-          // (a warp without rows keeps pace with the products: it must not be two phases ahead of any barrier)
-          ok = product_done(gt - 2);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) {
-            if (lane == 0) give_up(45);
-            alive = false;
-            break;
-          }
+        } else {
+          if (!my_turn()) break;
+          pass_turn();
         }
         asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_p[gt & 1]);
+        if (lane == 0) mbar_arrive(&bar_p[set]);
       }
+      if (WIDE && first > at)                             // (a set without rows passes its turns)
+        for (int t = at; t < g.unit + g.j1 && alive; ++t)
+          if (my_turn()) pass_turn();
       if (!alive) break;
-      if (!idle) take_sums();
       const TreeSeg now = g;
-      if (at < end) {  // the next stretch's queries: the products of this one's have read theirs
+      const int len = now.j1 - now.j0;                    // tiles of the stretch
+      at += len;
+      if (!WIDE) {
+        s_ml[seg & 1][set][row] = make_float2(m_run, l_run);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_ml);
+      }
+      if (at < end) {  // the next stretch's queries, as soon as the last S of this one has been made
         g = tree_seg(a, plan, at, end);
+        if (!wait(&bar_qfree, seg & 1)) break;
         queries(g);
       }
 
-      // ---- this stretch's result: O from tensor memory once the last product has finished
-      const bool whole = now.j0 == 0 && now.j1 == now.s.nt;
-      const bool row_ok[2] = {row0 < n_rows, row0 + 8 < n_rows};
-      float corr[2] = {1.f, 1.f};
-      if (a.sink != nullptr && whole) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if (!row_ok[r]) continue;
-          // a score without key or value that counts once; maxima are kept in units of log 2
-          const float sk = a.sink[now.hk * G + (now.rt * kTtRows + row0 + 8 * r) % G] * 1.4426950408889634f;
-          const float m_new = fmaxf(m_run[r], sk);
-          corr[r] = exp2f(m_run[r] - m_new);
-          l_run[r] = l_run[r] * corr[r] + exp2f(sk - m_new);
-          m_run[r] = m_new;
-        }
-      }
-      {
-        bool ok = product_done(gt - 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {
-          if (lane == 0) give_up(45);
-          alive = false;
-          break;
-        }
-      }
+      // ---- the stretch's result once the last products have finished: of every set's rows, or the two sets' parts joined, half of the columns each
+      if ((!WIDE && !wait(&bar_ml, seg & 1)) || !wait(&bar_done, seg & 1)) break;
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      const bool whole = now.j0 == 0 && now.j1 == now.s.nt;
       const bool repair = reinterpret_cast<volatile int*>(s_bad)[seg & 1] == seg;
       if (!idle) {
+        constexpr int kCols = WIDE ? DH : DH / 2;
+        const int col0 = WIDE ? 0 : set * kCols;
+        float m = m_run, l = l_run, w0 = 1.f, w1 = 1.f;   // maximum and sum, and what the two sets' parts are multiplied by
+        if (!WIDE) {
+          const float2 ml0 = s_ml[seg & 1][0][row], ml1 = s_ml[seg & 1][1][row];
+          m = fmaxf(ml0.x, ml1.x);
+          const float mu = m == -CUDART_INF_F ? 0.f : m;
+          w0 = at_ex2(ml0.x - mu);                        // (a set that saw no key: 0)
+          w1 = at_ex2(ml1.x - mu);
+          l = ml0.y * w0 + ml1.y * w1;
+        }
+        const int gr = now.rt * kRows + row, tk = gr / G, hq = now.hk * G + (gr - tk * G);
+        const bool row_ok = row < n_rows;
+        if (whole) {
+          if (a.sink != nullptr && row_ok) {
+            // a score without key or value that counts once; maxima are kept in units of log 2
+            const float sk = a.sink[hq] * 1.4426950408889634f;
+            const float m_new = fmaxf(m, sk), f = exp2f(m - m_new);
+            l = l * f + exp2f(sk - m_new);
+            w0 *= f;
+            w1 *= f;
+          }
+          const float inv = l == 0.f ? 0.f : 1.f / l;     // (NaN stays NaN)
+          w0 *= inv;
+          w1 *= inv;
+        }
+        // whose parts: its own, or both sets' (of a single tile, of the one whose turn it was)
+        const bool in0 = WIDE ? set == 0 : len > 1 || (((now.unit + now.j0 - begin) & 1) == 0), in1 = WIDE ? set == 1 : len > 1 || !in0;
         const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (now.j0 > 0 ? 0 : 1);
-        float inv[2];
+        float* part = a.part_o + (slot * kRows + row) * DH + col0;
+        bf16* out = a.out + (static_cast<size_t>(now.s.t0 + tk) * a.Hq + hq) * DH + col0;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) inv[r] = whole ? (l_run[r] == 0.f ? 0.f : corr[r] / l_run[r]) : 1.f;  // (NaN stays NaN)
+        for (int c = 0; c < kCols / 32; ++c) {
+          float o[32];
+          unsigned x[32];
+          const unsigned from = lane_base + kTtO + col0 + 32 * c;
 #pragma unroll
-        for (int c = 0; c < NSUB; ++c) {
-          unsigned o[32];
-          at_tmem_ld(lane_base + kTtO + c * 64, o);
-          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          __syncwarp();
+          if (in0) {
+            tmem_ld32(from, x);
+            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(x[e]) * w0;
+          }
+          if (in1) {
+            tmem_ld32(from + 128, x);
+            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = fmaf(__uint_as_float(x[e]), w1, o[e]);
+          }
           if (repair) {
             // values that are not finite, to the rows that see their keys
             for (int j = now.j0; j < now.j1; ++j) {
@@ -715,57 +793,40 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
               for (int k = 0; k < valid; ++k) {
                 const bf16* vr;
                 const int key = now.s.first + j * kAtKeys + k, node = (j - now.s.ctx_tiles) * kAtKeys + k;
+                bool see;
                 if (own) {
                   vr = a.v + (now.s.t0 + node) * a.ldv + now.hk * DH;
+                  see = a.mask ? node < 64 * a.words && (a.mask[static_cast<size_t>(now.s.t0 + my_tok) * a.words + (node >> 6)] >> (node & 63) & 1ull)
+                               : node <= my_tok;
                 } else {
                   const int page = min(max(a.block_table[static_cast<size_t>(now.seq) * a.max_blocks + key / a.page_size], 0), a.pages - 1);
                   vr = a.pool + ((static_cast<long long>(page) * 2 + 1) * a.page_size + key % a.page_size) * a.Hkv * DH + now.hk * DH;
+                  see = key >= my_lo;
                 }
+                if (!see) continue;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                  bool see;
-                  if (own)
-                    see = a.mask ? node < 64 * a.words && (a.mask[static_cast<size_t>(now.s.t0 + my_tok[r]) * a.words + (node >> 6)] >> (node & 63) & 1ull)
-                                 : node <= my_tok[r];
-                  else
-                    see = key >= my_lo[r];
-                  if (!see) continue;
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) {
-                    const float x = __bfloat162float(vr[c * 64 + 4 * i + k4]);
-                    if (!(fabsf(x) < CUDART_INF_F)) o[2 * i + r] = __float_as_uint(__uint_as_float(o[2 * i + r]) + x);
-                  }
+                for (int e = 0; e < 32; ++e) {
+                  const float y = __bfloat162float(vr[col0 + 32 * c + e]);
+                  if (!(fabsf(y) < CUDART_INF_F)) o[e] += y;
                 }
               }
             }
           }
-          if (whole) {
-            const unsigned sel = (k4 & 1) ? 0x3276u : 0x5410u;  // see at_pair
+          if (row_ok && whole) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int gr = now.rt * kTtRows + row0 + 8 * r, tk = gr / G;
-              unsigned* dst = reinterpret_cast<unsigned*>(a.out + (static_cast<size_t>(now.s.t0 + tk) * a.Hq + now.hk * G + (gr - tk * G)) * DH + c * 64) +
-                              (k4 & 1) * 2 + (k4 >> 1);
+            for (int e = 0; e < 32; e += 8)
+              *reinterpret_cast<uint4*>(out + 32 * c + e) = make_uint4(at_pack(o[e], o[e + 1]), at_pack(o[e + 2], o[e + 3]), at_pack(o[e + 4], o[e + 5]),
+                                                                      at_pack(o[e + 6], o[e + 7]));
+          } else if (row_ok) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const unsigned word = at_pair(__uint_as_float(o[4 * e + r]) * inv[r], __uint_as_float(o[4 * e + 2 + r]) * inv[r], sel);
-                if (row_ok[r]) dst[4 * e] = word;
-              }
-            }
-          } else {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              if (!row_ok[r]) continue;
-              float* dst = a.part_o + (slot * kTtRows + row0 + 8 * r) * DH + c * 64 + k4;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) dst[4 * i] = __uint_as_float(o[2 * i + r]);
-              if (c == 0 && k4 == 0) a.part_ml[slot * kTtRows + row0 + 8 * r] = make_float2(m_run[r], l_run[r]);
-            }
+            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(part + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
+        if (!whole && row_ok && (WIDE || set == 0)) a.part_ml[slot * kRows + row] = make_float2(m, l);
       }
-      // (the next stretch's first product into O comes behind this warp's arrival for its probabilities)
       asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_read);
     }
   }
 
@@ -794,7 +855,7 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const __grid_con
   plan.first = plan.held + a.n_seq;
   tree_plan<kTmThreads>(a, plan, s_red);  // (lengths and tables were there before the launch in front of this one passed its wait)
   pdl_wait();                                // (every block waits: the next launch takes this one's end for that of both)
-  const int total = plan.pre[a.n_seq];
+  const int total = plan.total;
   if (total == 0) return;
   const int shares = tree_shares(a, total);
   const int share = blockIdx.x + 1;
@@ -803,12 +864,12 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const __grid_con
   const TreeSeg g = tree_seg(a, plan, at, total);
   if (g.j0 == 0 || g.unit < tree_begin(share - 1, total, shares)) return;  // not cut here, or an earlier block's
   const int last = tree_block(g.unit + g.s.nt - 1, total, shares);
-  const int G = a.Hq / a.Hkv, n_rows = min(kTtRows, g.s.n_new * G - g.rt * kTtRows);
+  const int G = a.Hq / a.Hkv, n_rows = min(a.rows, g.s.n_new * G - g.rt * a.rows);
   constexpr int C4 = DH / 4;
   constexpr int kBatch = 4;
   for (int i = blockIdx.y * kTmThreads + threadIdx.x; i < n_rows * C4; i += gridDim.y * kTmThreads) {
     const int r = i / C4, d = (i % C4) * 4;
-    const int row = g.rt * kTtRows + r, tk = row / G, hq = g.hk * G + (row - tk * G);
+    const int row = g.rt * a.rows + r, tk = row / G, hq = g.hk * G + (row - tk * G);
     float mx = -CUDART_INF_F, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (a.sink != nullptr) {
@@ -822,8 +883,8 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const __grid_con
       for (int u = 0; u < kBatch; ++u) {
         const int c = min(c0 + u, last);
         const size_t slot = 2 * static_cast<size_t>(c) + (c == share - 1 ? 1 : 0);  // the unit's beginning ends its block's share
-        ml[u] = a.part_ml[slot * kTtRows + r];
-        x[u] = *reinterpret_cast<const float4*>(a.part_o + (slot * kTtRows + r) * DH + d);
+        ml[u] = a.part_ml[slot * a.rows + r];
+        x[u] = *reinterpret_cast<const float4*>(a.part_o + (slot * a.rows + r) * DH + d);
       }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
@@ -843,17 +904,16 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const __grid_con
   }
 }
 
-template <int DH>
+template <int DH, bool WIDE>
 int launch_tree_tc(const TreeMaps& maps, const TreeTcArgs& a, cudaStream_t stream) {
-  const size_t smem = tree_smem(DH) + tree_plan_bytes(a.n_seq);
-  auto kern = tree_attention_tc_kernel<DH>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+  const size_t smem = tree_smem(DH, WIDE) + tree_plan_bytes(a.n_seq);
+  auto kern = tree_attention_tc_kernel<DH, WIDE>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));  // (of the current device: at every call)
   if (e != cudaSuccess) return static_cast<int>(e);
   launch_pdl(kern, dim3(a.shares), dim3(kTtThreads), smem, stream, maps, a);
   const int st = launch_status();
   if (st != 0 || a.shares == 1) return st;
-  launch_pdl(tree_merge_kernel<DH>, dim3(a.shares - 1, kTtRows * DH / 4 / (2 * kTmThreads)), dim3(kTmThreads), tree_plan_bytes(a.n_seq), stream, a);
+  launch_pdl(tree_merge_kernel<DH>, dim3(a.shares - 1, a.rows * DH / 4 / (2 * kTmThreads)), dim3(kTmThreads), tree_plan_bytes(a.n_seq), stream, a);
   return launch_status();
 }
 
@@ -862,17 +922,17 @@ int launch_tree_tc(const TreeMaps& maps, const TreeTcArgs& a, cudaStream_t strea
 // Whether pmm_tree_attention_tc takes this shape.
 PMM_EXPORT int pmm_tree_attention_tc_supported(int Hq, int Hkv, int Dh, int page_size, long long pages, int n_seq) {
   if (Hkv <= 0 || Hq % Hkv) return 0;
-  return ((Dh == 64 || Dh == 128) && page_size > 0 && page_size % 16 == 0 && pages > 0 && pages * 2 * page_size <= 0x7fffffffll && n_seq <= pmm::kTtSeqs)
+  return ((Dh == 64 || Dh == 128) && page_size > 0 && page_size % 8 == 0 && pages > 0 && pages * 2 * page_size <= 0x7fffffffll && n_seq <= pmm::kTtSeqs)
              ? 1 : 0;
 }
 
-// Floats of scratch for `sms` multiprocessors: two parts a block of 128 rows of 128 values, maximum and sum.
-PMM_EXPORT long long pmm_tree_attention_scratch(int sms) { return static_cast<long long>(sms) * 2 * pmm::kTtRows * (128 + 2); }
+// Floats of scratch for `sms` multiprocessors: two parts a block of 256 rows of 128 values, maximum and sum.
+PMM_EXPORT long long pmm_tree_attention_scratch(int sms) { return static_cast<long long>(sms) * 2 * 2 * pmm::kTtRows * (128 + 2); }
 
 PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* pool,
                                      int pages, const int* block_table, int max_blocks, const int* held, const int* cu, const int* positions,
                                      const void* mask, int words, const float* sink, void* out, float scale, int window, int page_size, int n_seq,
-                                     int T, int Hq, int Hkv, int Dh, float* scratch, int sms, int* status, cudaStream_t stream) {
+                                     int T, int Hq, int Hkv, int Dh, int wide, float* scratch, int sms, int* status, cudaStream_t stream) {
   if (T <= 0 || n_seq <= 0) return 0;
   if (!pmm_tree_attention_tc_supported(Hq, Hkv, Dh, page_size, pages, n_seq) || max_blocks <= 0 || !(scale > 0.f) || (window != 0 && !positions) ||
       (mask && words < 1) || !scratch || sms < 1 || !status)
@@ -882,8 +942,8 @@ PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k
   if (ldq % 8 || ldk % 8 || ldv % 8) return PMM_ERR_BAD_ARGUMENT;
   pmm::EncodeTiledFn fn = pmm::encode_tiled_fn();
   if (!fn) return PMM_ERR_BAD_ARGUMENT;
-  const int box = page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : 16;
-  const long long kv_dim = static_cast<long long>(Hkv) * Dh, pool_rows = static_cast<long long>(pages) * 2 * page_size;
+  const int box = page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : page_size % 16 == 0 ? 16 : 8;
+  const long long kv_dim = static_cast<long long>(Hkv) * Dh;
   pmm::TreeMaps maps;
   bool ok = true;
   auto encode = [&](CUtensorMap* map, const void* base, long long n, long long ld, int box_rows) {
@@ -894,15 +954,10 @@ PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k
     ok = ok && fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
-  const pmm::bf16 *pool_b = static_cast<const pmm::bf16*>(pool), *k_b = static_cast<const pmm::bf16*>(k);
   if (T == 1) ldk = ldv = kv_dim;  // (a matrix of one row has no stride of its own)
-  encode(&maps.pool_v, pool, pool_rows, kv_dim, box);
+  encode(&maps.pool, pool, static_cast<long long>(pages) * 2 * page_size, kv_dim, box);
+  encode(&maps.own_k, k, T, ldk, pmm::kAtBox);
   encode(&maps.own_v, v, T, ldv, pmm::kAtBox);
-  for (int e = 0; e < 2; ++e) {
-    encode(&maps.pool_k[e], pool_b + e * kv_dim, pool_rows / 2, 2 * kv_dim, box / 2);
-    const int odd = T > 1 ? e : 0;  // (of a single row there are no odd ones, and none is asked for)
-    encode(&maps.own_k[e], k_b + odd * ldk, (T + 1 - odd) / 2, 2 * ldk, pmm::kAtBox / 2);
-  }
   if (!ok) return PMM_ERR_BAD_ARGUMENT;
   pmm::TreeTcArgs a{};
   a.q = static_cast<const pmm::bf16*>(q);
@@ -921,8 +976,9 @@ PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k
   a.sink = sink;
   a.out = static_cast<pmm::bf16*>(out);
   a.shares = sms;
+  a.rows = wide ? 2 * pmm::kTtRows : pmm::kTtRows;
   a.part_o = scratch;
-  a.part_ml = reinterpret_cast<float2*>(scratch + static_cast<size_t>(a.shares) * 2 * pmm::kTtRows * Dh);
+  a.part_ml = reinterpret_cast<float2*>(scratch + static_cast<size_t>(a.shares) * 2 * a.rows * Dh);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.window = window;
   a.page_size = page_size;
@@ -933,5 +989,6 @@ PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k
   a.Hkv = Hkv;
   a.min_tiles = 2;
   a.status = status;
-  return Dh == 64 ? pmm::launch_tree_tc<64>(maps, a, stream) : pmm::launch_tree_tc<128>(maps, a, stream);
+  if (Dh == 64) return wide ? pmm::launch_tree_tc<64, true>(maps, a, stream) : pmm::launch_tree_tc<64, false>(maps, a, stream);
+  return wide ? pmm::launch_tree_tc<128, true>(maps, a, stream) : pmm::launch_tree_tc<128, false>(maps, a, stream);
 }

@@ -191,7 +191,7 @@ _SIGNATURES = {
     "pmm_tree_attention_scratch": [c_int],
     "pmm_tree_attention_tc": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p,
                               c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
-                              c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
+                              c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
     "pmm_verify_scratch": [c_longlong, c_int],
     "pmm_verify_drafts": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
                           c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p],
@@ -2471,7 +2471,9 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: T
             held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words, _ptr(sink), out.data_ptr(), softmax_scale, window,
             pool.shape[2], n_seq, T, n_q_heads, n_kv_heads, head_dim)
     if dtype is torch.bfloat16 and _fn("pmm_tree_attention_tc_supported")(n_q_heads, n_kv_heads, head_dim, pool.shape[2], pool.shape[0], n_seq):
-        _call("pmm_tree_attention_tc", *args, scratch.data_ptr(), sms, _tc_status(q.device).data_ptr(), stream)
+        # units of 256 rows (token, query head of a group) where the requests bring more than 128 on average: K and V once for them
+        wide = T * (n_q_heads // n_kv_heads) > 128 * n_seq
+        _call("pmm_tree_attention_tc", *args, wide, scratch.data_ptr(), sms, _tc_status(q.device).data_ptr(), stream)
     else:
         _call("pmm_tree_attention", *args, _dt(q), stream)
 
