@@ -26,6 +26,8 @@
 #include "attention_tc.cuh"
 #include <math_constants.h>
 
+#include <type_traits>
+
 namespace pmm {
 
 constexpr int kTtSeqs = 1024;  // requests whose lengths fit shared memory
@@ -34,30 +36,55 @@ constexpr int kTtThreads = 12 * 32;  // copies, two warps that issue, one withou
 // tensor memory: S (and P) of the two sets of warps, O of the two
 constexpr unsigned kTtO = 256, kTtCols = 512;
 __host__ __device__ constexpr int tree_q_sub() { return kTtRows * kAtDhBlock * 2; }        // a sub-tile of Q: 64 head-size columns
-// tiles in flight (16 or 32 KB each): what the queries leave of shared memory
-// K_j is copy 2 j, V_j copy 2 j + 1 of the block, in slot (copy % ring).  The ring is a multiple of 4, so that all copies of a slot are of one
-// kind and, where the sets take the tiles in turn, of one set: who waits for a slot has seen the copy before in it land (a barrier
-// tells a copy only from the one before, and a wait that skips one may take the last but one for its own).
-__host__ __device__ constexpr int tree_ring(int dh) { return dh == 64 ? 8 : 4; }
+// Tiles in flight (16 or 32 KB each): what queries and lengths leave of shared memory.  K_j is copy 2 j, V_j copy 2 j + 3 of the block (the order in which they
+// are asked for; there is no copy 1), in slot (copy % ring).  A copy's barrier tells it only from the one before on that barrier, and a wait that skips one may take the last but one for
+// its own; so there are as many barriers as make all copies of one to be of one kind and, where the sets take the tiles in turn, of one set.
+__host__ __device__ constexpr int tree_ring(int dh, bool wide) { return dh == 64 ? 11 : wide ? 4 : 5; }
+__host__ __device__ constexpr int tree_bars(int ring) { return ring % 4 == 0 ? ring : 4 * ring; }
 __host__ __device__ constexpr size_t tree_smem(int dh, bool wide) {
-  return static_cast<size_t>(dh / kAtDhBlock) * ((wide ? 2 : 1) * tree_q_sub() + tree_ring(dh) * kAtKvSub) + 1024 /*alignment*/;
+  return static_cast<size_t>(dh / kAtDhBlock) * ((wide ? 2 : 1) * tree_q_sub() + tree_ring(dh, wide) * kAtKvSub) + 1024 /*alignment*/;
 }
 
 // S = Q K^T: both K-major; O += P V: V as it lies in the cache (MN-major), all DH columns at once.
-constexpr unsigned kTtIdescS = at_idesc_s(kTtRows);
+constexpr int kTtHalf = kAtKeys / 2;  // keys of an S product
+constexpr unsigned kTtIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<unsigned>(kTtHalf >> 3) << 17) | (static_cast<unsigned>(kTtRows >> 4) << 24);
 __host__ __device__ constexpr unsigned tree_idesc_o(int dh) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (static_cast<unsigned>(dh >> 3) << 17) | (static_cast<unsigned>(kTtRows >> 4) << 24);
 }
-// A product whose A operand lies in tensor memory (row i in lane i, two neighbouring elements a column).
-__device__ __forceinline__ void umma_ts_lead(unsigned tmem_d, unsigned tmem_a, unsigned long long b_desc, unsigned idesc, unsigned accumulate, unsigned lead) {
+// Products and commits by one elected thread of a warp that is here as a whole, the same one every time.  elect.sync is how the compiler learns that a
+// single thread issues: a commit takes 8 clocks, with a predicate (lane == 0) 55, and eight products 312 or fewer, not 401.
+__device__ __forceinline__ void tree_mma_ss(unsigned tmem_d, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
   asm volatile(
       "{\n\t.reg .pred p, l;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 l, %5, 0;\n\t"
+      "elect.sync _|l, 0xffffffff;\n\t"
+      "@l tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+      :
+      : "r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// (the A operand in tensor memory: row i in lane i, two neighbouring elements a column)
+__device__ __forceinline__ void tree_mma_ts(unsigned tmem_d, unsigned tmem_a, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, l;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync _|l, 0xffffffff;\n\t"
       "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
       :
-      : "r"(tmem_d), "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "r"(tmem_d), "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+__device__ __forceinline__ void tree_commit(unsigned long long* bar) {
+  asm volatile(
+      "{\n\t.reg .pred l;\n\t"
+      "elect.sync _|l, 0xffffffff;\n\t"
+      "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+
+// 16 bytes to shared memory, or zeros.
+__device__ __forceinline__ void cp_async16_fill(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
 // 32 lanes of tensor memory x 16 columns, a lane a row.
@@ -99,8 +126,9 @@ struct TreeTcArgs {
   int words;
   const float* sink;
   bf16* out;
-  float* part_o;        // [2 * blocks][rows][DH]
+  float4* part_o;       // [2 * blocks][DH / 4][rows]: neighbouring threads, a row each, write neighbouring places
   float2* part_ml;      // [2 * blocks][rows]
+  int* cuts;            // [blocks][8]: a unit that shares cut: its rows (0: none), first token, head, row tile, last block
   float scale_log2;
   int window, page_size, box, n_seq, T, Hq, Hkv, shares, min_tiles;
   int rows;             // of a unit: 128 or 256
@@ -248,14 +276,14 @@ __device__ __forceinline__ int tree_valid(const TreeSeq& s, int j) {
 template <int DH, bool WIDE>
 __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const __grid_constant__ TreeMaps maps, const __grid_constant__ TreeTcArgs a) {
   constexpr int NSUB = DH / kAtDhBlock;
-  constexpr int kRing = tree_ring(DH);
+  constexpr int kRing = tree_ring(DH, WIDE), kBars = tree_bars(kRing);
   constexpr int kRows = WIDE ? 2 * kTtRows : kTtRows;  // of a unit
   constexpr int kSlot = NSUB * kAtKvSub;
   constexpr int kQSub = tree_q_sub();
   extern __shared__ unsigned char smem_raw[];
   // the queries are in place / have been read by a unit's last S; a slot is full / empty; a set's S and P are there; a unit's last
   // products are done; both sets' maxima and sums are there; both have read their O; it is a set's turn to make its exponentials
-  __shared__ __align__(8) unsigned long long bar_q, bar_qfree, bar_full[kRing], bar_empty[kRing], bar_s[2], bar_p[2], bar_turn[2], bar_done, bar_ml, bar_read;
+  __shared__ __align__(8) unsigned long long bar_q, bar_qfree, bar_full[kBars], bar_empty[kRing], bar_s[2][2], bar_p[2][2], bar_o[2], bar_done, bar_ml, bar_read;
   __shared__ float2 s_ml[2][2][kTtRows];  // (of two stretches in turn: one set may be a stretch ahead)
   __shared__ unsigned s_tmem_base;
   __shared__ int s_abort, s_red[32], s_bad[2];
@@ -274,20 +302,22 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
   if (tid == 0) {
     mbar_init(&bar_q, 8);
     mbar_init(&bar_qfree, 2);
-#pragma unroll
-    for (int i = 0; i < kRing; ++i) {
-      mbar_init(&bar_full[i], 1);
-      mbar_init(&bar_empty[i], WIDE ? 2 : 1);
-    }
+    for (int i = 0; i < kBars; ++i) mbar_init(&bar_full[i], 1);
+    for (int i = 0; i < kRing; ++i) mbar_init(&bar_empty[i], WIDE ? 2 : 1);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar_s[i], 1);
-      mbar_init(&bar_p[i], 4);
-      mbar_init(&bar_turn[i], 4);
+      mbar_init(&bar_o[i], 1);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&bar_s[i][h], 1);
+        mbar_init(&bar_p[i][h], 4);
+      }
     }
     mbar_init(&bar_done, 2);
     mbar_init(&bar_ml, 8);
     mbar_init(&bar_read, 8);
+    mbar_arrive(&bar_full[1]);  // (copy 1, which is none, has come and gone)
+    for (int i = 0; i < (WIDE ? 2 : 1); ++i) mbar_arrive(&bar_empty[1]);
     s_abort = 0;
     s_bad[0] = s_bad[1] = -1;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -295,30 +325,30 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
   }
   pdl_wait();
   pdl_launch_dependents();  // (behind the wait: the merge reads the lengths ahead of its own)
-  tree_plan<kTtThreads>(a, plan, s_red);
-  const int total = plan.total;
-  const int shares = tree_shares(a, total);
-  if (static_cast<int>(blockIdx.x) >= shares || total == 0) return;
-  const int begin = tree_begin(blockIdx.x, total, shares), end = tree_begin(blockIdx.x + 1, total, shares);
-  const int n_tiles = end - begin;  // (at least one)
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem_base)), "r"(kTtCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-  __syncthreads();
+  tree_plan<kTtThreads>(a, plan, s_red);
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const unsigned tmem_base = s_tmem_base;
+  const int total = plan.total;
+  const int shares = tree_shares(a, total);
+  int* record = a.cuts + 8 * blockIdx.x;  // of the unit that is cut at this block's first tile, for the merge
+  if (static_cast<int>(blockIdx.x) >= shares || total == 0) {
+    if (tid == 0) record[0] = 0;
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(kTtCols) : "memory");
+    return;
+  }
+  const int begin = tree_begin(blockIdx.x, total, shares), end = tree_begin(blockIdx.x + 1, total, shares);
+  const int n_tiles = end - begin;  // (at least one)
   volatile int* abort_flag = &s_abort;
   auto give_up = [&](int code) {
     if (!*abort_flag) atomicExch(a.status, code);
     s_abort = 1;
   };
 
-  // The block is launched with 168 registers a thread, 64,512 in all: 96 for the first four warps, 200 for the softmax warps, whose 128
-  // scores a thread do not fit otherwise (128 * 96 + 256 * 200 = 63,488).
-  if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer (the whole warp walks, a lane a box)
     const int page_size = a.page_size;
@@ -330,7 +360,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
       bool own;            // the step's own tokens
     };
     auto request = [&](const Tile& t, bool is_v) {
-      const int item = is_v ? 2 * n_v + 1 : 2 * n_k, slot = item % kRing;
+      const int item = is_v ? 2 * n_v + 3 : 2 * n_k, slot = item % kRing;
       if (item >= kRing && ok) {
         int got = 1;
         if (lane == 0) got = mbar_wait(&bar_empty[slot], (item / kRing - 1) & 1, abort_flag) ? 1 : 0;
@@ -340,13 +370,14 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
       if (!ok) return;
       const int keys = t.own ? kAtBox : a.box;  // of a box
       const int boxes = (t.valid + keys - 1) / keys;
-      if (lane == 0) mbar_expect_tx(&bar_full[slot], static_cast<unsigned>(boxes * keys * NSUB * 128));
+      unsigned long long* full = &bar_full[item % kBars];
+      if (lane == 0) mbar_expect_tx(full, static_cast<unsigned>(boxes * keys * NSUB * 128));
       __syncwarp();
       const int d = lane % NSUB, b = lane / NSUB;  // a lane a copy: sub-tile of 64 columns, box
       const int row = __shfl_sync(0xffffffffu, t.row, b);
       if (b < boxes)
         tma_load_2d(sRing + slot * kSlot + d * kAtKvSub + b * keys * 128, t.own ? (is_v ? &maps.own_v : &maps.own_k) : &maps.pool,
-                    t.hk * DH + d * kAtDhBlock, row + (is_v && !t.own ? page_size : 0), &bar_full[slot]);
+                    t.hk * DH + d * kAtDhBlock, row + (is_v && !t.own ? page_size : 0), full);
       ++(is_v ? n_v : n_k);
     };
     Tile prev{};
@@ -382,10 +413,12 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
     __syncwarp();
     if (lane == 0 && s_abort) {
       // copies already requested still write into this block's shared memory: wait for them
+      const int items = 2 * max(n_k, n_v) + 3;
       for (int u = 0; u < kRing; ++u) {  // the last copy of every slot
-        const int last = (u & 1) ? 2 * (n_v - 1) + 1 : 2 * (n_k - 1), it = last - (last - u + kRing) % kRing;
+        int it = items - 1;
+        while (it >= 0 && (it % kRing != u || ((it & 1) ? it == 1 || (it - 3) / 2 >= n_v : it / 2 >= n_k))) --it;
         if (it < 0) continue;
-        for (unsigned i = 0; i < kSpinLimit && !mbar_try_wait(&bar_full[it % kRing], (it / kRing) & 1); ++i) {
+        for (unsigned i = 0; i < kSpinLimit && !mbar_try_wait(&bar_full[it % kBars], (it / kBars) & 1); ++i) {
         }
       }
     }
@@ -395,33 +428,24 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
     // What the products are issued with, and everything that decides whether they are, comes out of a reduction or a vote: it is known to
     // be the same in the whole warp and stays in uniform registers (130 to 180 clocks a product where it is not, 64 where it is).
     auto uniform = [](unsigned x) { return static_cast<int>(__reduce_max_sync(0xffffffffu, x)); };
-    const int n = uniform(n_tiles), items = 2 * n;
+    const int n = uniform(n_tiles);
     const unsigned tmem = uniform(tmem_base), s_tmem = tmem + kAtKeys * set, o_tmem = tmem + kTtO + 128 * set;
-    const unsigned lead = lane == 0 ? 1u : 0u;
     const unsigned long long q_desc = umma_desc(sQ + (WIDE ? set * NSUB * kQSub : 0)), ring_desc = umma_desc(sRing);
     // (of a V tile: 64 columns further lie one sub-tile further)
     const unsigned long long v_ring = (ring_desc & ~(0x3fffull << 16)) | (static_cast<unsigned long long>(kAtKvSub >> 4) << 16);
     auto wait = [&](unsigned long long* bar, unsigned parity) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;  // (no lane may fall a phase behind)
     };
-    auto full = [&](int it) { return wait(&bar_full[it % kRing], (it / kRing) & 1); };
-    // a slot's copy has been used (nobody waits for the last copies' slots); by a set without rows, at once
-    auto used = [&](int it, bool rows) {
-      if (it + kRing < items) {
-        if (rows)
-          umma_commit_lead(&bar_empty[it % kRing], lead);
-        else if (lane == 0)
-          mbar_arrive(&bar_empty[it % kRing]);
-      }
-    };
     constexpr int kStep = WIDE ? 1 : 2;
     // The set's tiles, stretch by stretch.  Two walks over them: of the S products and, a tile behind, of the P V.  (A set has tiles in
     // every stretch but those of one tile, and no two of those without one follow one another.)  Tiles are counted within the block.
     struct Walk {
       int seg, t, end;               // the stretch's number, the next tile, the stretch's end
+      int h;                         // the next half of it
       int live, in, rows;            // in: its queries are in place; rows: the set has some (of 256, the second may have none)
       int own, last;                 // the unit's first tile of the step's own tokens, its last tile
       int ctx_steps, last_steps;     // sixteens of keys in the last tile of cached keys, and in the last of all
+      int slot, bar, phase;          // of the tile's copy
     };
     auto load = [&](Walk& w, int at) {
       const TreeSeg g = tree_seg(a, plan, at, end);
@@ -441,86 +465,167 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
         ++w.seg;
       }
     };
-    Walk ws;
+    auto next = [&](Walk& w) {  // the set's next tile
+      w.t += kStep;
+      w.slot += 2 * kStep;
+      w.slot = w.slot >= kRing ? w.slot - kRing : w.slot;
+      w.bar += 2 * kStep;
+      w.phase = w.bar >= kBars ? w.phase ^ 1 : w.phase;
+      w.bar = w.bar >= kBars ? w.bar - kBars : w.bar;
+    };
+    Walk ws, wp;
     ws.seg = ws.in = 0;
     ws.t = WIDE ? 0 : set;
+    ws.h = 0;
     ws.live = 1;
+    ws.slot = ws.bar = WIDE ? 0 : 2 * set;  // (copy 2 t)
+    ws.phase = 0;
     load(ws, begin);
-    Walk wp = ws;
-    auto enter = [&]() {
-      if (!ws.in) ws.in = wait(&bar_q, ws.seg & 1);
-      return ws.in != 0;
+    wp = ws;
+    const int first_v = 2 * wp.t + 3;       // (copy 2 t + 3)
+    wp.slot = first_v % kRing;
+    wp.bar = first_v % kBars;
+    wp.phase = first_v / kBars & 1;
+    auto steps_of = [](const Walk& w) { return w.t == w.own - 1 ? w.ctx_steps : w.t == w.last ? w.last_steps : kAtKeys / 16; };
+    auto full = [&](const Walk& w) { return wait(&bar_full[w.bar], w.phase); };
+    // a slot's copy has been used (by a set without rows, at once)
+    auto used = [&](const Walk& w) {
+      if (w.rows)
+        tree_commit(&bar_empty[w.slot]);
+      else if (lane == 0)
+        mbar_arrive(&bar_empty[w.slot]);
     };
-    auto issue_s = [&]() {  // the next S, where there is one
-      while (ws.live && ws.t >= ws.end) {  // (a stretch without a tile of this set)
-        if (!enter()) return false;
-        umma_commit_lead(&bar_qfree, lead);
-        leave(ws);
-      }
-      if (!ws.live) return true;
-      const int item = 2 * ws.t, slot = item % kRing;
-      if (!enter() || !full(item)) return false;
-      if (ws.rows) {
-        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        const unsigned long long k_desc = ring_desc + static_cast<unsigned>(slot * (kSlot >> 4));
+    auto product_s = [&](const Walk& w, int h) {
+      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      const unsigned long long k_desc = ring_desc + static_cast<unsigned>(w.slot * (kSlot >> 4) + h * (kTtHalf * 128 >> 4));
 #pragma unroll
-        for (int k = 0; k < DH / 16; ++k)
-          umma_f16_lead(s_tmem, q_desc + (k >> 2) * (kQSub >> 4) + 2 * (k & 3), k_desc + (k >> 2) * (kAtKvSub >> 4) + 2 * (k & 3), kTtIdescS,
-                        k > 0 ? 1u : 0u, lead);
-        umma_commit_lead(&bar_s[set], lead);
+      for (int k = 0; k < DH / 16; ++k)
+        tree_mma_ss(s_tmem + kTtHalf * h, q_desc + (k >> 2) * (kQSub >> 4) + 2 * (k & 3), k_desc + (k >> 2) * (kAtKvSub >> 4) + 2 * (k & 3), kTtIdescS,
+                    k > 0 ? 1u : 0u);
+      tree_commit(&bar_s[set][h]);
+    };
+    auto product_o = [&](const Walk& w, int h, int sixteens, int more) {
+      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      const unsigned long long v_desc = v_ring + static_cast<unsigned>(w.slot * (kSlot >> 4) + h * (kTtHalf * 128 >> 4));
+      auto product = [&](int k) {  // 16 keys: 16 rows of 128 bytes of every sub-tile
+        tree_mma_ts(o_tmem, s_tmem + kTtHalf * h + 8 * k, v_desc + ((k * 16 * 128) >> 4), tree_idesc_o(DH), k > 0 ? 1u : static_cast<unsigned>(more));
+      };
+      if (sixteens == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) product(k);
+      } else {
+        for (int k = 0; k < sixteens; ++k) product(k);
       }
-      used(item, ws.rows);
-      ws.t += kStep;
-      if (ws.t >= ws.end) {  // the stretch's last of this set: its queries may make way
-        umma_commit_lead(&bar_qfree, lead);
-        leave(ws);
+      tree_commit(&bar_o[set]);
+    };
+    int taken = 0;  // bit h: the place of half h holds an S or P that has not been used
+    // Every next S whose place is free; another stretch's once all products of this one have been issued (its queries wait for what waits for them).
+    auto issue_s = [&]() {
+      while (ws.live) {
+        if (!ws.in) {
+          if (taken) return true;
+          if (!wait(&bar_q, ws.seg & 1)) return false;
+          ws.in = 1;
+        }
+        if (ws.t >= ws.end) {  // the set's last of the stretch, or none in it: its queries may make way
+          tree_commit(&bar_qfree);
+          leave(ws);
+          continue;
+        }
+        if (taken >> ws.h & 1) return true;
+        if (ws.h == 0 && !full(ws)) return false;
+        if (ws.rows) product_s(ws, ws.h);
+        taken |= 1 << ws.h;
+        if (ws.h == 0 && steps_of(ws) > 4) {
+          ws.h = 1;
+        } else {
+          used(ws);
+          ws.h = 0;
+          next(ws);
+        }
       }
       return true;
     };
-    int code = issue_s() ? 0 : 43, n_p = 0;  // tiles of P used
+    int code = issue_s() ? 0 : 43, n_p = 0;  // bit h: the parity of the next P of half h
     int more = 0, told = 0;                  // O goes on; the stretch's end has been told
     while (code == 0 && wp.live) {
       if (wp.t >= wp.end) {
-        if (!told) umma_commit_lead(&bar_done, lead);
+        if (!told) tree_commit(&bar_done);
         told = more = 0;
         const int left = wp.seg;
         leave(wp);
         if (wp.live && !wait(&bar_read, left & 1)) code = 44;  // (its O has been read)
         continue;
       }
-      const int item = 2 * wp.t + 1, slot = item % kRing;
-      if (!full(item) || (wp.rows && !wait(&bar_p[set], n_p & 1))) {
+      // Whole tiles with another of the stretch behind them, both halves of their S made: the same without questions (2,390 clocks for half a
+      // tile of both sets with them; a warp's way through branches costs more than the products that it issues).
+      if (ws.rows && taken == 3 && ws.in && ws.seg == wp.seg && ws.t == wp.t + kStep) {
+        int until = wp.end;  // the first tile that is not whole, or the end
+        if (wp.ctx_steps < 8 && wp.t < wp.own) until = min(until, wp.own - 1);
+        if (wp.last_steps < 8) until = min(until, wp.last);
+        for (; ws.t < until && code == 0;) {
+          if (!full(wp) || !wait(&bar_p[set][0], n_p & 1)) {
+            code = 44;
+            break;
+          }
+          product_o(wp, 0, 4, more);
+          more = 1;
+          if (!full(ws)) {
+            code = 43;
+            break;
+          }
+          product_s(ws, 0);
+          if (!wait(&bar_p[set][1], n_p >> 1)) {
+            code = 44;
+            break;
+          }
+          product_o(wp, 1, 4, 1);
+          tree_commit(&bar_empty[wp.slot]);
+          product_s(ws, 1);
+          tree_commit(&bar_empty[ws.slot]);
+          n_p ^= 3;
+          next(wp);
+          next(ws);
+        }
+        if (code != 0) break;
+        if (!issue_s()) {  // (the stretch's queries may make way)
+          code = 43;
+          break;
+        }
+      }
+      const int steps = steps_of(wp);
+      if (!full(wp)) {
         code = 44;
         break;
       }
-      if (wp.rows) {
-        ++n_p;
-        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        const int steps = wp.t == wp.own - 1 ? wp.ctx_steps : wp.t == wp.last ? wp.last_steps : kAtKeys / 16;
-        const unsigned long long v_desc = v_ring + static_cast<unsigned>(slot * (kSlot >> 4));
-        auto product = [&](int k) {  // 16 keys: 16 rows of 128 bytes of every sub-tile
-          umma_ts_lead(o_tmem, s_tmem + 8 * k, v_desc + ((k * 16 * 128) >> 4), tree_idesc_o(DH), k > 0 ? 1u : static_cast<unsigned>(more), lead);
-        };
-        if (steps == kAtKeys / 16) {
-#pragma unroll
-          for (int k = 0; k < kAtKeys / 16; ++k) product(k);
-        } else {
-          for (int k = 0; k < steps; ++k) product(k);
+#pragma unroll 1
+      for (int h = 0; h < (steps > 4 ? 2 : 1); ++h) {
+        if (wp.rows) {
+          if (!wait(&bar_p[set][h], n_p >> h & 1)) {
+            code = 44;
+            break;
+          }
+          n_p ^= 1 << h;
+          product_o(wp, h, min(4, steps - 4 * h), more);
+        }
+        taken &= ~(1 << h);
+        more = 1;
+        if (h == 1 || steps <= 4) {
+          used(wp);
+          next(wp);
+          if (wp.t >= wp.end) {
+            tree_commit(&bar_done);
+            told = 1;
+          }
+        }
+        if (!issue_s()) {
+          code = 43;
+          break;
         }
       }
-      used(item, wp.rows);
-      more = 1;
-      wp.t += kStep;
-      if (wp.t >= wp.end) {
-        umma_commit_lead(&bar_done, lead);
-        told = 1;
-      }
-      if (!issue_s()) code = 43;  // (into the S whose P has just been used: products run in order)
     }
     if (code != 0) give_up(code);
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
+  } else if (warp >= 4) {
     // ---------------------------------------------------------------- softmax and output (a thread a row, two sets of warps)
     const int set = (warp - 4) >> 2, quarter = warp & 3;
     const int row = (WIDE ? set * kTtRows : 0) + quarter * 32 + lane;  // of the unit (quarter * 32 + lane: its lane of tensor memory)
@@ -540,41 +645,28 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
     auto queries = [&](const TreeSeg& g) {
       const int n_rows = min(kRows, g.s.n_new * G - g.rt * kRows);
       constexpr int kPieces = DH / 8;
-      for (int p0 = soft_tid; p0 < kRows * kPieces; p0 += 1024) {  // neighbouring lanes take neighbouring pieces
-        uint4 x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int p = p0 + 256 * i, r = p / kPieces, c = p % kPieces;
-          const int gr = g.rt * kRows + r, tk = gr / G;
-          x[i] = r < n_rows ? *reinterpret_cast<const uint4*>(a.q + (g.s.t0 + tk) * a.ldq + (g.hk * G + (gr - tk * G)) * DH + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int p = p0 + 256 * i, r = p / kPieces, c = p % kPieces;
-          *reinterpret_cast<uint4*>(sQ + ((r >> 7) * NSUB + (c >> 3)) * kQSub + at_swizzled(r & 127, c & 7)) = x[i];
-        }
+#pragma unroll 4
+      for (int p = soft_tid; p < kRows * kPieces; p += 256) {  // neighbouring lanes take neighbouring pieces
+        const int r = p / kPieces, c = p % kPieces, gr = g.rt * kRows + r, tk = gr / G;
+        const bf16* src = r < n_rows ? a.q + (g.s.t0 + tk) * a.ldq + (g.hk * G + (gr - tk * G)) * DH + c * 8 : a.q;
+        cp_async16_fill(sQ + ((r >> 7) * NSUB + (c >> 3)) * kQSub + at_swizzled(r & 127, c & 7), src, r < n_rows);
       }
+      asm volatile("cp.async.wait_all;\n" ::: "memory");
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar_q);
     };
-    int n_s = 0;                                          // tiles of S that this set has taken
-    // The sets make their exponentials in turn, the first set first: side by side they share the units, and both then wait for their
-    // products at the same time (5,850 clocks a tile of both sets; in turn XX).
-    int n_turn = 0;
-    auto my_turn = [&]() {
-      if (set == 1 || n_turn > 0) {
-        if (!wait(&bar_turn[set], (set == 1 ? n_turn : n_turn - 1) & 1)) return false;
-      }
-      ++n_turn;
-      return true;
-    };
-    auto pass_turn = [&]() {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar_turn[set ^ 1]);
-    };
+    int n_s = 0, n_half = 0;                              // bit h: the parity of the next S of half h; halves that this set has taken
     TreeSeg g = tree_seg(a, plan, begin, end);
     queries(g);
+    if (soft_tid == 0) {  // (the block behind the one in which the unit begins tells the merge)
+      const bool cut = g.j0 > 0 && g.unit >= tree_begin(blockIdx.x - 1, total, shares);
+      record[0] = cut ? min(kRows, g.s.n_new * G - g.rt * kRows) : 0;
+      record[1] = g.s.t0;
+      record[2] = g.hk;
+      record[3] = g.rt;
+      record[4] = tree_block(g.unit + g.s.nt - 1, total, shares);
+    }
     for (int seg = 0, at = begin; at < end && alive; ++seg) {
       const int n_rows = min(kRows, g.s.n_new * G - g.rt * kRows);
       const bool idle = (WIDE ? set * kTtRows : 0) + quarter * 32 >= n_rows;           // (the whole warp: none of its rows exists)
@@ -597,13 +689,13 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
         const bool own = j >= g.s.ctx_tiles;
         const int base = g.s.first + j * kAtKeys;         // (cached keys)
         const int valid = tree_valid(g.s, j);
-        if (!wait(&bar_s[set], n_s++ & 1)) break;
+        if (!wait(&bar_s[set][0], n_s & 1)) break;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         if (valid % 16 != 0 || mixed(g, j)) {
           // values that must not meet a probability of zero: rows behind the last valid one become zero; where rows see the
           // keys differently, so do values that are not finite
-          const int item = 2 * gt + 1, slot = item % kRing;
-          if (!wait(&bar_full[slot], (item / kRing) & 1)) break;
+          const int item = 2 * gt + 3, slot = item % kRing;
+          if (!wait(&bar_full[item % kBars], (item / kBars) & 1)) break;
           unsigned char* sV = sRing + slot * kSlot;
           const int from = mixed(g, j) ? 0 : valid * (DH / 8), to = (valid + 15) / 16 * 16 * (DH / 8);
           for (int p = from + set_tid; p < to; p += 128) {
@@ -634,84 +726,96 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
           }
           fence_proxy_async();
         }
-        if (!idle) {
-          unsigned v[kAtKeys];
+        // Half h of the scores to probabilities; masked: some rows may not see some of the keys.
+        auto half = [&](int h, auto masked) {
+          const unsigned here = s_tmem + kTtHalf * h;
+          unsigned v[kTtHalf];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + 32 * c, v + 32 * c);
+          for (int c = 0; c < 2; ++c) tmem_ld32(here + 32 * c, v + 32 * c);
           asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-          if (own) {
-            // the bits of the row's visible keys among these 128: of its mask, or up to the token itself
-            const int k0 = (j - g.s.ctx_tiles) * kAtKeys;
-            const int upto = a.mask ? valid : min(valid, my_tok + 1 - k0);
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              const int nb = upto - 32 * h;
-              unsigned w = nb <= 0 ? 0u : nb >= 32 ? ~0u : (1u << nb) - 1u;
-              if (a.mask) {
-                const int at_word = k0 / 64 + (h >> 1);
-                w &= at_word < a.words
-                         ? static_cast<unsigned>(a.mask[static_cast<size_t>(g.s.t0 + my_tok) * a.words + at_word] >> (32 * (h & 1))) : 0u;
-              }
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(w >> i & 1u)) v[32 * h + i] = __float_as_uint(-CUDART_INF_F);
+          if (decltype(masked)::value) {
+            // the bits of the row's visible keys among these 64
+            const int left = valid - kTtHalf * h;
+            unsigned long long w = left >= 64 ? ~0ull : (1ull << left) - 1ull;
+            if (own) {  // of its mask, or up to the token itself
+              const int k0 = (j - g.s.ctx_tiles) * kAtKeys + kTtHalf * h, upto = my_tok + 1 - k0;
+              if (a.mask)
+                w &= k0 / 64 < a.words ? a.mask[static_cast<size_t>(g.s.t0 + my_tok) * a.words + k0 / 64] : 0ull;
+              else
+                w &= upto <= 0 ? 0ull : upto >= 64 ? ~0ull : (1ull << upto) - 1ull;
+            } else {
+              const int skip = my_lo - (base + kTtHalf * h);
+              w &= skip <= 0 ? ~0ull : skip >= 64 ? 0ull : ~0ull << skip;
             }
-          } else if (valid < kAtKeys || base < my_lo) {
 #pragma unroll
-            for (int i = 0; i < kAtKeys; ++i)
-              if (base + i < my_lo || i >= valid) v[i] = __float_as_uint(-CUDART_INF_F);
+            for (int i = 0; i < kTtHalf; ++i)
+              if (!(static_cast<unsigned>(w >> (i & 32)) >> (i & 31) & 1u)) v[i] = __float_as_uint(-CUDART_INF_F);
           }
           float mx[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) mx[u] = fmaxf(__uint_as_float(v[u]), __uint_as_float(v[u + 4]));
 #pragma unroll
-          for (int i = 8; i < kAtKeys; i += 8)
+          for (int i = 8; i < kTtHalf; i += 8)
 #pragma unroll
             for (int u = 0; u < 4; ++u) mx[u] = at_max3(mx[u], __uint_as_float(v[i + u]), __uint_as_float(v[i + u + 4]));
           const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;  // scale > 0
           // raise the maximum in use only when the row's maximum has run ahead of it by more than kAtLazy
           const bool raise = (m > m_run + kAtLazy || m_run == -CUDART_INF_F) && m != -CUDART_INF_F;
-          const float alpha = raise ? at_ex2(m_run - m) : 1.f;
-          m_run = raise ? m : m_run;
-          const float mu = m_run == -CUDART_INF_F ? 0.f : m_run;
-          if (t > first && __any_sync(0xffffffffu, alpha != 1.f)) {
-            // (this set's product before is done: S, which came behind it, is)
+          if (__any_sync(0xffffffffu, raise)) {
+            const float alpha = raise ? at_ex2(m_run - m) : 1.f;
+            m_run = raise ? m : m_run;
+            l_run *= alpha;
+            if (t > first || h == 1) {
+              if (!wait(&bar_o[set], (n_half - 1) & 1)) return;  // this set's product before
+              asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll
-            for (int c = 0; c < DH / 16; ++c) {
-              unsigned o[16];
-              tree_tmem_ld16(o_tmem + 16 * c, o);
-              asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+              for (int c = 0; c < DH / 16; ++c) {
+                unsigned o[16];
+                tree_tmem_ld16(o_tmem + 16 * c, o);
+                asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tree_tmem_st16(o_tmem + 16 * c, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tree_tmem_st16(o_tmem + 16 * c, o);
+              }
             }
           }
-          if (!my_turn()) break;
+          const float mu = m_run == -CUDART_INF_F ? 0.f : m_run;
           // P, two neighbouring keys a word, in the place of S
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < kAtKeys / 2; ++i) {
+          for (int i = 0; i < kTtHalf / 2; ++i) {
             const float p0 = at_ex2(fmaf(__uint_as_float(v[2 * i]), a.scale_log2, -mu));  // masked: ex2(-inf) = 0
             const float p1 = at_ex2(fmaf(__uint_as_float(v[2 * i + 1]), a.scale_log2, -mu));
             sum[2 * (i & 1)] += p0;
             sum[2 * (i & 1) + 1] += p1;
             v[i] = at_pack(p0, p1);
-            if (i % 32 == 31) tmem_st32(s_tmem + i / 32 * 32, v + i / 32 * 32);
           }
-          pass_turn();
-          l_run = l_run * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+          tmem_st32(here, v);
+          l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-        } else {
-          if (!my_turn()) break;
-          pass_turn();
+        };
+        const bool plain = valid == kAtKeys && !mixed(g, j);
+        const int halves = valid > kTtHalf ? 2 : 1;
+#pragma unroll 1
+        for (int h = 0; h < halves && alive; ++h) {
+          if (h == 1) {
+            if (!wait(&bar_s[set][1], n_s >> 1 & 1)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          }
+          n_s ^= 1 << h;
+          if (!idle) {
+            if (plain)
+              half(h, std::false_type{});
+            else
+              half(h, std::true_type{});
+          }
+          ++n_half;
+          asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_p[set][h]);
         }
-        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_p[set]);
+        if (!alive) break;
       }
-      if (WIDE && first > at)                             // (a set without rows passes its turns)
-        for (int t = at; t < g.unit + g.j1 && alive; ++t)
-          if (my_turn()) pass_turn();
       if (!alive) break;
       const TreeSeg now = g;
       const int len = now.j1 - now.j0;                    // tiles of the stretch
@@ -762,7 +866,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
         // whose parts: its own, or both sets' (of a single tile, of the one whose turn it was)
         const bool in0 = WIDE ? set == 0 : len > 1 || (((now.unit + now.j0 - begin) & 1) == 0), in1 = WIDE ? set == 1 : len > 1 || !in0;
         const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (now.j0 > 0 ? 0 : 1);
-        float* part = a.part_o + (slot * kRows + row) * DH + col0;
+        float4* part = a.part_o + (slot * (DH / 4) + col0 / 4) * kRows + row;
         bf16* out = a.out + (static_cast<size_t>(now.s.t0 + tk) * a.Hq + hq) * DH + col0;
 #pragma unroll
         for (int c = 0; c < kCols / 32; ++c) {
@@ -819,7 +923,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
                                                                       at_pack(o[e + 6], o[e + 7]));
           } else if (row_ok) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(part + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < 32; e += 4) part[static_cast<size_t>(8 * c + e / 4) * kRows] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
         if (!whole && row_ok && (WIDE || set == 0)) a.part_ml[slot * kRows + row] = make_float2(m, l);
@@ -838,38 +942,26 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
   }
 }
 
-// Units that the shares cut: block (x, y) takes the unit that holds the first tile of share x + 1, where the share in front of it
-// holds the unit's beginning, and the y-th piece of its rows.
+// Units that the shares cut: block (x, y) takes the unit that block x + 1 of the launch in front has told, and the y-th piece of it.
 //   M = max m_i;  o = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M)
-constexpr int kTmThreads = 128;
+// A warp takes 8 rows of 16 columns: 128 bytes of a part at a time and whole sectors of the result.
+constexpr int kTmThreads = 256, kTmPieces = 16;
 
 template <int DH>
 __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const __grid_constant__ TreeTcArgs a) {
-  extern __shared__ int plan_mem[];
-  __shared__ int s_red[32];
   pdl_launch_dependents();
-  TreePlan plan;
-  plan.pre = plan_mem;
-  plan.cu = plan.pre + a.n_seq + 1;
-  plan.held = plan.cu + a.n_seq + 1;
-  plan.first = plan.held + a.n_seq;
-  tree_plan<kTmThreads>(a, plan, s_red);  // (lengths and tables were there before the launch in front of this one passed its wait)
-  pdl_wait();                                // (every block waits: the next launch takes this one's end for that of both)
-  const int total = plan.total;
-  if (total == 0) return;
-  const int shares = tree_shares(a, total);
+  pdl_wait();  // (every block waits: the next launch takes this one's end for that of both)
   const int share = blockIdx.x + 1;
-  if (share >= shares) return;
-  const int at = tree_begin(share, total, shares);
-  const TreeSeg g = tree_seg(a, plan, at, total);
-  if (g.j0 == 0 || g.unit < tree_begin(share - 1, total, shares)) return;  // not cut here, or an earlier block's
-  const int last = tree_block(g.unit + g.s.nt - 1, total, shares);
-  const int G = a.Hq / a.Hkv, n_rows = min(a.rows, g.s.n_new * G - g.rt * a.rows);
-  constexpr int C4 = DH / 4;
+  const int4 cut = *reinterpret_cast<const int4*>(a.cuts + 8 * share);
+  const int n_rows = cut.x, t0 = cut.y, hk = cut.z, rt = cut.w;
+  if (n_rows == 0) return;
+  const int last = a.cuts[8 * share + 4];
+  const int G = a.Hq / a.Hkv, lane = threadIdx.x & 31;
   constexpr int kBatch = 4;
-  for (int i = blockIdx.y * kTmThreads + threadIdx.x; i < n_rows * C4; i += gridDim.y * kTmThreads) {
-    const int r = i / C4, d = (i % C4) * 4;
-    const int row = g.rt * a.rows + r, tk = row / G, hq = g.hk * G + (row - tk * G);
+  for (int i = blockIdx.y * (kTmThreads / 32) + threadIdx.x / 32; i < (n_rows + 7) / 8 * (DH / 16); i += kTmPieces * (kTmThreads / 32)) {
+    const int r = i / (DH / 16) * 8 + (lane & 7), c4 = i % (DH / 16) * 4 + (lane >> 3);
+    if (r >= n_rows) continue;
+    const int row = rt * a.rows + r, tk = row / G, hq = hk * G + (row - tk * G);
     float mx = -CUDART_INF_F, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (a.sink != nullptr) {
@@ -884,7 +976,7 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const __grid_con
         const int c = min(c0 + u, last);
         const size_t slot = 2 * static_cast<size_t>(c) + (c == share - 1 ? 1 : 0);  // the unit's beginning ends its block's share
         ml[u] = a.part_ml[slot * a.rows + r];
-        x[u] = *reinterpret_cast<const float4*>(a.part_o + (slot * a.rows + r) * DH + d);
+        x[u] = a.part_o[(slot * (DH / 4) + c4) * a.rows + r];
       }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
@@ -900,7 +992,7 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const __grid_con
       }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    stf4(a.out + (static_cast<size_t>(g.s.t0 + tk) * a.Hq + hq) * DH + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    stf4(a.out + (static_cast<size_t>(t0 + tk) * a.Hq + hq) * DH + 4 * c4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   }
 }
 
@@ -913,7 +1005,7 @@ int launch_tree_tc(const TreeMaps& maps, const TreeTcArgs& a, cudaStream_t strea
   launch_pdl(kern, dim3(a.shares), dim3(kTtThreads), smem, stream, maps, a);
   const int st = launch_status();
   if (st != 0 || a.shares == 1) return st;
-  launch_pdl(tree_merge_kernel<DH>, dim3(a.shares - 1, a.rows * DH / 4 / (2 * kTmThreads)), dim3(kTmThreads), tree_plan_bytes(a.n_seq), stream, a);
+  launch_pdl(tree_merge_kernel<DH>, dim3(a.shares - 1, kTmPieces), dim3(kTmThreads), 0, stream, a);
   return launch_status();
 }
 
@@ -926,8 +1018,8 @@ PMM_EXPORT int pmm_tree_attention_tc_supported(int Hq, int Hkv, int Dh, int page
              ? 1 : 0;
 }
 
-// Floats of scratch for `sms` multiprocessors: two parts a block of 256 rows of 128 values, maximum and sum.
-PMM_EXPORT long long pmm_tree_attention_scratch(int sms) { return static_cast<long long>(sms) * 2 * 2 * pmm::kTtRows * (128 + 2); }
+// Floats of scratch for `sms` multiprocessors: two parts a block of 256 rows of 128 values, maximum and sum; eight numbers a block.
+PMM_EXPORT long long pmm_tree_attention_scratch(int sms) { return static_cast<long long>(sms) * (2 * 2 * pmm::kTtRows * (128 + 2) + 8); }
 
 PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* pool,
                                      int pages, const int* block_table, int max_blocks, const int* held, const int* cu, const int* positions,
@@ -977,8 +1069,9 @@ PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k
   a.out = static_cast<pmm::bf16*>(out);
   a.shares = sms;
   a.rows = wide ? 2 * pmm::kTtRows : pmm::kTtRows;
-  a.part_o = scratch;
+  a.part_o = reinterpret_cast<float4*>(scratch);
   a.part_ml = reinterpret_cast<float2*>(scratch + static_cast<size_t>(a.shares) * 2 * a.rows * Dh);
+  a.cuts = reinterpret_cast<int*>(scratch + static_cast<size_t>(a.shares) * 2 * a.rows * (Dh + 2));
   a.scale_log2 = scale * 1.4426950408889634f;
   a.window = window;
   a.page_size = page_size;
