@@ -130,7 +130,7 @@ struct TreeTcArgs {
   float2* part_ml;      // [2 * blocks][rows]
   int* cuts;            // [blocks][8]: a unit that shares cut: its rows (0: none), first token, head, row tile, last block
   float scale_log2;
-  int window, page_size, box, n_seq, T, Hq, Hkv, shares, min_tiles;
+  int window, page_size, box, n_seq, T, Hq, Hkv, shares;
   int rows;             // of a unit: 128 or 256
   int* status;
 };
@@ -228,7 +228,7 @@ __device__ __forceinline__ void tree_plan(const TreeTcArgs& a, TreePlan& p, int*
 }
 
 // How many blocks share `total` tiles, the tile at which block b's share begins, and the block in whose share tile x lies.
-__device__ __forceinline__ int tree_shares(const TreeTcArgs& a, int total) { return max(1, min(a.shares, total / a.min_tiles)); }
+__device__ __forceinline__ int tree_shares(const TreeTcArgs& a, int total) { return max(1, min(a.shares, total)); }
 __device__ __forceinline__ int tree_begin(int b, int total, int shares) { return static_cast<int>(static_cast<long long>(b) * total / shares); }
 __device__ __forceinline__ int tree_block(int x, int total, int shares) {
   return static_cast<int>(((static_cast<long long>(x) + 1) * shares - 1) / total);
@@ -1012,10 +1012,9 @@ int launch_tree_tc(const TreeMaps& maps, const TreeTcArgs& a, cudaStream_t strea
 }  // namespace pmm
 
 // Whether pmm_tree_attention_tc takes this shape.
-PMM_EXPORT int pmm_tree_attention_tc_supported(int Hq, int Hkv, int Dh, int page_size, long long pages, int n_seq) {
-  if (Hkv <= 0 || Hq % Hkv) return 0;
-  return ((Dh == 64 || Dh == 128) && page_size > 0 && page_size % 8 == 0 && pages > 0 && pages * 2 * page_size <= 0x7fffffffll && n_seq <= pmm::kTtSeqs)
-             ? 1 : 0;
+static bool tree_tc_supported(int Hq, int Hkv, int Dh, int page_size, long long pages, int n_seq) {
+  return Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && (Dh == 64 || Dh == 128) && page_size > 0 && page_size % 8 == 0 && pages > 0 &&
+         pages * 2 * page_size <= 0x7fffffffll && n_seq <= pmm::kTtSeqs;
 }
 
 // Floats of scratch for `sms` multiprocessors: two parts a block of 256 rows of 128 values, maximum and sum; eight numbers a block.
@@ -1026,7 +1025,7 @@ PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k
                                      const void* mask, int words, const float* sink, void* out, float scale, int window, int page_size, int n_seq,
                                      int T, int Hq, int Hkv, int Dh, int wide, float* scratch, int sms, int* status, cudaStream_t stream) {
   if (T <= 0 || n_seq <= 0) return 0;
-  if (!pmm_tree_attention_tc_supported(Hq, Hkv, Dh, page_size, pages, n_seq) || max_blocks <= 0 || !(scale > 0.f) || (window != 0 && !positions) ||
+  if (!tree_tc_supported(Hq, Hkv, Dh, page_size, pages, n_seq) || max_blocks <= 0 || !(scale > 0.f) || (window != 0 && !positions) ||
       (mask && words < 1) || !scratch || sms < 1 || !status)
     return PMM_ERR_BAD_ARGUMENT;
   for (const void* p : {q, k, v, pool, static_cast<const void*>(out), static_cast<const void*>(scratch)})
@@ -1080,7 +1079,6 @@ PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k
   a.T = T;
   a.Hq = Hq;
   a.Hkv = Hkv;
-  a.min_tiles = 2;
   a.status = status;
   if (Dh == 64) return wide ? pmm::launch_tree_tc<64, true>(maps, a, stream) : pmm::launch_tree_tc<64, false>(maps, a, stream);
   return wide ? pmm::launch_tree_tc<128, true>(maps, a, stream) : pmm::launch_tree_tc<128, false>(maps, a, stream);

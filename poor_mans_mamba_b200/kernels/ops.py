@@ -187,7 +187,6 @@ _SIGNATURES = {
     "pmm_tree_attention": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p,
                            c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
                            c_int, c_int, c_int, c_void_p],
-    "pmm_tree_attention_tc_supported": [c_int, c_int, c_int, c_int, c_longlong, c_int],
     "pmm_tree_attention_scratch": [c_int],
     "pmm_tree_attention_tc": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p,
                               c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
@@ -288,10 +287,12 @@ _WATCHES: Dict[torch.device, _StatusWatch] = {}
 
 
 def _watch(device: torch.device) -> _StatusWatch:
-    device = torch.device(device)
-    if device.index is None and device.type == "cuda":
-        device = torch.device("cuda", torch.cuda.current_device())
     w = _WATCHES.get(device)
+    if w is None:
+        device = torch.device(device)
+        if device.index is None and device.type == "cuda":
+            device = torch.device("cuda", torch.cuda.current_device())
+        w = _WATCHES.get(device)
     if w is None:
         w = _StatusWatch(device)
         _WATCHES[device] = w
@@ -2321,6 +2322,7 @@ def sample_rows(logits: Tensor, temperature: Optional[Tensor], seeds: Optional[T
 # ----------------------------------------------------------------------------- steps of drafted tokens
 # A request's tokens of such a step are its last token (the root, token 0) and the drafted ones, each behind its parent.
 TREE_MASK_WORDS = 4  # 64-bit words of a token's mask: trees of up to 256 tokens
+TREE_TC_MAX_SEQS = 1024  # requests of a step on the tensor cores (their lengths lie in shared memory)
 
 
 def _ints(what: str, *checks) -> None:
@@ -2396,11 +2398,18 @@ def tree_attention_scratch(device) -> Tensor:
     return torch.empty(_sized("pmm_tree_attention_scratch", _sm_count(device)), dtype=torch.float32, device=device)
 
 
+_SIZES: Dict[tuple, int] = {}
+
+
 def _sized(name: str, *args: int) -> int:
-    """What a function of the library that counts scratch says."""
-    f = _fn(name)
-    f.restype = c_longlong
-    return f(*args)
+    """What a function of the library that counts scratch says (of these numbers always the same)."""
+    key = (name, *args)
+    size = _SIZES.get(key)
+    if size is None:
+        f = _fn(name)
+        f.restype = c_longlong
+        size = _SIZES[key] = f(*args)
+    return size
 
 
 _SMS: Dict[int, int] = {}
@@ -2439,7 +2448,7 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: T
     check_head_dim(head_dim, FLOAT_ATTENTION_MAX_HEAD)
     if n_kv_heads <= 0 or n_q_heads <= 0 or n_q_heads % n_kv_heads:
         raise KernelError(f"{what}: query heads must be a multiple of key/value heads")
-    T, n_seq, dtype = q.shape[0], held.numel(), q.dtype
+    T, n_seq, dtype, pool_shape = q.shape[0], held.numel(), q.dtype, pool.shape
     kv_dim = n_kv_heads * head_dim
     ldq = _aligned_rows(what, "q", q, T, n_q_heads * head_dim)
     ldk = _aligned_rows(what, "k", k, T, kv_dim)
@@ -2448,8 +2457,8 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: T
         raise KernelError(f"{what}: q, k, v, pool and out must be of one type")
     if not out.is_contiguous() or out.shape != q.shape or out.data_ptr() % 16:
         raise KernelError(f"{what}: out must be contiguous [T, Hq*Dh] on a 16-byte boundary")
-    if not (pool.dim() == 4 and pool.shape[1] == 2 and pool.shape[3] == kv_dim and pool.is_contiguous() and pool.data_ptr() % 16 == 0
-            and pool.shape[0] > 0):
+    if not (len(pool_shape) == 4 and pool_shape[1] == 2 and pool_shape[3] == kv_dim and pool.is_contiguous() and pool.data_ptr() % 16 == 0
+            and pool_shape[0] > 0):
         raise KernelError(f"{what}: pool must be contiguous [pages, 2, page_size, Hkv*Dh]")
     _ints(what, ("block_table", block_table, None), ("held", held, None), ("cu_seqlens", cu_seqlens, n_seq + 1))
     if not (block_table.dim() == 2 and block_table.shape[0] == n_seq and n_seq > 0 and block_table.shape[1] > 0):
@@ -2463,17 +2472,21 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: T
         raise KernelError(f"{what}: a window needs the tokens' positions")
     if sink is not None:
         _f32vec(sink, n_q_heads, "tree_attention: sink")
-    sms = _sm_count(q.device)
+    device = q.device
+    sms = _sm_count(device)
     if not (scratch.dtype is torch.float32 and scratch.is_contiguous() and scratch.data_ptr() % 16 == 0
             and scratch.numel() >= _sized("pmm_tree_attention_scratch", sms)):
         raise KernelError(f"{what}: scratch comes from tree_attention_scratch")
-    args = (q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, pool.data_ptr(), pool.shape[0], block_table.data_ptr(), block_table.shape[1],
+    pages, page_size = pool_shape[0], pool_shape[2]
+    args = (q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, pool.data_ptr(), pages, block_table.data_ptr(), block_table.shape[1],
             held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words, _ptr(sink), out.data_ptr(), softmax_scale, window,
-            pool.shape[2], n_seq, T, n_q_heads, n_kv_heads, head_dim)
-    if dtype is torch.bfloat16 and _fn("pmm_tree_attention_tc_supported")(n_q_heads, n_kv_heads, head_dim, pool.shape[2], pool.shape[0], n_seq):
+            page_size, n_seq, T, n_q_heads, n_kv_heads, head_dim)
+    # (the rule of pmm_tree_attention_tc, which refuses what does not keep it)
+    if (dtype is torch.bfloat16 and head_dim in (64, 128) and page_size % 8 == 0 and n_seq <= TREE_TC_MAX_SEQS
+            and 2 * pages * page_size <= 0x7fffffff):
         # units of 256 rows (token, query head of a group) where the requests bring more than 128 on average: K and V once for them
         wide = T * (n_q_heads // n_kv_heads) > 128 * n_seq
-        _call("pmm_tree_attention_tc", *args, wide, scratch.data_ptr(), sms, _tc_status(q.device).data_ptr(), stream)
+        _call("pmm_tree_attention_tc", *args, wide, scratch.data_ptr(), sms, _watch(device).words.data_ptr(), stream)
     else:
         _call("pmm_tree_attention", *args, _dt(q), stream)
 
