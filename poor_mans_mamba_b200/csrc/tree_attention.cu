@@ -4,9 +4,8 @@
 //   sc[j] = (q.K[j]) * scale;  p = exp(sc - max);  o = sum p V / sum p,   0 for a row that sees no key
 // The step's own keys and values lie densely in k and v: the cache takes only those that are kept in the end.
 //
-// This kernel: float arithmetic on the CUDA cores, any storage type and head size.  A block per (token, query head); its eight
-// warps share the keys in pieces of 32 (a key per lane for the scores, a slice of the head per lane for the values) and merge
-// their maxima, sums and results at the end.  The keys of a group's query heads are read once per head, from L2.
+// Float arithmetic on the CUDA cores, any storage type and head size, in two kernels: up to a head size of 256 blocks of rows (a row: a
+// token and a query head of the group) that share what they read of the keys, beyond it a block per token and query head.
 #include "common.cuh"
 #include <math_constants.h>
 
@@ -70,6 +69,8 @@ __device__ __forceinline__ bool ta_sees(const unsigned long long* mask, int word
   return j < 64 * words && (mask[j >> 6] >> (j & 63) & 1ull) != 0ull;
 }
 
+// Head sizes beyond 256.  A block per (token, query head); its eight warps share the keys in pieces of 32 (a key per lane for the scores, a
+// slice of the head per lane for the values) and merge their maxima, sums and results at the end.
 template <typename S, int ACC>
 __global__ void __launch_bounds__(kTaWarps * 32) tree_attention_kernel(const TreeAttnArgs<S> a) {
   extern __shared__ float qs[];  // the query, then every warp's result
@@ -127,9 +128,8 @@ __global__ void __launch_bounds__(kTaWarps * 32) tree_attention_kernel(const Tre
       l = l * corr + warp_sum(p);
 #pragma unroll
       for (int i = 0; i < ACC; ++i) acc[i] *= corr;
-      // values of kKeys keys at a time, so that as many rows travel together (one behind the other a row costs an L2 latency: 32 us
-      // where 4 requests with 12 tokens and 8 heads see 300 keys, together 21); of keys that are not seen they may be anything
-      constexpr int kKeys = ACC <= 4 ? 8 : 32 / ACC;
+      // values of kKeys keys at a time, so that as many rows travel together; of keys that are not seen they may be anything
+      constexpr int kKeys = 32 / ACC;
 #pragma unroll 1
       for (int b = 0; b < 32; b += kKeys) {
         const unsigned some = left >> b & ((1u << kKeys) - 1u);
@@ -190,6 +190,332 @@ __global__ void __launch_bounds__(kTaWarps * 32) tree_attention_kernel(const Tre
   }
 }
 
+// Head sizes up to 256.  A cluster of blocks takes up to 32 rows of one request and key/value head; its blocks take the keys in tiles of 64 in
+// turn.  A tile of K and V lies in shared memory once for all rows (a block per row read the keys anew: 8 requests of 19 tokens with 32 / 8 heads
+// of 128 over 433 keys took 123 us, so 55; 12 requests of a token over 53 keys
+// 10, so 14).  A warp has up to eight rows and 32 of a tile's keys: a lane a key for the scores, a slice of the head a lane for the values, so maxima, sums
+// and results stay in its registers.  In the end every block leaves (maximum, sum, unnormalised result) in its shared memory, and the cluster's
+// blocks join a share of the rows each, in the order of the blocks.  What bounds it: shared memory, 12 reads of 128 bytes for 32 products of a warp's scores,
+// 24 for 128 of its values.
+constexpr int kTfRows = 32, kTfKeys = 64, kTfThreads = 256, kTfPer = 8;
+constexpr int kTfCluster = 8;  // blocks of a cluster at most
+
+// Bytes of shared memory: the queries; a tile of K and V, rows 16 bytes further apart than they are long (in the end two parts of the results).
+__host__ __device__ constexpr int tf_row(int dh, int elem) { return dh * elem + 16; }
+__host__ __device__ constexpr size_t tf_smem(int dh, int elem) {
+  return static_cast<size_t>(kTfRows) * dh * sizeof(float) + static_cast<size_t>(2) * kTfKeys * tf_row(dh, elem);
+}
+static_assert(2 * kTfKeys * 2 >= 2 * kTfRows * 4, "two parts of float results fit where a tile of two-byte elements was");
+__device__ __forceinline__ void tf_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// A float of block `rank`'s shared memory, where this block has it at p.
+__device__ __forceinline__ float tf_remote(const float* p, int rank) {
+  unsigned at;
+  float x;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(static_cast<unsigned>(__cvta_generic_to_shared(p))), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+// s[i] += q_i . k over the head, for the first n of a warp's rows (q: the first, `step` floats to the next).
+__device__ __forceinline__ void tf_scores(float (&s)[kTfPer], const float* q, int step, const float* kr, int Dh, int n) {
+#pragma unroll 2
+  for (int d = 0; d < Dh; d += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(kr + d);
+#pragma unroll
+    for (int i = 0; i < kTfPer; ++i)
+      if (i < n) {
+        const float4 y = *reinterpret_cast<const float4*>(q + i * step + d);
+        s[i] += y.x * x.x;
+        s[i] += y.y * x.y;
+        s[i] += y.z * x.z;
+        s[i] += y.w * x.w;
+      }
+  }
+}
+__device__ __forceinline__ void tf_scores(float (&s)[kTfPer], const float* q, int step, const __nv_bfloat16* kr, int Dh, int n) {
+  for (int d = 0; d < Dh; d += 8) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(kr + d);
+    const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float2 x0 = __bfloat1622float2(h2[2 * c]), x1 = __bfloat1622float2(h2[2 * c + 1]);
+#pragma unroll
+      for (int i = 0; i < kTfPer; ++i)
+        if (i < n) {
+          const float4 y = *reinterpret_cast<const float4*>(q + i * step + d + 4 * c);
+          s[i] += y.x * x0.x;
+          s[i] += y.y * x0.y;
+          s[i] += y.z * x1.x;
+          s[i] += y.w * x1.y;
+        }
+    }
+  }
+}
+
+template <typename S, int ACC>
+__global__ void __launch_bounds__(kTfThreads, ACC <= 4 ? 2 : 1) tree_rows_kernel(const TreeAttnArgs<S> a, int T, int cluster) {
+  extern __shared__ __align__(16) unsigned char tf_mem[];
+  __shared__ float2 s_ml[2][kTfRows];
+  __shared__ __align__(16) float s_p[kTfThreads / 32][kTfPer][32];
+  __shared__ int s_sum[kTfThreads / 32], s_found[2], s_tok[kTfRows], s_lo[kTfRows];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, Dh = a.Dh, G = a.Hq / a.Hkv;
+  const int tile = blockIdx.x / cluster, rank = blockIdx.x % cluster, hk = blockIdx.y;
+  pdl_launch_dependents();
+  pdl_wait();
+  // ---- the request whose row tile this is
+  if (tid == 0) s_found[0] = -1;
+  int before = 0;
+  for (int base = 0; base < a.n_seq; base += kTfThreads) {
+    const int s = base + tid;
+    int n = 0;
+    if (s < a.n_seq) {
+      const int b0 = min(max(a.cu[s], 0), T), b1 = min(max(a.cu[s + 1], b0), T);
+      n = ((b1 - b0) * G + kTfRows - 1) / kTfRows;
+    }
+    int run = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    if (lane == 31) s_sum[warp] = run;
+    __syncthreads();
+    int at = before;
+#pragma unroll
+    for (int w = 0; w < kTfThreads / 32; ++w) {
+      if (w < warp) at += s_sum[w];
+      before += s_sum[w];
+    }
+    at += run - n;
+    if (tile >= at && tile < at + n) {
+      s_found[0] = s;
+      s_found[1] = tile - at;
+    }
+    __syncthreads();
+    if (s_found[0] >= 0) break;
+  }
+  if (s_found[0] < 0) return;  // (the same for the whole cluster)
+  const int seq = s_found[0], row0 = s_found[1] * kTfRows;
+  const int t0 = min(max(a.cu[seq], 0), T), n_new = min(max(a.cu[seq + 1], t0), T) - t0;
+  const int held = max(0, static_cast<int>(min(static_cast<long long>(a.held[seq]), static_cast<long long>(a.max_blocks) * a.page_size)));
+  const int n_rows = min(kTfRows, n_new * G - row0);
+  const int* bt = a.block_table + static_cast<size_t>(seq) * a.max_blocks;
+  const long long kv_dim = static_cast<long long>(a.Hkv) * Dh, v_plane = a.page_size * kv_dim;
+  float* sQ = reinterpret_cast<float*>(tf_mem);
+  unsigned char* sK = tf_mem + static_cast<size_t>(kTfRows) * Dh * sizeof(float);
+  const int row_bytes = tf_row(Dh, sizeof(S));
+  unsigned char* sV = sK + kTfKeys * row_bytes;
+  int first = 0;  // the first cached key that any of the rows may see (or the last one's end)
+  if (a.window != 0) {
+    first = held;
+    for (int tok = row0 / G; tok <= (row0 + n_rows - 1) / G; ++tok) first = min(first, first_visible(a.positions[t0 + tok], a.window));
+  }
+  const int ctx_tiles = (held - first + kTfKeys - 1) / kTfKeys, n_tiles = ctx_tiles + (n_new + kTfKeys - 1) / kTfKeys;
+  auto fetch = [&](int j) {  // four threads a key
+    const bool own = j >= ctx_tiles;
+    const int base = own ? (j - ctx_tiles) * kTfKeys : first + j * kTfKeys, key = tid >> 2;
+    if (key < min(kTfKeys, (own ? n_new : held) - base)) {
+      const S *kr, *vr;
+      if (own) {
+        kr = a.k + (t0 + base + key) * a.ldk + hk * Dh;
+        vr = a.v + (t0 + base + key) * a.ldv + hk * Dh;
+      } else {
+        const int page = min(max(bt[(base + key) / a.page_size], 0), a.pages - 1);  // (no read leaves the pool)
+        kr = a.pool + (static_cast<long long>(page) * 2 * a.page_size + (base + key) % a.page_size) * kv_dim + hk * Dh;
+        vr = kr + v_plane;
+      }
+      const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(sK + key * row_bytes));
+      constexpr int kElems = 16 / static_cast<int>(sizeof(S));
+#pragma unroll 4
+      for (int c = tid & 3; c < Dh / kElems; c += 4) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + 16 * c), "l"(kr + c * kElems) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + kTfKeys * row_bytes + 16 * c), "l"(vr + c * kElems) : "memory");
+      }
+    }
+  };
+  if (rank < n_tiles) {
+    fetch(rank);
+    for (int i = tid; i < n_rows * (Dh / 8); i += kTfThreads) {
+      const int r = i / (Dh / 8), d = 8 * (i - r * (Dh / 8)), tok = (row0 + r) / G, h = (row0 + r) - tok * G;
+      const S* from = a.q + (t0 + tok) * a.ldq + (hk * G + h) * Dh + d;
+      const float4 x = ldf4(from), y = ldf4(from + 4);
+      *reinterpret_cast<float4*>(sQ + r * Dh + d) = x;
+      *reinterpret_cast<float4*>(sQ + r * Dh + d + 4) = y;
+    }
+  }
+  if (tid < kTfRows) {
+    const int tok = min(row0 + tid, n_new * G - 1) / G;
+    s_tok[tid] = tok;
+    s_lo[tid] = a.window != 0 ? first_visible(a.positions[t0 + tok], a.window) : 0;
+  }
+  const int half = warp >> 2, wr = warp & 3;                // of a tile's keys; of the rows: wr, wr + 4, ..
+  const int mine = max(0, (n_rows - wr + 3) / 4);           // rows of this warp
+  float m[kTfPer], l[kTfPer], acc[kTfPer][ACC];
+#pragma unroll
+  for (int i = 0; i < kTfPer; ++i) {
+    m[i] = -CUDART_INF_F;
+    l[i] = 0.f;
+#pragma unroll
+    for (int u = 0; u < ACC; ++u) acc[i][u] = 0.f;
+  }
+  for (int j = rank; j < n_tiles; j += cluster) {
+    const bool own = j >= ctx_tiles;
+    const int base = (own ? (j - ctx_tiles) * kTfKeys : first + j * kTfKeys) + 32 * half;
+    const int n_keys = min(32, (own ? n_new : held) - base);  // of this warp's half
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+    __syncthreads();
+    if (mine > 0 && n_keys > 0) {
+      float s[kTfPer];
+#pragma unroll
+      for (int i = 0; i < kTfPer; ++i) s[i] = 0.f;
+      tf_scores(s, sQ + wr * Dh, 4 * Dh, reinterpret_cast<const S*>(sK + (32 * half + min(lane, n_keys - 1)) * row_bytes), Dh, mine);
+      unsigned sees[kTfPer];
+      bool all = true;
+#pragma unroll
+      for (int i = 0; i < kTfPer; ++i) {
+        sees[i] = 0u;
+        if (i >= mine) continue;
+        const int r = wr + 4 * i, tok = s_tok[r], key = base + lane;
+        const bool see = lane < n_keys && (!own ? key >= s_lo[r] : a.mask ? ta_sees(a.mask + static_cast<size_t>(t0 + tok) * a.words, a.words, key) : key <= tok);
+        sees[i] = __ballot_sync(0xffffffffu, see);
+        all = all && sees[i] == 0xffffffffu;
+        const float sc = see ? s[i] * a.scale : -CUDART_INF_F;
+        const float m_new = fmaxf(m[i], warp_max(sc)), mu = m_new == -CUDART_INF_F ? 0.f : m_new;
+        const float corr = expf(m[i] - mu), p = see ? expf(sc - mu) : 0.f;  // (of a NaN: NaN)
+        s_p[warp][i][lane] = p;
+        m[i] = m_new;
+        l[i] = l[i] * corr + p;  // (a lane's part of the sum)
+#pragma unroll
+        for (int u = 0; u < ACC; ++u) acc[i][u] *= corr;
+      }
+      __syncwarp();
+      const unsigned char* vr = sV + 32 * half * row_bytes;
+      auto value = [&](int k, int u) { return lane + 32 * u < Dh ? ldf(reinterpret_cast<const S*>(vr + k * row_bytes) + lane + 32 * u) : 0.f; };
+      if (all) {
+#pragma unroll 1
+        for (int k = 0; k < 32; k += 4) {
+          float v[4][ACC];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int u = 0; u < ACC; ++u) v[e][u] = value(k + e, u);
+#pragma unroll
+          for (int i = 0; i < kTfPer; ++i)
+            if (i < mine) {
+              const float4 p = *reinterpret_cast<const float4*>(&s_p[warp][i][k]);
+#pragma unroll
+              for (int u = 0; u < ACC; ++u) {
+                acc[i][u] += p.x * v[0][u];
+                acc[i][u] += p.y * v[1][u];
+                acc[i][u] += p.z * v[2][u];
+                acc[i][u] += p.w * v[3][u];
+              }
+            }
+        }
+      } else {
+#pragma unroll 2
+        for (int k = 0; k < n_keys; ++k) {
+          float v[ACC];
+#pragma unroll
+          for (int u = 0; u < ACC; ++u) v[u] = value(k, u);
+#pragma unroll
+          for (int i = 0; i < kTfPer; ++i)
+            if (sees[i] >> k & 1u) {  // (values of keys that are not seen may be anything)
+              const float p = s_p[warp][i][k];
+#pragma unroll
+              for (int u = 0; u < ACC; ++u) acc[i][u] += p * v[u];
+            }
+        }
+      }
+    }
+    __syncthreads();  // (the tile has been used)
+    if (j + cluster < n_tiles) fetch(j + cluster);
+  }
+  // ---- every block's parts, then a share of the rows a block
+  float* part = reinterpret_cast<float*>(sK);  // [half][rows][Dh]
+#pragma unroll
+  for (int i = 0; i < kTfPer; ++i) {
+    if (i >= mine) continue;
+    const int r = wr + 4 * i;
+#pragma unroll
+    for (int u = 0; u < ACC; ++u)
+      if (lane + 32 * u < Dh) part[(half * kTfRows + r) * Dh + lane + 32 * u] = acc[i][u];
+    const float sum = warp_sum(l[i]);
+    if (lane == 0) s_ml[half][r] = make_float2(m[i], sum);
+  }
+  tf_cluster_sync();
+  for (int r = rank + cluster * warp; r < n_rows; r += cluster * (kTfThreads / 32)) {
+    const int tok = s_tok[r], hq = hk * G + (row0 + r) - tok * G;
+    // (lane 2 c + h: half h of block c)
+    const bool there = lane < 2 * cluster;
+    const float part_m = there ? tf_remote(&s_ml[lane & 1][r].x, lane >> 1) : -CUDART_INF_F, part_l = there ? tf_remote(&s_ml[lane & 1][r].y, lane >> 1) : 0.f;
+    float top = warp_max(part_m);
+    if (a.sink) top = fmaxf(top, a.sink[hq]);  // a score without key or value that counts once
+    if (top == -CUDART_INF_F) top = 0.f;
+    const float f = expf(part_m - top);
+    float sum = warp_sum(part_l * f);
+    if (a.sink) sum += expf(a.sink[hq] - top);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (NaN stays NaN)
+    const unsigned some = __ballot_sync(0xffffffffu, part_l != 0.f);  // (parts in which the row sees a key)
+    float o[ACC];
+#pragma unroll
+    for (int u = 0; u < ACC; ++u) o[u] = 0.f;
+#pragma unroll 1
+    for (int p0 = 0; p0 < 2 * cluster; p0 += 4) {
+      float x[4][ACC];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int u = 0; u < ACC; ++u)
+          x[e][u] = (some >> (p0 + e) & 1u) && lane + 32 * u < Dh ? tf_remote(part + (((p0 + e) & 1) * kTfRows + r) * Dh + lane + 32 * u, (p0 + e) >> 1) : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float fp = __shfl_sync(0xffffffffu, f, p0 + e);
+#pragma unroll
+        for (int u = 0; u < ACC; ++u)
+          if (some >> (p0 + e) & 1u) o[u] += fp * x[e][u];
+      }
+    }
+    S* out = a.out + (static_cast<long long>(t0 + tok) * a.Hq + hq) * Dh;
+#pragma unroll
+    for (int u = 0; u < ACC; ++u)
+      if (lane + 32 * u < Dh) stf(out + lane + 32 * u, o[u] * inv);
+  }
+  tf_cluster_sync();  // (no block leaves while another reads its parts)
+}
+
+template <typename S, int ACC>
+int launch_tree_rows(const TreeAttnArgs<S>& a, int T, int sms, cudaStream_t stream) {
+  const int G = a.Hq / a.Hkv;
+  const long long tiles = (static_cast<long long>(T) * G + kTfRows - 1) / kTfRows + min(T, a.n_seq);  // (at most)
+  const long long keys = static_cast<long long>(a.max_blocks) * a.page_size / kTfKeys + 1;                                // tiles of them, about
+  int cluster = kTfCluster;
+  while (cluster > 1 && (tiles * a.Hkv * cluster > 2ll * sms || cluster > keys)) cluster /= 2;
+  if (tiles * cluster > 0x7fffffffll) return PMM_ERR_BAD_ARGUMENT;
+  const size_t smem = tf_smem(a.Dh, sizeof(S));
+  auto kern = tree_rows_kernel<S, ACC>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));  // (of the current device: at every call)
+  if (e != cudaSuccess) return static_cast<int>(e);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * cluster), a.Hkv);
+  cfg.blockDim = dim3(kTfThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2]{};
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kern, a, T, cluster);
+  return launch_status();
+}
+
 }  // namespace pmm
 
 // q [T, Hq*Dh], k, v [T, Hkv*Dh] with row strides in elements, rows on 16-byte boundaries; pool [pages, 2, page_size, Hkv*Dh]; out [T,
@@ -197,18 +523,19 @@ __global__ void __launch_bounds__(kTaWarps * 32) tree_attention_kernel(const Tre
 PMM_EXPORT int pmm_tree_attention(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* pool, int pages,
                                   const int* block_table, int max_blocks, const int* held, const int* cu, const int* positions, const void* mask,
                                   int words, const float* sink, void* out, float scale, int window, int page_size, int n_seq, int T, int Hq,
-                                  int Hkv, int Dh, int dtype, cudaStream_t stream) {
+                                  int Hkv, int Dh, int dtype, int sms, cudaStream_t stream) {
   if (T <= 0 || n_seq <= 0) return 0;
-  if (Dh <= 0 || Dh % 16 || Dh > 512 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq > 65535 || page_size <= 0 || max_blocks <= 0 || pages <= 0 || !(scale > 0.f) ||
+  if (Dh <= 0 || Dh % 16 || Dh > 512 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq > 65535 || page_size <= 0 || sms < 1 || max_blocks <= 0 || pages <= 0 || !(scale > 0.f) ||
       (window != 0 && !positions) || (mask && words < 1))
     return PMM_ERR_BAD_ARGUMENT;
   PMM_DISPATCH_DTYPE(dtype, S, {
     pmm::TreeAttnArgs<S> a{static_cast<const S*>(q), ldq, static_cast<const S*>(k), ldk, static_cast<const S*>(v), ldv, static_cast<const S*>(pool),
                            block_table, max_blocks, pages, held, cu, positions, static_cast<const unsigned long long*>(mask), words, sink,
                            static_cast<S*>(out), scale, window, page_size, n_seq, Hq, Hkv, Dh};
-    auto kern = Dh <= 64 ? pmm::tree_attention_kernel<S, 2> : Dh <= 128 ? pmm::tree_attention_kernel<S, 4>
-              : Dh <= 256 ? pmm::tree_attention_kernel<S, 8> : pmm::tree_attention_kernel<S, 16>;
-    pmm::launch_pdl(kern, dim3(T, Hq), dim3(pmm::kTaWarps * 32), static_cast<size_t>(pmm::kTaWarps) * Dh * sizeof(float), stream, a);
+    if (Dh <= 64) return pmm::launch_tree_rows<S, 2>(a, T, sms, stream);
+    if (Dh <= 128) return pmm::launch_tree_rows<S, 4>(a, T, sms, stream);
+    if (Dh <= 256) return pmm::launch_tree_rows<S, 8>(a, T, sms, stream);
+    pmm::launch_pdl(pmm::tree_attention_kernel<S, 16>, dim3(T, Hq), dim3(pmm::kTaWarps * 32), static_cast<size_t>(pmm::kTaWarps) * Dh * sizeof(float), stream, a);
   });
   return pmm::launch_status();
 }

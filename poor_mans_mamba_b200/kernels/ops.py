@@ -186,7 +186,7 @@ _SIGNATURES = {
                           c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p],
     "pmm_tree_attention": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p,
                            c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
-                           c_int, c_int, c_int, c_void_p],
+                           c_int, c_int, c_int, c_int, c_void_p],
     "pmm_tree_attention_scratch": [c_int],
     "pmm_tree_attention_tc": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p,
                               c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
@@ -2488,7 +2488,7 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: T
         wide = T * (n_q_heads // n_kv_heads) > 128 * n_seq
         _call("pmm_tree_attention_tc", *args, wide, scratch.data_ptr(), sms, _watch(device).words.data_ptr(), stream)
     else:
-        _call("pmm_tree_attention", *args, _dt(q), stream)
+        _call("pmm_tree_attention", *args, _dt(q), sms, stream)
 
 
 def verify_drafts_scratch(n_rows: int, vocab: int, device) -> Tensor:
