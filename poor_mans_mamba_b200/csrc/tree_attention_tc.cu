@@ -8,16 +8,18 @@
 // share is finished by its block; of a unit that shares cut, every block leaves (maximum, sum, unnormalised result) in scratch
 // and a second launch merges them in the order of the keys, so results do not depend on which block came first.
 // Within a block warp 0 brings K and V tiles by TMA (cached keys in boxes that lie inside a page, the step's own from k and
-// v) into a ring; two sets of four warps turn S = Q K^T into P, a thread a row, all 128 of its scores in registers, so that
+// v) into a ring; two sets of four warps turn S = Q K^T into P, a thread a row, 64 of its scores at a time in registers, so that
 // maximum and sum need no other thread; and for each set a warp issues S and O += P V.  Units of 128 rows: the sets take the
 // tiles in turn, and their results are joined when the unit ends.  Units of 256: every set has 128 rows, and K and V are brought
-// once for both.  Each set has its S, running maximum and sum, and its O in tensor memory (4 x 128 columns); P takes the place
-// of the S that it is made from.  A set's products are executed in order: its S is complete only when its P V before is.
+// once for both (16 requests of 8,192 with trees of 64, 64 / 8 heads of 128: 308 us, in units of 128 331; 144 rows a unit: 32 and 33).
+// Each set has its S, running maximum and sum, and its O in tensor memory (4 x 128 columns); P takes the place of the S that it is
+// made from.  S and P go in halves of 64 keys, each with barriers of its own: while one half's exponentials are made, the other
+// half's P V and the S behind it run, so neither side waits for the other's answer (whole tiles: 385 us where halves take 305).
 // The ring and the products run on across units.
-// What bounds a tile of 128 rows and 128 keys, clocks: products 1,026 (16 of 128 x 128 x 16, 64 each; half as many rows take as
-// long), exponentials 1,024 (16 a clock), shared memory 1,250 (64 KB in, 96 KB read by the products, 128 bytes a clock), 64 KB from
-// memory 2,800 where it comes from there.  A warp that issues spends 1,400 clocks a tile on barriers, and the products behind
-// one another in its queue do not cover that: hence a warp a set.
+// What bounds half a tile of two sets, 256 rows and 64 keys, clocks: products 1,259 (the S of 64 columns read Q at 128 bytes a clock:
+// 48 each instead of 32), exponentials 1,024 (16 a clock), 32 KB from L2 at 5.4 TB/s of all blocks 1,450; it takes 2,250, of them 2,000 a
+// warp's own way through load, maximum, exponentials and store: two warps a scheduler do not cover each other's latencies.  With
+// units of 128 rows memory bounds it: 32 x 16,384 takes 245 us, the copies alone 237.
 // Of a tile's values only the 16 keys at a time that hold a valid one are multiplied; rows behind the last valid one (stale
 // places of a page, other requests' tokens) are set to zero first, for 0 * NaN is NaN.  Where a tile's keys are not seen by
 // all rows alike (the step's own tokens, a window's edge) values that are not finite are taken out of the product and added
@@ -36,9 +38,10 @@ constexpr int kTtThreads = 12 * 32;  // copies, two warps that issue, one withou
 // tensor memory: S (and P) of the two sets of warps, O of the two
 constexpr unsigned kTtO = 256, kTtCols = 512;
 __host__ __device__ constexpr int tree_q_sub() { return kTtRows * kAtDhBlock * 2; }        // a sub-tile of Q: 64 head-size columns
-// Tiles in flight (16 or 32 KB each): what queries and lengths leave of shared memory.  K_j is copy 2 j, V_j copy 2 j + 3 of the block (the order in which they
-// are asked for; there is no copy 1), in slot (copy % ring).  A copy's barrier tells it only from the one before on that barrier, and a wait that skips one may take the last but one for
-// its own; so there are as many barriers as make all copies of one to be of one kind and, where the sets take the tiles in turn, of one set.
+// Tiles in flight (16 or 32 KB each): what queries and lengths leave of shared memory (32 x 16,384: 245 us with 5, 260 with 4).  K_j is copy
+// 2 j, V_j copy 2 j + 3 of the block (the order in which they are asked for; there is no copy 1), in slot (copy % ring).  A copy's barrier
+// tells it only from the one before on that barrier, and a wait that skips one may take the last but one for its own; so there are
+// as many barriers as make all copies of one to be of one kind and, where the sets take the tiles in turn, of one set.
 __host__ __device__ constexpr int tree_ring(int dh, bool wide) { return dh == 64 ? 11 : wide ? 4 : 5; }
 __host__ __device__ constexpr int tree_bars(int ring) { return ring % 4 == 0 ? ring : 4 * ring; }
 __host__ __device__ constexpr size_t tree_smem(int dh, bool wide) {
@@ -51,8 +54,9 @@ constexpr unsigned kTtIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast
 __host__ __device__ constexpr unsigned tree_idesc_o(int dh) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (static_cast<unsigned>(dh >> 3) << 17) | (static_cast<unsigned>(kTtRows >> 4) << 24);
 }
-// Products and commits by one elected thread of a warp that is here as a whole, the same one every time.  elect.sync is how the compiler learns that a
-// single thread issues: a commit takes 8 clocks, with a predicate (lane == 0) 55, and eight products 312 or fewer, not 401.
+// Products and commits by one elected thread of a warp that is here as a whole, the same one every time.  elect.sync is how the
+// compiler learns that a single thread issues: a commit takes 8 clocks, with a predicate (lane == 0) 55, and eight products 312 or
+// fewer, not 401.
 __device__ __forceinline__ void tree_mma_ss(unsigned tmem_d, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
   asm volatile(
       "{\n\t.reg .pred p, l;\n\t"
@@ -324,7 +328,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<unsigned long long>(&maps.pool)) : "memory");
   }
   pdl_wait();
-  pdl_launch_dependents();  // (behind the wait: the merge reads the lengths ahead of its own)
+  pdl_launch_dependents();  // (behind the wait: the merge's blocks would hold places that the launch in front needs)
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem_base)), "r"(kTtCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
@@ -557,8 +561,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
         if (wp.live && !wait(&bar_read, left & 1)) code = 44;  // (its O has been read)
         continue;
       }
-      // Whole tiles with another of the stretch behind them, both halves of their S made: the same without questions (2,390 clocks for half a
-      // tile of both sets with them; a warp's way through branches costs more than the products that it issues).
+      // Whole tiles with another of the stretch behind them, both halves of their S made: the same without questions (a warp's way
+      // through branches costs more than the products that it issues: 338 us with them where 305 without).
       if (ws.rows && taken == 3 && ws.in && ws.seg == wp.seg && ws.t == wp.t + kStep) {
         int until = wp.end;  // the first tile that is not whole, or the end
         if (wp.ctx_steps < 8 && wp.t < wp.own) until = min(until, wp.own - 1);
