@@ -275,6 +275,74 @@ def test_tree_attention_values_that_are_not_numbers(dtype, d, held):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (12, 2, 128), (64, 8, 128), (16, 1, 64), (4, 1, 256)])
+@pytest.mark.parametrize("held,new", [([3000, 10, 0, 1500, 700, 129], [17, 1, 4, 0, 33, 2]), ([1, 2049, 64, 4000], [40, 9, 64, 1]),
+                                      ([1285, 1286, 1287, 1340, 1344], [20, 20, 20, 20, 20])])
+def test_tree_attention_ragged_and_long(dtype, heads, held, new):
+    """Units of a few rows beside units of hundreds, contexts of many tiles beside none, last tiles of every size."""
+    c = Case(held, new, heads, dtype, 64, seed=new[0], extra_rows=3)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("page", [1, 8, 10, 24, 40, 48, 128, 200, 256])
+@pytest.mark.parametrize("window", [0, 70])
+def test_tree_attention_page_sizes(dtype, page, window):
+    for heads in ((8, 2, 64), (6, 2, 128)):
+        c = Case([333, 40, 0, 801], [6, 9, 4, 30], heads, dtype, page, seed=page, extra_pages=2)
+        c.run(window)
+        c.check(window)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [33, 257, 600, 1024, 1025])
+def test_tree_attention_of_many_requests(dtype, n):
+    """(More than 1,024 take the float kernel.)"""
+    held = [(7 * s * s + 3 * s) % 41 for s in range(n)]
+    new = [(5, 0, 1, 2, 0, 3, 1)[s % 7] for s in range(n)]
+    c = Case(held, new, (4, 2, 64), dtype, 16, seed=n)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_tree_attention_queries_and_cached_rows_that_are_not_numbers(dtype, d):
+    """A query that is not a number spoils its own row, a cached row the rows of its request that see it."""
+    c = Case([300, 70, 500], [12, 40, 5], (8, 2, d), dtype, 64, seed=13)
+    c.q[2, :d] = math.nan
+    c.q[c.cu[1] + 7, 5 * d + 3] = math.nan
+    c.run()
+    c.check()
+    page = int(c.table[2, 1])
+    c.pool[page, 0, 5, :d] = math.nan         # a key: its rows are no numbers
+    c.ctx[2][0, 64 + 5, :d] = math.nan
+    page = int(c.table[0, 3])
+    c.pool[page, 1, 50, d + 1] = math.inf     # a value: one column of its rows
+    c.ctx[0][1, 3 * 64 + 50, d + 1] = math.inf
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tree_attention_side_by_side(dtype):
+    """Calls on two streams at once, a scratch each."""
+    cases = [Case([4000, 900], [20, 8], (8, 2, 128), dtype, 64, seed=1), Case([100, 2500, 640], [5, 33, 1], (8, 2, 128), dtype, 64, seed=2)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    scratch = [K().tree_attention_scratch(DEV) for _ in cases]
+    lengths = [(i32(c.held), i32(c.cu)) for c in cases]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for c, s, x, (held, cu) in zip(cases, streams, scratch, lengths):
+            with torch.cuda.stream(s):
+                K().tree_attention(c.q, c.k, c.v, c.pool, c.table, held, cu, c.out, c.hq, c.hkv, c.d, c.scale, x, mask=c.mask)
+    torch.cuda.synchronize()
+    for c in cases:
+        c.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_tree_attention_large_scores(dtype):
     """Scores far apart: single keys take the whole weight, maxima rise late."""
     c = Case([700, 64], [20, 3], (8, 2, 64), dtype, 64, seed=11)
