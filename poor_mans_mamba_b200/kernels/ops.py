@@ -2539,6 +2539,8 @@ def verify_drafts(logits: Tensor, tokens: Tensor, cu_seqlens: Tensor, uniforms: 
         raise KernelError(f"{what}: temperature must be contiguous float32 [{n}]")
     if not (path.dim() == 2 and path.shape[0] == n and path.shape[1] > 0 and tokens_out.shape == path.shape):
         raise KernelError(f"{what}: tokens_out and path must be int32 [requests, width]")
+    if tokens_out.data_ptr() in (tokens.data_ptr(), path.data_ptr()) or path.data_ptr() == tokens.data_ptr():
+        raise KernelError(f"{what}: tokens, tokens_out and path must be three (requests read and write side by side)")
     if not (scratch.is_contiguous() and scratch.data_ptr() % 16 == 0
             and scratch.numel() * scratch.element_size() >= _sized("pmm_verify_scratch", T, V)):
         raise KernelError(f"{what}: scratch comes from verify_drafts_scratch for as many rows")
@@ -2568,6 +2570,8 @@ def keep_accepted(rows: Tensor, pool: Tensor, slots: Tensor, cu_seqlens: Tensor,
         raise KernelError(f"{what}: a place per token and a path per request")
     if pool.shape[1] * pool.shape[3] > 0x7fffffff:
         raise KernelError(f"{what}: places in the pool do not fit 32 bits")
+    if 0 <= rows.data_ptr() - pool.data_ptr() < pool.numel() * pool.element_size():
+        raise KernelError(f"{what}: rows must not lie in the pool (they are read and written side by side)")
     if T == 0:
         return
     sl, sp, sr, _ = rows.stride()

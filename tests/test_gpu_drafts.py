@@ -617,7 +617,7 @@ def test_verify_drafts_refusals():
     call()
     for kw in (dict(logits=logits.half()), dict(logits=logits.t()), dict(tokens=i[:3]), dict(cu_seqlens=i), dict(uniforms=logits[:, 0]),
                dict(tokens_out=w[0]), dict(path=w[:, :3]), dict(count=i), dict(scratch=scratch[:8]), dict(temperature=logits[:2, 0].contiguous()),
-               dict(parents=i[:2]), dict(parents=i, draft_logits=logits), dict(draft_logits=logits[:3])):
+               dict(parents=i[:2]), dict(parents=i, draft_logits=logits), dict(draft_logits=logits[:3]), dict(path=w), dict(tokens=w.view(4))):
         with pytest.raises(K().KernelError):
             call(**kw)
 
@@ -656,6 +656,8 @@ def test_keep_accepted_refusals():
                     (3, i32([0])), (4, i32([0] * 4)), (5, i32([1, 1])), (0, rows.half()), (2, torch.zeros(4, device=DEV))]:
         with pytest.raises(K().KernelError):
             K().keep_accepted(*good[:at], bad, *good[at + 1:])
+    with pytest.raises(K().KernelError):
+        K().keep_accepted(pool[:, 1, :, :4], *good[1:])  # rows in the pool itself
 
 
 # ----------------------------------------------------------------------------- the operators together
