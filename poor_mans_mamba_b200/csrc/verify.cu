@@ -112,11 +112,15 @@ __device__ __forceinline__ double vf_weight(float l, float top, double c, const 
 // The request that row r belongs to: how many end at or before it.  Called by a whole warp.
 __device__ __forceinline__ int vf_request(const int* cu, int n, int r) {
   int s = 0;
-  for (int b = 0; b < n; b += 32) {
-    const int i = b + (threadIdx.x & 31);
-    const int c = __popc(__ballot_sync(0xffffffffu, i < n && cu[i + 1] <= r));
+  for (int b = 0; b < n; b += 128) {  // four loads in flight
+    int ends[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) ends[u] = cu[min(b + 32 * u + static_cast<int>(threadIdx.x & 31), n - 1) + 1];
+    int c = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) c += __popc(__ballot_sync(0xffffffffu, b + 32 * u + static_cast<int>(threadIdx.x & 31) < n && ends[u] <= r));
     s += c;
-    if (c < 32) break;
+    if (c < 128) break;
   }
   return s;
 }
@@ -165,20 +169,27 @@ __global__ void __launch_bounds__(kVfThreads, 4) verify_stats_kernel(const Verif
   const unsigned w = blockIdx.x * kVfWarps + (threadIdx.x >> 5);
   const int r = static_cast<int>(w / a.chunks), c = static_cast<int>(w % a.chunks);
   const bool of_draft = blockIdx.y == 1;
-  if (r >= min(a.cu[a.n], a.n_rows)) return;
-  const int s = vf_request(a.cu, a.n, r);
-  const float temp = a.temperature ? a.temperature[s] : 0.f;
-  const bool greedy = !(temp > 0.f);
-  if (of_draft && (greedy || r == a.cu[s + 1] - 1)) return;  // (nothing was drafted behind a chain's last token)
+  if (r >= a.n_rows) return;
   const int base = c * kVfChunk + lane;
   const float* row = (of_draft ? a.draft + r * a.ld_draft : a.logits + r * a.ld) + base;
   float v[kVfEach];
-  if (c * kVfChunk + kVfChunk <= a.V) {
+  auto load = [&]() {
+    if (c * kVfChunk + kVfChunk <= a.V) {
 #pragma unroll
-    for (int k = 0; k < kVfEach; ++k) v[k] = row[k * 32];
-  } else {
+      for (int k = 0; k < kVfEach; ++k) v[k] = row[k * 32];
+    } else {
 #pragma unroll
-    for (int k = 0; k < kVfEach; ++k) v[k] = base + k * 32 < a.V ? row[k * 32] : -CUDART_INF_F;
+      for (int k = 0; k < kVfEach; ++k) v[k] = base + k * 32 < a.V ? row[k * 32] : -CUDART_INF_F;
+    }
+  };
+  if (!of_draft) load();  // (beside the request's search; not every row of the draft is wanted)
+  const int s = vf_request(a.cu, a.n, r);
+  if (s >= a.n) return;   // (behind the last request)
+  const float temp = a.temperature ? a.temperature[s] : 0.f;
+  const bool greedy = !(temp > 0.f);
+  if (of_draft) {
+    if (greedy || r == a.cu[s + 1] - 1) return;  // (nothing was drafted behind a chain's last token)
+    load();
   }
   float top = -CUDART_INF_F;
   int at = base;
