@@ -109,6 +109,13 @@ __device__ __forceinline__ double vf_weight(float l, float top, double c, const 
   return live ? w : top == CUDART_INF_F && l == top ? 1.0 : 0.0;
 }
 
+// 2^x to 2^-22 of itself, 0 below 2^-126 (what is smaller than that beside the largest weight, 1, counts for nothing).
+__device__ __forceinline__ float vf_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // The request that row r belongs to: how many end at or before it.  Called by a whole warp.
 __device__ __forceinline__ int vf_request(const int* cu, int n, int r) {
   int s = 0;
@@ -225,7 +232,7 @@ __global__ void __launch_bounds__(kVfThreads, 4) verify_stats_kernel(const Verif
 #pragma unroll
         for (int k = 0; k < kVfEach; ++k) {
           const float x = (v[k] - top) * c2;
-          part[k & 3] += x == x ? exp2f(x) : 0.f;
+          part[k & 3] += fmaxf(vf_ex2(x), 0.f);  // (NaN gives way)
         }
         sum = (static_cast<double>(part[0]) + part[1]) + (static_cast<double>(part[2]) + part[3]);
       }
