@@ -18,9 +18,9 @@
 // First launch: a warp per (row, 1,024 entries) reads its entries once and leaves their maximum and the sum of
 // exp((l - maximum) / T); for drafts with a distribution in 32 bits (the sums are off by less than 2^-17 of themselves), for
 // fixed proposals, each node of which draws, in 64.
-// Second launch: a cluster of up to eight blocks per request.  With a draft's distribution, u q(x) < p(x) is decided from the first
+// Second launch: a cluster of up to 16 blocks per request.  With a draft's distribution, u q(x) < p(x) is decided from the first
 // launch's sums where the sides are 2^-14 apart or more, else (hardly ever) from exact sums of the two rows; then the row
-// that the next token is drawn from, and the draft's behind it, go once through the cluster's 64 warps.  A draw is one block's work:
+// that the next token is drawn from, and the draft's behind it, go once through the cluster's warps.  A draw is one block's work:
 // it finds the piece of 1,024 by the pieces' sums and the entry in it, four entries a thread; a tree's nodes draw side by side.
 #include "common.cuh"
 #include <math_constants.h>
@@ -31,7 +31,7 @@ constexpr int kVfThreads = 256;
 constexpr int kVfWarps = kVfThreads / 32;
 constexpr int kVfEach = 32;
 constexpr int kVfChunk = 32 * kVfEach;
-constexpr int kVfCluster = 8;       // blocks of a cluster at most
+constexpr int kVfCluster = 16;      // blocks of a cluster at most
 constexpr int kVfChunksMax = 2048;  // sums of a row's pieces in shared memory
 constexpr int kVfStep = 4;          // entries of a row that a lane takes at a time in the second launch
 constexpr int kVfNear = 4;          // places that a lane remembers
@@ -764,10 +764,14 @@ PMM_EXPORT int pmm_verify_drafts(const float* logits, long long ld, const float*
     const cudaError_t e = cudaFuncSetAttribute(pmm::verify_walk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  // as many blocks a request as are on the device at once (two a multiprocessor), up to eight: 64 chains at 130,049 take 106 us with
-  // four, 113 with eight
+  // as many blocks a request as are on the device at once (two a multiprocessor), up to 16: 64 chains at 130,049 take 97 us with four, 105
+  // with eight, 118 with two; 16 trees of 16 nodes at 65,537 22 with 16, 25 with eight, 31 with four
   a.cluster = pmm::kVfCluster;
   while (a.cluster > 1 && static_cast<long long>(n) * a.cluster > 2ll * sms) a.cluster /= 2;
+  if (a.cluster > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(pmm::verify_walk_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(n) * a.cluster);
   cfg.blockDim = dim3(pmm::kVfThreads);
