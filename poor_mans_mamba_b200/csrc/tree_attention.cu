@@ -9,6 +9,8 @@
 #include "common.cuh"
 #include <math_constants.h>
 
+#include <type_traits>
+
 namespace pmm {
 
 constexpr int kTaWarps = 8;
@@ -218,23 +220,24 @@ __device__ __forceinline__ float tf_remote(const float* p, int rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(x) : "r"(at) : "memory");
   return x;
 }
-// s[i] += q_i . k over the head, for the first n of a warp's rows (q: the first, `step` floats to the next).
-__device__ __forceinline__ void tf_scores(float (&s)[kTfPer], const float* q, int step, const float* kr, int Dh, int n) {
+// s[i] += q[i] . k over the head, for N rows.
+template <int N>
+__device__ __forceinline__ void tf_scores(float (&s)[N], const float* const (&q)[N], const float* kr, int Dh) {
 #pragma unroll 2
   for (int d = 0; d < Dh; d += 4) {
     const float4 x = *reinterpret_cast<const float4*>(kr + d);
 #pragma unroll
-    for (int i = 0; i < kTfPer; ++i)
-      if (i < n) {
-        const float4 y = *reinterpret_cast<const float4*>(q + i * step + d);
-        s[i] += y.x * x.x;
-        s[i] += y.y * x.y;
-        s[i] += y.z * x.z;
-        s[i] += y.w * x.w;
-      }
+    for (int i = 0; i < N; ++i) {
+      const float4 y = *reinterpret_cast<const float4*>(q[i] + d);
+      s[i] += y.x * x.x;
+      s[i] += y.y * x.y;
+      s[i] += y.z * x.z;
+      s[i] += y.w * x.w;
+    }
   }
 }
-__device__ __forceinline__ void tf_scores(float (&s)[kTfPer], const float* q, int step, const __nv_bfloat16* kr, int Dh, int n) {
+template <int N>
+__device__ __forceinline__ void tf_scores(float (&s)[N], const float* const (&q)[N], const __nv_bfloat16* kr, int Dh) {
   for (int d = 0; d < Dh; d += 8) {
     const uint4 raw = *reinterpret_cast<const uint4*>(kr + d);
     const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
@@ -242,14 +245,13 @@ __device__ __forceinline__ void tf_scores(float (&s)[kTfPer], const float* q, in
     for (int c = 0; c < 2; ++c) {
       const float2 x0 = __bfloat1622float2(h2[2 * c]), x1 = __bfloat1622float2(h2[2 * c + 1]);
 #pragma unroll
-      for (int i = 0; i < kTfPer; ++i)
-        if (i < n) {
-          const float4 y = *reinterpret_cast<const float4*>(q + i * step + d + 4 * c);
-          s[i] += y.x * x0.x;
-          s[i] += y.y * x0.y;
-          s[i] += y.z * x1.x;
-          s[i] += y.w * x1.y;
-        }
+      for (int i = 0; i < N; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(q[i] + d + 4 * c);
+        s[i] += y.x * x0.x;
+        s[i] += y.y * x0.y;
+        s[i] += y.z * x1.x;
+        s[i] += y.w * x1.y;
+      }
     }
   }
 }
@@ -366,18 +368,23 @@ __global__ void __launch_bounds__(kTfThreads, ACC <= 4 ? 2 : 1) tree_rows_kernel
     const int n_keys = min(32, (own ? n_new : held) - base);  // of this warp's half
     asm volatile("cp.async.wait_all;\n" ::: "memory");
     __syncthreads();
-    if (mine > 0 && n_keys > 0) {
-      float s[kTfPer];
+    // N of the warp's rows, or more than it has: the last one again, whose results nobody reads (a question per row and step costs
+    // more than its products)
+    auto work = [&](auto rows) {
+      constexpr int N = decltype(rows)::value;
+      float s[N];
+      const float* q[N];
 #pragma unroll
-      for (int i = 0; i < kTfPer; ++i) s[i] = 0.f;
-      tf_scores(s, sQ + wr * Dh, 4 * Dh, reinterpret_cast<const S*>(sK + (32 * half + min(lane, n_keys - 1)) * row_bytes), Dh, mine);
-      unsigned sees[kTfPer];
+      for (int i = 0; i < N; ++i) {
+        s[i] = 0.f;
+        q[i] = sQ + (wr + 4 * min(i, mine - 1)) * Dh;
+      }
+      tf_scores<N>(s, q, reinterpret_cast<const S*>(sK + (32 * half + min(lane, n_keys - 1)) * row_bytes), Dh);
+      unsigned sees[N];
       bool all = true;
 #pragma unroll
-      for (int i = 0; i < kTfPer; ++i) {
-        sees[i] = 0u;
-        if (i >= mine) continue;
-        const int r = wr + 4 * i, tok = s_tok[r], key = base + lane;
+      for (int i = 0; i < N; ++i) {
+        const int r = wr + 4 * min(i, mine - 1), tok = s_tok[r], key = base + lane;
         const bool see = lane < n_keys && (!own ? key >= s_lo[r] : a.mask ? ta_sees(a.mask + static_cast<size_t>(t0 + tok) * a.words, a.words, key) : key <= tok);
         sees[i] = __ballot_sync(0xffffffffu, see);
         all = all && sees[i] == 0xffffffffu;
@@ -402,17 +409,16 @@ __global__ void __launch_bounds__(kTfThreads, ACC <= 4 ? 2 : 1) tree_rows_kernel
 #pragma unroll
             for (int u = 0; u < ACC; ++u) v[e][u] = value(k + e, u);
 #pragma unroll
-          for (int i = 0; i < kTfPer; ++i)
-            if (i < mine) {
-              const float4 p = *reinterpret_cast<const float4*>(&s_p[warp][i][k]);
+          for (int i = 0; i < N; ++i) {
+            const float4 p = *reinterpret_cast<const float4*>(&s_p[warp][i][k]);
 #pragma unroll
-              for (int u = 0; u < ACC; ++u) {
-                acc[i][u] += p.x * v[0][u];
-                acc[i][u] += p.y * v[1][u];
-                acc[i][u] += p.z * v[2][u];
-                acc[i][u] += p.w * v[3][u];
-              }
+            for (int u = 0; u < ACC; ++u) {
+              acc[i][u] += p.x * v[0][u];
+              acc[i][u] += p.y * v[1][u];
+              acc[i][u] += p.z * v[2][u];
+              acc[i][u] += p.w * v[3][u];
             }
+          }
         }
       } else {
 #pragma unroll 2
@@ -421,7 +427,7 @@ __global__ void __launch_bounds__(kTfThreads, ACC <= 4 ? 2 : 1) tree_rows_kernel
 #pragma unroll
           for (int u = 0; u < ACC; ++u) v[u] = value(k, u);
 #pragma unroll
-          for (int i = 0; i < kTfPer; ++i)
+          for (int i = 0; i < N; ++i)
             if (sees[i] >> k & 1u) {  // (values of keys that are not seen may be anything)
               const float p = s_p[warp][i][k];
 #pragma unroll
@@ -429,6 +435,16 @@ __global__ void __launch_bounds__(kTfThreads, ACC <= 4 ? 2 : 1) tree_rows_kernel
             }
         }
       }
+    };
+    if (n_keys > 0) {
+      if (mine > 4)
+        work(std::integral_constant<int, 8>{});
+      else if (mine > 2)
+        work(std::integral_constant<int, 4>{});
+      else if (mine == 2)
+        work(std::integral_constant<int, 2>{});
+      else if (mine == 1)
+        work(std::integral_constant<int, 1>{});
     }
     __syncthreads();  // (the tile has been used)
     if (j + cluster < n_tiles) fetch(j + cluster);
