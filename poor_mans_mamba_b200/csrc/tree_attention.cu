@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(kTaWarps * 32) tree_attention_kernel(const Tre
 
 // Head sizes up to 256.  A cluster of blocks takes up to 32 rows of one request and key/value head; its blocks take the keys in tiles of 64 in
 // turn.  A tile of K and V lies in shared memory once for all rows (a block per row read the keys anew: 8 requests of 19 tokens with 32 / 8 heads
-// of 128 over 433 keys took 123 us, so 55; 12 requests of a token over 53 keys
-// 10, so 14).  A warp has up to eight rows and 32 of a tile's keys: a lane a key for the scores, a slice of the head a lane for the values, so maxima, sums
+// of 128 over 433 keys took 123 us, so 52; 12 requests of a token over 53 keys
+// 10 either way).  A warp has up to eight rows and 32 of a tile's keys: a lane a key for the scores, a slice of the head a lane for the values, so maxima, sums
 // and results stay in its registers.  In the end every block leaves (maximum, sum, unnormalised result) in its shared memory, and the cluster's
 // blocks join a share of the rows each, in the order of the blocks.  What bounds it: shared memory, 12 reads of 128 bytes for 32 products of a warp's scores,
 // 24 for 128 of its values.
@@ -506,9 +506,14 @@ template <typename S, int ACC>
 int launch_tree_rows(const TreeAttnArgs<S>& a, int T, int sms, cudaStream_t stream) {
   const int G = a.Hq / a.Hkv;
   const long long tiles = (static_cast<long long>(T) * G + kTfRows - 1) / kTfRows + min(T, a.n_seq);  // (at most)
-  const long long keys = static_cast<long long>(a.max_blocks) * a.page_size / kTfKeys + 1;                                // tiles of them, about
+  // Blocks of a cluster: the tables' width tells how many tiles of keys there may be, and requests of equal size how many tiles of rows.  Up
+  // to four blocks a multiprocessor (19 requests of 8 tokens over 608 keys, 32 / 8 heads of 128: 129 us with one, 77 with two), and from
+  // two on at least two tiles a block (6 of 2 over 514 keys: 30 us with eight, 21 with four).
+  const long long each = (static_cast<long long>(T) * G + a.n_seq - 1) / a.n_seq, blocks = a.n_seq * ((each + kTfRows - 1) / kTfRows) * a.Hkv;
+  long long keys = static_cast<long long>(a.max_blocks) * a.page_size / kTfKeys + 1;
+  if (a.window != 0) keys = min(keys, static_cast<long long>(abs(a.window)) / kTfKeys + 4);
   int cluster = kTfCluster;
-  while (cluster > 1 && (tiles * a.Hkv * cluster > 2ll * sms || cluster > keys)) cluster /= 2;
+  while (cluster > 1 && (blocks * cluster > 4ll * sms || cluster > keys || (blocks * cluster > 2ll * sms && 2 * cluster > keys))) cluster /= 2;
   if (tiles * cluster > 0x7fffffffll) return PMM_ERR_BAD_ARGUMENT;
   const size_t smem = tf_smem(a.Dh, sizeof(S));
   auto kern = tree_rows_kernel<S, ACC>;
