@@ -9,7 +9,7 @@
 // go out together; 512 requests are two loads a thread and length) instead of a launch of its own for the sums.
 //
 // keep_accepted: rows[l, plane, cu[s] + path[s, j]] -> pool[l, slot / P, plane, slot % P], slot = slots[cu[s] + j], j < count[s].
-// A copy: a block per (layer and plane, request), every thread's pieces asked for before the first is stored.
+// A copy: a block per (some layers and planes, request), a warp a row, up to eight pieces of a lane asked for before the first is stored.
 //
 // What these kernels write, later launches read ahead of their wait (sequence bounds, tables, cached keys): neither lets the
 // launch behind it begin early.
@@ -125,44 +125,54 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(const StepT
   }
 }
 
-constexpr int kKeepThreads = 128;
-constexpr int kKeepLoads = 4;  // pieces of a thread in flight
+constexpr int kKeepThreads = 256;
+constexpr int kKeepLoads = 4;   // pieces of a row that a lane has in flight
+constexpr int kKeepPlanes = 4;  // layers and planes of a block where there are many
 
 // V: the piece that a thread copies at a time (16 bytes where rows begin on such boundaries).
 template <typename V>
 __global__ void __launch_bounds__(kKeepThreads)
     keep_accepted_kernel(const V* rows, long long ld_layer, long long ld_plane, long long ld_row, int n_rows, V* pool, long long pages,
-                         int planes, int page_size, int width, const int* slots, const int* cu, const int* path, int path_width,
-                         const int* count) {
+                         int layers, int planes, int per_block, int page_size, int width, const int* slots, const int* cu, const int* path,
+                         int path_width, const int* count) {
   pdl_wait();
-  const int s = blockIdx.y, tid = threadIdx.x;
-  const int layer = blockIdx.x / planes, plane = blockIdx.x % planes;
+  const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t0 = cu[s], t1 = min(cu[s + 1], n_rows);
   const int kept = min(min(count[s], path_width), t1 - t0);
   if (kept <= 0) return;
-  const V* src = rows + layer * ld_layer + plane * ld_plane;
-  V* dst = pool + (static_cast<long long>(layer) * pages * planes + plane) * page_size * width;
+  const int lp0 = blockIdx.x * per_block, n_lp = min(per_block, layers * planes - lp0);
   const long long n_slots = pages * page_size;
-  const long long items = static_cast<long long>(kept) * width;
-  for (long long base = tid; base < items; base += kKeepThreads * kKeepLoads) {
-    V v[kKeepLoads];
-    long long to[kKeepLoads];
+  constexpr int kWarps = kKeepThreads / 32;
+  struct Row {
+    const V* src;
+    V* dst;
+  };
+  auto row = [&](int i) {  // row i of the block's: kept token i % kept of layer and plane lp0 + i / kept (none: no source)
+    Row r{nullptr, nullptr};
+    if (i >= kept * n_lp) return r;
+    const int lp = lp0 + i / kept, j = i % kept, layer = lp / planes, plane = lp - layer * planes;
+    const int node = path[static_cast<size_t>(s) * path_width + j], slot = slots[t0 + j];
+    if (node < 0 || t0 + node >= t1 || slot < 0 || slot >= n_slots) return r;
+    r.src = rows + layer * ld_layer + plane * ld_plane + static_cast<long long>(t0 + node) * ld_row;
+    r.dst = pool + ((static_cast<long long>(layer) * pages + slot / page_size) * planes + plane) * page_size * width +
+            static_cast<long long>(slot % page_size) * width;
+    return r;
+  };
+  for (int i = warp; i < kept * n_lp; i += 2 * kWarps) {  // two rows at a time
+    const Row r[2] = {row(i), row(i + kWarps)};
+    for (int base = lane; base < width; base += 32 * kKeepLoads) {
+      V v[2][kKeepLoads];
 #pragma unroll
-    for (int u = 0; u < kKeepLoads; ++u) {
-      const long long it = base + u * kKeepThreads;
-      to[u] = -1;
-      if (it < items) {
-        const int j = static_cast<int>(it / width), c = static_cast<int>(it - static_cast<long long>(j) * width);
-        const int node = path[static_cast<size_t>(s) * path_width + j], slot = slots[t0 + j];
-        if (node >= 0 && t0 + node < t1 && slot >= 0 && slot < n_slots) {
-          v[u] = src[static_cast<long long>(t0 + node) * ld_row + c];
-          to[u] = (static_cast<long long>(slot / page_size) * planes * page_size + slot % page_size) * width + c;
-        }
-      }
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int u = 0; u < kKeepLoads; ++u)
+          if (r[k].src != nullptr && base + 32 * u < width) v[k][u] = r[k].src[base + 32 * u];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int u = 0; u < kKeepLoads; ++u)
+          if (r[k].src != nullptr && base + 32 * u < width) r[k].dst[base + 32 * u] = v[k][u];
     }
-#pragma unroll
-    for (int u = 0; u < kKeepLoads; ++u)
-      if (to[u] >= 0) dst[to[u]] = v[u];
   }
 }
 
@@ -193,12 +203,14 @@ PMM_EXPORT int pmm_keep_accepted(const void* rows, long long ld_layer, long long
   // the widest piece that every row begins on
   const long long all = reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(pool) | (ld_layer * item) | (ld_plane * item) |
                         (ld_row * item) | (static_cast<long long>(width) * item);
-  const dim3 grid(layers * planes, n);
+  // four planes a block where a thousand blocks are left: 64 requests of 8 tokens, 32 layers of 1,024, 11.1 us, with one plane a block 12.9
+  const int per_block = static_cast<long long>(layers) * planes * n >= 4096 ? pmm::kKeepPlanes : 1;
+  const dim3 grid((layers * planes + per_block - 1) / per_block, n);
   auto go = [&](auto zero) {
     using V = decltype(zero);
     const int per = static_cast<int>(sizeof(V)) / item;
     pmm::launch_pdl(pmm::keep_accepted_kernel<V>, grid, dim3(pmm::kKeepThreads), 0, stream, static_cast<const V*>(rows), ld_layer / per,
-                    ld_plane / per, ld_row / per, n_rows, static_cast<V*>(pool), pages, planes, page_size, width / per, slots, cu, path, path_width,
+                    ld_plane / per, ld_row / per, n_rows, static_cast<V*>(pool), pages, layers, planes, per_block, page_size, width / per, slots, cu, path, path_width,
                     count);
     return pmm::launch_status();
   };

@@ -511,7 +511,7 @@ int launch_tree_rows(const TreeAttnArgs<S>& a, int T, int sms, cudaStream_t stre
   // two on at least two tiles a block (6 of 2 over 514 keys: 30 us with eight, 21 with four).
   const long long each = (static_cast<long long>(T) * G + a.n_seq - 1) / a.n_seq, blocks = a.n_seq * ((each + kTfRows - 1) / kTfRows) * a.Hkv;
   long long keys = static_cast<long long>(a.max_blocks) * a.page_size / kTfKeys + 1;
-  if (a.window != 0) keys = min(keys, static_cast<long long>(abs(a.window)) / kTfKeys + 4);
+  if (a.window != 0) keys = min(keys, llabs(static_cast<long long>(a.window)) / kTfKeys + 4);
   int cluster = kTfCluster;
   while (cluster > 1 && (blocks * cluster > 4ll * sms || cluster > keys || (blocks * cluster > 2ll * sms && 2 * cluster > keys))) cluster /= 2;
   if (tiles * cluster > 0x7fffffffll) return PMM_ERR_BAD_ARGUMENT;
