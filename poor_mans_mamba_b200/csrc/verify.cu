@@ -95,8 +95,8 @@ __device__ __forceinline__ void vf_table(double* table) {
   const int j = threadIdx.x;
   if (j < 32) table[j] = __hiloint2double(__double2hiint(kVfPowers[j]) - (j << 15), __double2loint(kVfPowers[j]));
 }
-// 32 log2(e) / T (temperatures below 1e-36 count as that: no product below leaves its type)
-__device__ __forceinline__ double vf_scale(float temp) { return 32.0 * 1.4426950408889634074 / fmax(static_cast<double>(temp), 1e-36); }
+// 32 log2(e) / T (temperatures outside 1e-36..1e36 count as the nearer of the two: no product below leaves its type)
+__device__ __forceinline__ double vf_scale(float temp) { return 32.0 * 1.4426950408889634074 / fmin(fmax(static_cast<double>(temp), 1e-36), 1e36); }
 
 __device__ __forceinline__ float vf_clean(float l) { return l == l ? l : -CUDART_INF_F; }
 
@@ -219,12 +219,16 @@ __global__ void __launch_bounds__(kVfThreads, 4) verify_stats_kernel(const Verif
       for (int k = 0; k < kVfEach; ++k) sum += v[k] == top ? 1.0 : 0.0;
     } else if (top > -CUDART_INF_F) {
       if (EXACT) {
-        // (what counts for nothing, NaN among it, is held where its weight, 2^-1000, leaves a sum of 1 and more as it is)
-        const float low = top - 31900.f / static_cast<float>(scale);
+        // What counts for nothing, NaN and -inf among it, is held at an exponent of -31900 / 32: a weight of 2^-997 leaves a sum of 1 and
+        // more as it is.  The exponent is held, not the logit: beside a large maximum or a small temperature no float says "31900 less".
+        // (It is not above 0, so of two numbers the lower one has the larger upper half.)
+        const unsigned least = static_cast<unsigned>(__double2hiint(-31900.0));
         double part[2] = {0.0, 0.0};
 #pragma unroll
-        for (int k = 0; k < kVfEach; ++k)
-          part[k & 1] += vf_exp2((static_cast<double>(fmaxf(v[k], low)) - static_cast<double>(top)) * scale, s_table);
+        for (int k = 0; k < kVfEach; ++k) {
+          const double y = (static_cast<double>(fmaxf(v[k], -CUDART_INF_F)) - static_cast<double>(top)) * scale;
+          part[k & 1] += vf_exp2(__hiloint2double(static_cast<int>(min(static_cast<unsigned>(__double2hiint(y)), least)), __double2loint(y)), s_table);
+        }
         sum = part[0] + part[1];
       } else {
         const float c2 = static_cast<float>(scale * 0.03125);

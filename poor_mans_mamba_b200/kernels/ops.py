@@ -2514,7 +2514,8 @@ def verify_drafts(logits: Tensor, tokens: Tensor, cu_seqlens: Tensor, uniforms: 
     Written per request: ``count`` [n] (1 + kept drafts; 0 for a request without tokens), ``tokens_out`` [n, width] the kept
     tokens and the next one, ``path`` [n, width] the root and the kept tokens' places among the request's, both -1 behind
     them.  Drafts deeper than the outputs are wide are not looked at.
-    NaN logits count as -inf.  A row that holds nothing else keeps no draft and gives token 0."""
+    NaN logits count as -inf.  A row that holds nothing else keeps no draft and gives token 0.  Positive temperatures
+    outside 1e-36..1e36 count as the nearer of the two."""
     what = "verify_drafts"
     stream = _launch_stream(what, logits, tokens, cu_seqlens, uniforms, tokens_out, path, count, scratch, temperature, parents, draft_logits)
     if not (logits.dtype is torch.float32 and logits.dim() == 2 and logits.stride(1) == 1):
