@@ -74,7 +74,7 @@ __device__ __forceinline__ bool ta_sees(const unsigned long long* mask, int word
 // Head sizes beyond 256.  A block per (token, query head); its eight warps share the keys in pieces of 32 (a key per lane for the scores, a
 // slice of the head per lane for the values) and merge their maxima, sums and results at the end.
 template <typename S, int ACC>
-__global__ void __launch_bounds__(kTaWarps * 32) tree_attention_kernel(const TreeAttnArgs<S> a) {
+__global__ void __launch_bounds__(kTaWarps * 32) tree_attention_kernel(const TreeAttnArgs<S> a, int T) {
   extern __shared__ float qs[];  // the query, then every warp's result
   __shared__ float s_m[kTaWarps], s_l[kTaWarps];
   pdl_launch_dependents();
@@ -89,7 +89,9 @@ __global__ void __launch_bounds__(kTaWarps * 32) tree_attention_kernel(const Tre
     if (c < kTaWarps * 32) break;
   }
   const int hk = hq / (a.Hq / a.Hkv);
-  const int t0 = a.cu[seq], n_new = a.cu[seq + 1] - t0, held = max(0, static_cast<int>(min(static_cast<long long>(a.held[seq]), static_cast<long long>(a.max_blocks) * a.page_size)));
+  // (bounds may pass the step's rows: those that are not there are not read)
+  const int t0 = min(max(a.cu[seq], 0), T), n_new = min(max(a.cu[seq + 1], t0), T) - t0;
+  const int held = max(0, static_cast<int>(min(static_cast<long long>(a.held[seq]), static_cast<long long>(a.max_blocks) * a.page_size)));
   const int lo = a.window != 0 ? first_visible(a.positions[t], a.window) : 0;
   const int* bt = a.block_table + static_cast<size_t>(seq) * a.max_blocks;
   const unsigned long long* mask = a.mask ? a.mask + static_cast<size_t>(t) * a.words : nullptr;
@@ -556,7 +558,7 @@ PMM_EXPORT int pmm_tree_attention(const void* q, long long ldq, const void* k, l
     if (Dh <= 64) return pmm::launch_tree_rows<S, 2>(a, T, sms, stream);
     if (Dh <= 128) return pmm::launch_tree_rows<S, 4>(a, T, sms, stream);
     if (Dh <= 256) return pmm::launch_tree_rows<S, 8>(a, T, sms, stream);
-    pmm::launch_pdl(pmm::tree_attention_kernel<S, 16>, dim3(T, Hq), dim3(pmm::kTaWarps * 32), static_cast<size_t>(pmm::kTaWarps) * Dh * sizeof(float), stream, a);
+    pmm::launch_pdl(pmm::tree_attention_kernel<S, 16>, dim3(T, Hq), dim3(pmm::kTaWarps * 32), static_cast<size_t>(pmm::kTaWarps) * Dh * sizeof(float), stream, a, T);
   });
   return pmm::launch_status();
 }

@@ -66,3 +66,23 @@ def test_verify_drafts_infinite_temperature():
             K().verify_drafts(logits.to(DEV), i32([0] * 3), i32([0, 1, 2, 3]), torch.full((3,), u, device=DEV), out, path, i32([0] * 3),
                               K().verify_drafts_scratch(3, 100, DEV), temperature=torch.full((3,), math.inf, device=DEV), draft_logits=draft)
             assert out[:, 0].tolist() == [int(u * 50)] * 3
+
+
+# ----------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(2, 1, 512), (2, 1, 256), (8, 2, 64), (6, 2, 128)])
+def test_tree_attention_bounds_beyond_the_step(dtype, heads):
+    """Bounds that pass the step's rows (`step_tables` leaves them so where the tokens have no room), masks that name the tokens that are
+    not there: nothing behind the rows of q, k and v is read."""
+    c = Case([70, 130], [5, 7], heads, dtype, 64, seed=21, extra_rows=24)
+    T = c.cu[-1]
+    c.mask = torch.full_like(c.mask, -1)
+    for see in c.see:
+        see[:] = True
+    for t in (c.q, c.k, c.v):
+        t[T:] = math.nan
+    whole, held, cu = c.out, i32(c.held), i32([0, 5, T + 17])
+    q, k, v, c.out = (t[:T] for t in (c.q, c.k, c.v, whole))
+    K().tree_attention(q, k, v, c.pool, c.table, held, cu, c.out, c.hq, c.hkv, c.d, c.scale, K().tree_attention_scratch(DEV), mask=c.mask[:T])
+    c.out = whole
+    c.check()
