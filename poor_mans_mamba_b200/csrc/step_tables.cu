@@ -40,17 +40,20 @@ struct StepTablesArgs {
   int words;
 };
 
+__device__ __forceinline__ int saturated(long long x) { return static_cast<int>(min(x, 0x7fffffffll)); }
+
 __device__ __forceinline__ int blocks_after(int held, int fresh, int blocks, int page_size) {
-  return max(blocks, static_cast<int>((static_cast<long long>(held) + fresh + page_size - 1) / page_size));
+  return max(blocks, saturated((static_cast<long long>(held) + fresh + page_size - 1) / page_size));
 }
 
 __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(const StepTablesArgs a) {
-  __shared__ int s_sum[2][kTablesThreads / 32];
+  __shared__ long long s_sum[2][kTablesThreads / 32];
   __shared__ int s_up[kTablesNodes];
   pdl_wait();
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int held = max(a.held[s], 0), fresh = max(a.fresh[s], 0), blocks = max(a.blocks[s], 0);
-  int tokens = 0, pages = 0;  // of the requests in front of this one
+  // of the requests in front of this one (in 64 bits: lengths that fit no step must not come out as places in front of the tables)
+  long long tokens = 0, pages = 0;
   for (int i = tid; i < s; i += kTablesThreads) {
     const int f = max(a.fresh[i], 0), b = max(a.blocks[i], 0);
     tokens += f;
@@ -66,30 +69,31 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(const StepT
     s_sum[1][warp] = pages;
   }
   __syncthreads();
-  int t0 = 0, g0 = 0;
+  long long first = 0, g0 = 0;
 #pragma unroll
   for (int w = 0; w < kTablesThreads / 32; ++w) {
-    t0 += s_sum[0][w];
+    first += s_sum[0][w];
     g0 += s_sum[1][w];
   }
   const int after = blocks_after(held, fresh, blocks, a.page_size);
+  const int t0 = saturated(first);
   if (tid == 0) {
     a.cu[s] = t0;
     a.blocks_out[s] = after;
     if (s == a.n - 1) {
-      a.cu[a.n] = t0 + fresh;
-      a.taken[0] = g0 + after - blocks;
+      a.cu[a.n] = saturated(first + fresh);
+      a.taken[0] = saturated(g0 + after - blocks);
     }
   }
   int* row = a.table + static_cast<size_t>(s) * a.width;
   // block b's page: one of the request's own, or the next free one
-  auto page_of = [&](int b) {
-    if (b >= a.width) return a.spare;
-    if (b < blocks) return row[b];
-    const int i = g0 + b - blocks;
+  auto page_of = [&](unsigned b) {
+    if (b >= static_cast<unsigned>(a.width)) return a.spare;
+    if (b < static_cast<unsigned>(blocks)) return row[b];
+    const long long i = g0 + b - blocks;
     return i < a.n_free ? a.free_pages[i] : a.spare;
   };
-  for (int b = blocks + tid; b < a.width; b += kTablesThreads) row[b] = b < after ? page_of(b) : a.spare;
+  for (int b = min(blocks, a.width) + tid; b < a.width; b += kTablesThreads) row[b] = b < after ? page_of(b) : a.spare;
 
   const int n = min(fresh, a.cap - t0);  // (t0 <= cap unless the lengths do not fit the step)
   const bool cached = n <= kTablesNodes;
@@ -98,10 +102,12 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(const StepT
     __syncthreads();
   }
   for (int i = tid; i < n; i += kTablesThreads) {
-    const int t = t0 + i, pos = held + i;
-    const int page = page_of(pos / a.page_size);
+    const int t = t0 + i;
+    const unsigned pos = static_cast<unsigned>(held) + i, size = a.page_size;
+    const int page = page_of(pos / size);
+    const long long slot = static_cast<long long>(page) * a.page_size + pos % size;
     a.seq_of[t] = s;
-    a.slots[t] = page < 0 || page == a.spare ? -1 : page * a.page_size + pos % a.page_size;
+    a.slots[t] = page < 0 || page == a.spare || slot > 0x7fffffffll ? -1 : static_cast<int>(slot);
     int depth = i;
     if (a.parents != nullptr) {
       depth = 0;
@@ -121,7 +127,7 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(const StepT
       for (int w = 0; w < 4; ++w)
         if (w < a.words) a.masks[static_cast<size_t>(t) * a.words + w] = bits[w];
     }
-    a.positions[t] = held + depth;
+    a.positions[t] = saturated(static_cast<long long>(held) + depth);
   }
 }
 

@@ -86,3 +86,42 @@ def test_tree_attention_bounds_beyond_the_step(dtype, heads):
     K().tree_attention(q, k, v, c.pool, c.table, held, cu, c.out, c.hq, c.hkv, c.d, c.scale, K().tree_attention_scratch(DEV), mask=c.mask[:T])
     c.out = whole
     c.check()
+
+
+# ----------------------------------------------------------------------------- tables
+@pytest.mark.parametrize("page", [1, 64])
+@pytest.mark.parametrize("tree", [False, True])
+def test_step_tables_of_lengths_beyond_32_bits(page, tree):
+    """Lengths whose sums pass 32 bits: bounds and counts stay at the largest number, places that there cannot be are -1, and
+    nothing is written or read outside the tables."""
+    most, cap, n = 2 ** 31 - 1, 9, 5
+    held, new, blocks = [3, most, 0, most - 1, 5], [4, most, most, 2, 6], [4, most, 0, 1, most]
+    rows = [[7, 8, 9, 6], [0, 1, 2, 3], [30, 30, 30, 30], [4, 30, 30, 30], [10, 11, 12, 13]]
+    guard = 300
+
+    def framed(size, fill=-7, dtype=torch.int32):
+        whole = torch.full((size + 2 * guard,), fill, dtype=dtype, device=DEV)
+        return whole, whole[guard:guard + size]
+
+    out = {k: framed(m) for k, m in dict(cu=n + 1, seq=cap, pos=cap, slots=cap, blocks=n, taken=1, table=4 * n).items()}
+    out["masks"] = framed(cap, dtype=torch.int64)
+    out["table"][1].copy_(i32(rows).view(-1))
+    parents = i32([-1, 0, 0, 2] + [-1, 0, 1, 2, 3])
+    K().step_tables(i32(held), i32(new), i32(blocks), out["table"][1].view(n, 4), i32([20, 21]), page, 30, out["cu"][1], out["seq"][1], out["pos"][1],
+                    out["slots"][1], out["blocks"][1], out["taken"][1], parents=parents if tree else None,
+                    masks=out["masks"][1].view(cap, 1) if tree else None)
+    for whole, inside in out.values():
+        assert (whole[:guard] == -7).all() and (whole[-guard:] == -7).all()
+    got = {k: v[1].tolist() for k, v in out.items()}
+    need = [max(b, min(-(-(h + m) // page), most)) for h, m, b in zip(held, new, blocks)]
+    assert got["cu"] == [0, 4, most, most, most, most] and got["blocks"] == need
+    assert got["taken"] == [min(most, sum(a - b for a, b in zip(need, blocks)))]
+    assert got["seq"] == [0] * 4 + [1] * 5
+    assert got["pos"] == [3 + d for d in ((0, 1, 1, 2) if tree else range(4))] + [most] * 5
+    # pages of 1: request 0 needs seven of a table of four (three are counted as taken and have no place), so the others find none left;
+    # of 64: it needs none, and the two free ones go to request 2
+    assert got["slots"] == ([6, -1, -1, -1] if page == 1 else [7 * 64 + 3 + i for i in range(4)]) + [-1] * 5
+    third = [30] * 4 if page == 1 else [20, 21, 30, 30]
+    assert [got["table"][4 * s:4 * s + 4] for s in range(n)] == [rows[0], rows[1], third, [4, 30, 30, 30], rows[4]]
+    if tree:
+        assert got["masks"] == [1, 3, 5, 13, 1, 3, 7, 15, 31]
