@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kKeepThreads)
                          int path_width, const int* count) {
   pdl_wait();
   const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t0 = cu[s], t1 = min(cu[s + 1], n_rows);
+  const int t0 = max(cu[s], 0), t1 = min(max(cu[s + 1], 0), n_rows);  // (no bound leads out of the rows)
   const int kept = min(min(count[s], path_width), t1 - t0);
   if (kept <= 0) return;
   const int lp0 = blockIdx.x * per_block, n_lp = min(per_block, layers * planes - lp0);

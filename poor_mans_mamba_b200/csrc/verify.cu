@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_walk_kernel(const Verify
   __syncthreads();
   pdl_wait();
   const int cluster = a.cluster, s = blockIdx.x / cluster, rank = blockIdx.x % cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int t0 = a.cu[s], t1 = min(a.cu[s + 1], a.n_rows);
+  const int t0 = max(a.cu[s], 0), t1 = min(max(a.cu[s + 1], 0), a.n_rows);  // (no bound leads out of the rows)
   const int nodes = t1 - t0;
   const float temp = a.temperature ? a.temperature[s] : 0.f;
   const bool greedy = !(temp > 0.f);

@@ -125,3 +125,30 @@ def test_step_tables_of_lengths_beyond_32_bits(page, tree):
     assert [got["table"][4 * s:4 * s + 4] for s in range(n)] == [rows[0], rows[1], third, [4, 30, 30, 30], rows[4]]
     if tree:
         assert got["masks"] == [1, 3, 5, 13, 1, 3, 7, 15, 31]
+
+
+# ----------------------------------------------------------------------------- bounds
+@pytest.mark.parametrize("cu", [[-4, 2, 6], [0, 2, 9], [5, -2 ** 31, 6], [-2 ** 31, -5, 6], [3, 2 ** 31 - 1, 2 ** 31 - 1]])
+@pytest.mark.parametrize("mode", ["tree", "drawn"])
+def test_verify_drafts_bounds_outside_the_rows(cu, mode):
+    """Bounds below the first row or beyond the last are cut to the rows; a request that ends before it begins has none."""
+    V, T = 300, 6
+    logits, draft, _, tokens, u = drafts_of([3, 3], V, 4, [1.0, 1.0], False)
+    parents = [-1, 0, 0, 1, 2, 3]
+    out, path, count = i32([[-9] * 4] * 2), i32([[-9] * 4] * 2), i32([-9] * 2)
+    K().verify_drafts(logits, i32(tokens), i32(cu), u.to(DEV), out, path, count, K().verify_drafts_scratch(T, V, DEV), temperature=torch.ones(2, device=DEV),
+                      parents=i32(parents) if mode == "tree" else None, draft_logits=draft if mode == "drawn" else None)
+    for s in range(2):
+        first = min(max(cu[s], 0), T)
+        cut = [first, max(first, min(max(cu[s + 1], 0), T))]
+        want = P.verify(logits.cpu(), tokens, cut, u, 4, [1.0], parents if mode == "tree" else None, draft.cpu() if mode == "drawn" else None)
+        assert dict(tokens=[out[s].tolist()], path=[path[s].tolist()], count=[int(count[s])]) == want
+
+
+@pytest.mark.parametrize("cu", [[-4, 2, 6], [0, 2, 9], [5, -2 ** 31, 6], [-2 ** 31, -5, 6], [3, 2 ** 31 - 1, 2 ** 31 - 1]])
+def test_keep_accepted_bounds_outside_the_rows(cu):
+    rows, pool = torch.randn(2, 2, 6, 64, device=DEV), torch.randn(2, 3, 2, 8, 64, device=DEV)
+    slots, path, count = [3, 20, 7, 11, 1, 16], [[0, 1, 3], [0, 2, 1]], [3, 3]
+    want = P.keep(rows.cpu(), pool.cpu(), slots, [min(max(x, 0), 6) for x in cu], path, count)
+    K().keep_accepted(rows, pool, i32(slots), i32(cu), i32(path), i32(count))
+    assert torch.equal(pool.cpu(), want)
