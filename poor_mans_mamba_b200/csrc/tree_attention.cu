@@ -156,10 +156,10 @@ __global__ void __launch_bounds__(kTaWarps * 32) tree_attention_kernel(const Tre
       }
     }
   }
-  if (a.sink && warp == 0) {  // a score without key or value that counts once
-    const float m_new = fmaxf(m, a.sink[hq]);
-    const float corr = expf(m - m_new);
-    l = l * corr + expf(a.sink[hq] - m_new);
+  if (a.sink && warp == 0) {  // a score without key or value that counts once (of -inf: not at all)
+    const float m_new = fmaxf(m, a.sink[hq]), mu = m_new == -CUDART_INF_F ? 0.f : m_new;
+    const float corr = expf(m - mu);
+    l = l * corr + expf(a.sink[hq] - mu);
 #pragma unroll
     for (int i = 0; i < ACC; ++i) acc[i] *= corr;
     m = m_new;

@@ -856,10 +856,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
         const bool row_ok = row < n_rows;
         if (whole) {
           if (a.sink != nullptr && row_ok) {
-            // a score without key or value that counts once; maxima are kept in units of log 2
+            // a score without key or value that counts once (of -inf: not at all); maxima are kept in units of log 2
             const float sk = a.sink[hq] * 1.4426950408889634f;
-            const float m_new = fmaxf(m, sk), f = exp2f(m - m_new);
-            l = l * f + exp2f(sk - m_new);
+            const float m_new = fmaxf(m, sk), mu = m_new == -CUDART_INF_F ? 0.f : m_new, f = exp2f(m - mu);
+            l = l * f + exp2f(sk - mu);
             w0 *= f;
             w1 *= f;
           }

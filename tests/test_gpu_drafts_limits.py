@@ -152,3 +152,22 @@ def test_keep_accepted_bounds_outside_the_rows(cu):
     want = P.keep(rows.cpu(), pool.cpu(), slots, [min(max(x, 0), 6) for x in cu], path, count)
     K().keep_accepted(rows, pool, i32(slots), i32(cu), i32(path), i32(count))
     assert torch.equal(pool.cpu(), want)
+
+
+# ----------------------------------------------------------------------------- attention of rows that see nothing
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (6, 2, 128), (16, 1, 64), (32, 2, 128), (2, 1, 256), (2, 1, 512)])
+@pytest.mark.parametrize("held,new", [([0, 0, 0], [40, 1, 64]), ([200], [64]), ([0], [130]), ([0] * 200, [3] * 200)])
+def test_tree_attention_sinks_of_minus_infinity(dtype, heads, held, new):
+    """Heads without a sink (-inf) beside heads with one: rows that see nothing are zero, whether their unit is one block's or was cut,
+    and no row is harmed by keys of its request that it does not see."""
+    c = Case(held, new, heads, dtype, 64, seed=31, words=3 if max(new) > 64 else 1)
+    for see in c.see:
+        see[:, :32] = False
+        see[::3] = False
+    c.write_mask()
+    sink = torch.randn(heads[0], generator=torch.Generator().manual_seed(3))
+    sink[::2] = -math.inf
+    for s in (torch.full_like(sink, -math.inf), sink):
+        c.run(1, s.to(DEV))
+        c.check(1, s.to(DEV))
