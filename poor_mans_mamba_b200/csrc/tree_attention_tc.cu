@@ -1034,11 +1034,15 @@ PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k
     return PMM_ERR_BAD_ARGUMENT;
   for (const void* p : {q, k, v, pool, static_cast<const void*>(out), static_cast<const void*>(scratch)})
     if (reinterpret_cast<uintptr_t>(p) % 16) return PMM_ERR_BAD_ARGUMENT;
+  const long long kv_dim = static_cast<long long>(Hkv) * Dh;
+  if (T == 1) {  // (a matrix of one row has no stride of its own)
+    ldq = static_cast<long long>(Hq) * Dh;
+    ldk = ldv = kv_dim;
+  }
   if (ldq % 8 || ldk % 8 || ldv % 8) return PMM_ERR_BAD_ARGUMENT;
   pmm::EncodeTiledFn fn = pmm::encode_tiled_fn();
   if (!fn) return PMM_ERR_BAD_ARGUMENT;
   const int box = page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : page_size % 16 == 0 ? 16 : 8;
-  const long long kv_dim = static_cast<long long>(Hkv) * Dh;
   pmm::TreeMaps maps;
   bool ok = true;
   auto encode = [&](CUtensorMap* map, const void* base, long long n, long long ld, int box_rows) {
@@ -1049,7 +1053,6 @@ PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k
     ok = ok && fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
-  if (T == 1) ldk = ldv = kv_dim;  // (a matrix of one row has no stride of its own)
   encode(&maps.pool, pool, static_cast<long long>(pages) * 2 * page_size, kv_dim, box);
   encode(&maps.own_k, k, T, ldk, pmm::kAtBox);
   encode(&maps.own_v, v, T, ldv, pmm::kAtBox);

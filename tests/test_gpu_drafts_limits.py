@@ -171,3 +171,19 @@ def test_tree_attention_sinks_of_minus_infinity(dtype, heads, held, new):
     for s in (torch.full_like(sink, -math.inf), sink):
         c.run(1, s.to(DEV))
         c.check(1, s.to(DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (12, 2, 128), (2, 1, 256)])
+def test_tree_attention_of_one_row_of_any_stride(dtype, heads):
+    """A step of one token in slices of rows whose length is odd: the only row begins where it has to."""
+    c = Case([200], [1], heads, dtype, 64, seed=5)
+    w = c.hq * c.d
+    for name in ("q", "k", "v"):
+        t = getattr(c, name)
+        wide = torch.zeros(2, w + 515 if w % 2 == 0 else w + 516, dtype=dtype, device=DEV)
+        wide[:1, :t.shape[1]] = t
+        setattr(c, name, wide[:1, :t.shape[1]])
+        assert getattr(c, name).stride(0) % 2 == 1
+    c.run()
+    c.check()
