@@ -10,6 +10,7 @@
 #define PMM_DTYPE_F32 0
 #define PMM_DTYPE_BF16 1
 #define PMM_ERR_BAD_ARGUMENT 1001  // outside the cudaError_t range that launches return
+#define PMM_ERR_OVERLAP 1002       // what is written lies, whole or in part, in what is read
 
 #define PMM_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -125,6 +126,16 @@ __device__ __forceinline__ float scan_exp(float v) { return expf(v); }
 __device__ __forceinline__ double scan_exp(double v) { return exp(v); }
 
 inline int launch_status() { return static_cast<int>(cudaGetLastError()); }
+
+// Whether any of `rows` rows of `width` bytes, `ld` bytes apart, lies in or reaches into [to, to + bytes).
+inline bool rows_overlap(const void* first, long long rows, long long ld, long long width, const void* to, long long bytes) {
+  if (!first || !to || rows <= 0 || width <= 0 || bytes <= 0) return false;
+  const long long at = static_cast<long long>(reinterpret_cast<uintptr_t>(first)), from = static_cast<long long>(reinterpret_cast<uintptr_t>(to));
+  // the first row that ends behind `to`
+  const long long i = at + width > from || ld <= 0 ? 0 : (from - at - width) / ld + 1;
+  return i < rows && at + i * ld + width > from && at + i * ld < from + bytes;
+}
+inline bool overlap(const void* a, long long bytes_a, const void* b, long long bytes_b) { return rows_overlap(a, 1, 0, bytes_a, b, bytes_b); }
 
 // Programmatic dependent launch.  A kernel started with launch_pdl may begin while the kernel
 // before it on the stream is still running; pdl_wait() inside it returns once that kernel has

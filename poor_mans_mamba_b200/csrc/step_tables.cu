@@ -206,6 +206,12 @@ PMM_EXPORT int pmm_keep_accepted(const void* rows, long long ld_layer, long long
   if (pages <= 0 || page_size <= 0 || width <= 0 || path_width <= 0 || n_rows < 0 || n > 65535 || (item != 2 && item != 4) ||
       static_cast<long long>(layers) * planes > 0x7fffffffll)
     return PMM_ERR_BAD_ARGUMENT;
+  const long long pool_bytes = static_cast<long long>(layers) * pages * planes * page_size * width * item;
+  for (int l = 0; l < layers; ++l)
+    for (int p = 0; p < planes; ++p)
+      if (pmm::rows_overlap(static_cast<const char*>(rows) + (l * ld_layer + p * ld_plane) * item, n_rows, ld_row * item,
+                            static_cast<long long>(width) * item, pool, pool_bytes))
+        return PMM_ERR_OVERLAP;
   // the widest piece that every row begins on
   const long long all = reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(pool) | (ld_layer * item) | (ld_plane * item) |
                         (ld_row * item) | (static_cast<long long>(width) * item);

@@ -28,6 +28,7 @@ from . import build as _build
 Tensor = torch.Tensor
 
 PMM_ERR_BAD_ARGUMENT = 1001
+PMM_ERR_OVERLAP = 1002
 
 
 class KernelError(RuntimeError):
@@ -224,6 +225,8 @@ def _call(name: str, *args) -> None:
     if rc != 0:
         if rc == PMM_ERR_BAD_ARGUMENT:
             raise KernelError(f"{name}: sizes or arguments outside what the kernel supports")
+        if rc == PMM_ERR_OVERLAP:
+            raise KernelError(f"{name}: a tensor that is written must not lie, not even in part, in one that is read or written beside it")
         raise KernelError(f"{name}: CUDA error {rc} at launch")
 
 
@@ -2554,7 +2557,7 @@ def keep_accepted(rows: Tensor, pool: Tensor, slots: Tensor, cu_seqlens: Tensor,
     """The kept tokens' rows into the cache pages: row cu[s] + path[s, j] of ``rows`` [layers, planes, T, width] to place
     slots[cu[s] + j] of ``pool`` [layers, pages, planes, page_size, width], j < count[s] (`verify_drafts`, `step_tables`; both
     may also be one layer's, without the first dimension).  Places of -1, and nodes that the request does not have, are left out.
-    ``rows`` may be a slice with strides; a row is contiguous.  What it writes, a launch directly behind may read ahead of its
+    ``rows`` may be a slice with strides, of which no row lies in the pool; a row is contiguous.  What it writes, a launch directly behind may read ahead of its
     wait: this one lets none begin early."""
     what = "keep_accepted"
     stream = _launch_stream(what, rows, pool, slots, cu_seqlens, path, count)
@@ -2571,8 +2574,6 @@ def keep_accepted(rows: Tensor, pool: Tensor, slots: Tensor, cu_seqlens: Tensor,
         raise KernelError(f"{what}: a place per token and a path per request")
     if pool.shape[1] * pool.shape[3] > 0x7fffffff:
         raise KernelError(f"{what}: places in the pool do not fit 32 bits")
-    if 0 <= rows.data_ptr() - pool.data_ptr() < pool.numel() * pool.element_size():
-        raise KernelError(f"{what}: rows must not lie in the pool (they are read and written side by side)")
     if T == 0:
         return
     sl, sp, sr, _ = rows.stride()

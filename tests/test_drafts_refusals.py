@@ -93,3 +93,28 @@ def test_plain_tables_of_a_small_step():
     assert t["seq_of"] == [0, 0, 1, -7, -7] and t["positions"] == [3, 4, 0, -7, -7] and t["slots"] == [5 * 4 + 3, 1 * 4, 2 * 4, -7, -7]
     assert t["masks"] == [[1], [3], [1], [-7], [-7]]
     assert math.isclose(sum(t["cu"]), 8)
+
+
+# ----------------------------------------------------------------------------- tensors that lie in one another
+def overlaps(name, good, **other):
+    args = dict(good)
+    for key, value in other.items():
+        assert key in args
+        args[key] = value
+    return K._fn(name)(*args.values()) == K.PMM_ERR_OVERLAP
+
+
+def test_keep_accepted_refuses_rows_in_the_pool():
+    """The pool has 1 MiB here; two planes of four rows of 128 bytes, 200 bytes apart."""
+    pool = 1 << 30
+    good = dict(KEEP, pool=pool, pages=64, page_size=64, planes=2, width=64, item=2, ld_plane=400, ld_layer=800, ld_row=100, slots=A, n=2)
+    size = 64 * 2 * 64 * 64 * 2
+    last = (400 + 3 * 100 + 64) * 2     # bytes from the first row to the end of the last
+    for at, bad in [(pool, True), (pool + 500, True), (pool - 2, True), (pool - last, False), (pool - last + 2, True), (pool + size - 2, True),
+                    (pool + size, False), (pool - 8 * last, False)]:
+        assert overlaps("pmm_keep_accepted", good, rows=at) == bad, at - pool
+    # rows around a pool: layers in front of it and behind it, none in it
+    wide = dict(good, layers=2, pages=16, ld_layer=(size + 4096) // 2)
+    assert not overlaps("pmm_keep_accepted", wide, rows=pool - 4096)
+    assert overlaps("pmm_keep_accepted", dict(wide, ld_layer=size // 4), rows=pool - 4096)
+    assert not overlaps("pmm_keep_accepted", dict(good, n_rows=0), rows=pool)
