@@ -2367,8 +2367,8 @@ def step_tables(held: Tensor, new: Tensor, blocks: Tensor, table: Tensor, free_p
     """A step's tables from the requests' lengths, on the device: ``held`` [n] tokens in the cache, ``new`` [n] tokens in this
     step (0: none), ``blocks`` [n] pages that a request owns already, all int32.
     ``table`` [n, width] keeps its first ``blocks`` entries; the pages that held + new tokens need beyond them are taken from
-    ``free_pages`` in the requests' order, everything behind is ``spare_page``.  Written: ``cu`` [n + 1], ``blocks_out`` [n]
-    (not ``blocks`` itself), ``taken`` [1] the number of pages that the step needs (more than there are free ones, or a table
+    ``free_pages`` in the requests' order, everything behind is ``spare_page``.  Written, and not in what is read (``blocks_out``
+    is not ``blocks`` itself: every request reads those in front of it): ``cu`` [n + 1], ``blocks_out`` [n], ``taken`` [1] the number of pages that the step needs (more than there are free ones, or a table
     that is too narrow: the missing pages are the spare page), and per token ``seq_of``, ``positions`` and ``slots`` (page *
     page_size + offset of the request's i-th token at held + i; -1 where its page is missing).  The three have room for a step
     of a fixed size: what lies behind the last token is left as it was.
@@ -2384,8 +2384,6 @@ def step_tables(held: Tensor, new: Tensor, blocks: Tensor, table: Tensor, free_p
           ("table", table, None))
     if n == 0 or table.dim() != 2 or table.shape[0] != n or table.shape[1] == 0:
         raise KernelError(f"{what}: table must be int32 [requests, blocks], and there must be a request")
-    if blocks_out.data_ptr() == blocks.data_ptr():
-        raise KernelError(f"{what}: blocks_out must not be blocks (every request reads those in front of it)")
     if page_size <= 0 or spare_page < 0 or (spare_page + 1) * page_size > 0x7fffffff:
         raise KernelError(f"{what}: places in the pool do not fit 32 bits")
     words = 0

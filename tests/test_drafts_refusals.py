@@ -118,3 +118,17 @@ def test_keep_accepted_refuses_rows_in_the_pool():
     assert not overlaps("pmm_keep_accepted", wide, rows=pool - 4096)
     assert overlaps("pmm_keep_accepted", dict(wide, ld_layer=size // 4), rows=pool - 4096)
     assert not overlaps("pmm_keep_accepted", dict(good, n_rows=0), rows=pool)
+
+
+def test_step_tables_refuses_outputs_in_its_inputs():
+    """Two requests of ten tokens: lengths of 8 bytes, a table of 64, tokens' tensors of 40."""
+    names = ["held", "new", "blocks", "free", "table", "cu", "seq_of", "positions", "slots", "blocks_out", "taken", "parents", "masks"]
+    apart = dict(TABLES, words=1, **{k: A + 4096 * i for i, k in enumerate(names)})
+    assert not overlaps("pmm_step_tables", apart)
+    size = dict(held=8, new=8, blocks=8, parents=40)
+    for out in ("cu", "blocks_out", "taken", "table", "seq_of", "positions", "slots", "masks"):
+        for name, bytes_of in size.items():
+            for at, bad in ((0, True), (bytes_of - 4, True), (bytes_of, False)):
+                assert overlaps("pmm_step_tables", apart, **{out: apart[name] + at}) == bad, (out, name, at)
+    assert overlaps("pmm_step_tables", apart, cu=apart["blocks"] - 8) and not overlaps("pmm_step_tables", apart, cu=apart["blocks"] - 12)
+    assert overlaps("pmm_step_tables", apart, table=apart["free"] - 60) and not overlaps("pmm_step_tables", apart, table=apart["free"] - 64)
