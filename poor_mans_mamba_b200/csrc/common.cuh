@@ -136,6 +136,17 @@ inline bool rows_overlap(const void* first, long long rows, long long ld, long l
   return i < rows && at + i * ld + width > from && at + i * ld < from + bytes;
 }
 inline bool overlap(const void* a, long long bytes_a, const void* b, long long bytes_b) { return rows_overlap(a, 1, 0, bytes_a, b, bytes_b); }
+struct Extent {
+  const void* at;
+  long long bytes;
+};
+template <int N, int M>
+inline bool overlap(const Extent (&a)[N], const Extent (&b)[M]) {
+  for (const Extent& x : a)
+    for (const Extent& y : b)
+      if (overlap(x.at, x.bytes, y.at, y.bytes)) return true;
+  return false;
+}
 
 // Programmatic dependent launch.  A kernel started with launch_pdl may begin while the kernel
 // before it on the stream is still running; pdl_wait() inside it returns once that kernel has

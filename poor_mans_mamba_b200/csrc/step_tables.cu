@@ -193,16 +193,10 @@ PMM_EXPORT int pmm_step_tables(const int* held, const int* fresh, const int* blo
       (parents == nullptr) != (masks == nullptr) || (parents && (words < 1 || words > 4)))
     return PMM_ERR_BAD_ARGUMENT;
   // Every request reads the lengths of those in front of it, and its own parents, while others write.
-  struct Span {
-    const void* at;
-    long long bytes;
-  };
-  const Span written[] = {{cu, 4ll * (n + 1)}, {blocks_out, 4ll * n}, {taken, 4}, {table, 4ll * n * width}, {seq_of, 4ll * cap}, {positions, 4ll * cap},
+  const pmm::Extent written[] = {{cu, 4ll * (n + 1)}, {blocks_out, 4ll * n}, {taken, 4}, {table, 4ll * n * width}, {seq_of, 4ll * cap}, {positions, 4ll * cap},
                           {slots, 4ll * cap}, {masks, 8ll * cap * words}};
-  const Span read[] = {{held, 4ll * n}, {fresh, 4ll * n}, {blocks, 4ll * n}, {parents, 4ll * cap}};
-  for (const Span& w : written)
-    for (const Span& r : read)
-      if (pmm::overlap(w.at, w.bytes, r.at, r.bytes)) return PMM_ERR_OVERLAP;
+  const pmm::Extent read[] = {{held, 4ll * n}, {fresh, 4ll * n}, {blocks, 4ll * n}, {parents, 4ll * cap}};
+  if (pmm::overlap(written, read)) return PMM_ERR_OVERLAP;
   for (int i = 0; i < 4; ++i)
     if (pmm::overlap(written[i].at, written[i].bytes, free_pages, 4ll * n_free)) return PMM_ERR_OVERLAP;
   pmm::StepTablesArgs a{held, fresh, blocks, table, width, free_pages, n_free, n, page_size, spare, cu, seq_of, positions, slots, cap, blocks_out,

@@ -740,6 +740,18 @@ PMM_EXPORT int pmm_verify_drafts(const float* logits, long long ld, const float*
   if (V <= 0 || sms < 1 || chunks > pmm::kVfChunksMax || n_rows < 0 || static_cast<long long>(n_rows) * chunks > 0x3fffffffll || width <= 0 || !scratch || reinterpret_cast<uintptr_t>(scratch) % 16 ||
       (draft && parents) || n > 0x7fffffff / pmm::kVfCluster)
     return PMM_ERR_BAD_ARGUMENT;
+  // Requests are read and written side by side.
+  const long long out_bytes = 4ll * n * width, rows_bytes = 4ll * n_rows;
+  const pmm::Extent written[] = {{tokens_out, out_bytes}, {path, out_bytes}, {count, 4ll * n}, {scratch, pmm_verify_scratch(n_rows, V)}};
+  const pmm::Extent read[] = {{tokens, rows_bytes}, {parents, rows_bytes}, {uniforms, rows_bytes}, {cu, 4ll * (n + 1)}, {temperature, 4ll * n}};
+  if (pmm::overlap(written, read)) return PMM_ERR_OVERLAP;
+  for (int i = 0; i < 4; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (pmm::overlap(written[i].at, written[i].bytes, written[j].at, written[j].bytes)) return PMM_ERR_OVERLAP;
+    if (pmm::rows_overlap(logits, n_rows, 4 * ld, 4ll * V, written[i].at, written[i].bytes) ||
+        pmm::rows_overlap(draft, n_rows, 4 * ld_draft, 4ll * V, written[i].at, written[i].bytes))
+      return PMM_ERR_OVERLAP;
+  }
   pmm::VerifyArgs a{};
   a.logits = logits;
   a.ld = ld;

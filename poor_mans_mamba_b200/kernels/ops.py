@@ -2514,7 +2514,8 @@ def verify_drafts(logits: Tensor, tokens: Tensor, cu_seqlens: Tensor, uniforms: 
     holds it.  A draw takes the first index whose running sum passes u times the whole, in 64 bits; ties go to the lowest index.
     Written per request: ``count`` [n] (1 + kept drafts; 0 for a request without tokens), ``tokens_out`` [n, width] the kept
     tokens and the next one, ``path`` [n, width] the root and the kept tokens' places among the request's, both -1 behind
-    them.  Drafts deeper than the outputs are wide are not looked at.
+    them.  Drafts deeper than the outputs are wide are not looked at.  None of the three lies in what is read or in another
+    of them (requests are read and written side by side).
     NaN logits count as -inf.  A row that holds nothing else keeps no draft and gives token 0.  Positive temperatures
     outside 1e-36..1e36 count as the nearer of the two."""
     what = "verify_drafts"
@@ -2541,8 +2542,6 @@ def verify_drafts(logits: Tensor, tokens: Tensor, cu_seqlens: Tensor, uniforms: 
         raise KernelError(f"{what}: temperature must be contiguous float32 [{n}]")
     if not (path.dim() == 2 and path.shape[0] == n and path.shape[1] > 0 and tokens_out.shape == path.shape):
         raise KernelError(f"{what}: tokens_out and path must be int32 [requests, width]")
-    if tokens_out.data_ptr() in (tokens.data_ptr(), path.data_ptr()) or path.data_ptr() == tokens.data_ptr():
-        raise KernelError(f"{what}: tokens, tokens_out and path must be three (requests read and write side by side)")
     if not (scratch.is_contiguous() and scratch.data_ptr() % 16 == 0
             and scratch.numel() * scratch.element_size() >= _sized("pmm_verify_scratch", T, V)):
         raise KernelError(f"{what}: scratch comes from verify_drafts_scratch for as many rows")

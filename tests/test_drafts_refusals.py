@@ -132,3 +132,22 @@ def test_step_tables_refuses_outputs_in_its_inputs():
                 assert overlaps("pmm_step_tables", apart, **{out: apart[name] + at}) == bad, (out, name, at)
     assert overlaps("pmm_step_tables", apart, cu=apart["blocks"] - 8) and not overlaps("pmm_step_tables", apart, cu=apart["blocks"] - 12)
     assert overlaps("pmm_step_tables", apart, table=apart["free"] - 60) and not overlaps("pmm_step_tables", apart, table=apart["free"] - 64)
+
+
+def test_verify_drafts_refuses_outputs_in_its_inputs():
+    """Two requests of four tokens over 100 entries, outputs four wide."""
+    names = ["logits", "tokens", "cu", "uniforms", "temperature", "scratch", "tokens_out", "path", "count"]
+    apart = dict(VERIFY, **{k: A + 8192 * i for i, k in enumerate(names)})
+    assert not overlaps("pmm_verify_drafts", apart)
+    size = dict(tokens=16, cu=12, uniforms=16, temperature=8, scratch=4 * 2 * 16 + 16, tokens_out=32, path=32, count=8)
+    for out in ("tokens_out", "path", "count"):
+        for name, bytes_of in size.items():
+            if name != out:
+                for at, bad in ((0, True), (bytes_of - 4, True), (bytes_of, False)):
+                    assert overlaps("pmm_verify_drafts", apart, **{out: apart[name] + at}) == bad, (out, name, at)
+    # rows of 100 entries, 150 apart: between them there is room
+    for rows in (dict(logits=A, ld=150), dict(draft=A + 8192 * 20, ld_draft=150)):
+        base = rows.get("draft", A)
+        for at, bad in ((0, True), (396, True), (400, False), (600 - 32, False), (600 - 28, True), (3 * 600 + 399, True), (3 * 600 + 400, False)):
+            assert overlaps("pmm_verify_drafts", apart, **rows, path=base + at) == bad, at
+    assert overlaps("pmm_verify_drafts", apart, **{"parents": apart["path"]})
