@@ -6,7 +6,7 @@
 //
 // Float arithmetic on the CUDA cores, any storage type and head size, in two kernels: up to a head size of 256 blocks of rows (a row: a
 // token and a query head of the group) that share what they read of the keys, beyond it a block per token and query head.
-#include "common.cuh"
+#include "tree_attention.cuh"
 #include <math_constants.h>
 
 #include <type_traits>
@@ -551,6 +551,7 @@ PMM_EXPORT int pmm_tree_attention(const void* q, long long ldq, const void* k, l
   if (Dh <= 0 || Dh % 16 || Dh > 512 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq > 65535 || page_size <= 0 || sms < 1 || max_blocks <= 0 || pages <= 0 || !(scale > 0.f) ||
       (window != 0 && !positions) || (mask && words < 1))
     return PMM_ERR_BAD_ARGUMENT;
+  if (pmm::tree_attention_overlap(q, ldq, k, ldk, v, ldv, pool, pages, out, page_size, T, Hq, Hkv, Dh, dtype == 0 ? 4 : 2)) return PMM_ERR_OVERLAP;
   PMM_DISPATCH_DTYPE(dtype, S, {
     pmm::TreeAttnArgs<S> a{static_cast<const S*>(q), ldq, static_cast<const S*>(k), ldk, static_cast<const S*>(v), ldv, static_cast<const S*>(pool),
                            block_table, max_blocks, pages, held, cu, positions, static_cast<const unsigned long long*>(mask), words, sink,

@@ -26,6 +26,7 @@
 // by hand to the rows that see them.
 // Every mbarrier wait is bounded (status codes 41..45, see attention_tc.cu).  No cluster multicast.
 #include "attention_tc.cuh"
+#include "tree_attention.cuh"
 #include <math_constants.h>
 
 #include <type_traits>
@@ -1040,6 +1041,7 @@ PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k
     ldk = ldv = kv_dim;
   }
   if (ldq % 8 || ldk % 8 || ldv % 8) return PMM_ERR_BAD_ARGUMENT;
+  if (pmm::tree_attention_overlap(q, ldq, k, ldk, v, ldv, pool, pages, out, page_size, T, Hq, Hkv, Dh, 2)) return PMM_ERR_OVERLAP;
   pmm::EncodeTiledFn fn = pmm::encode_tiled_fn();
   if (!fn) return PMM_ERR_BAD_ARGUMENT;
   const int box = page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : page_size % 16 == 0 ? 16 : 8;

@@ -2448,7 +2448,8 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: T
     cache holds them (`qkv_rope_store` without a pool leaves them so); they are not in the cache yet.  ``q``, ``k``, ``v`` may
     be column slices of wider rows.  ``window`` limits the cached keys as in `paged_attention`, counted from ``positions`` [T];
     among the step's tokens the mask alone decides.  ``sink``: see `paged_attention`.
-    A row that sees no key is zero; rows behind the last request (cu_seqlens[n] and further) are left as they are."""
+    A row that sees no key is zero; rows behind the last request (cu_seqlens[n] and further) are left as they are.  ``out`` may
+    be ``q`` itself, where that is contiguous; no other part of it lies in what is read."""
     what = "tree_attention"
     stream = _launch_stream(what, q, k, v, pool, block_table, held, cu_seqlens, out, scratch, mask, positions, sink)
     check_head_dim(head_dim, FLOAT_ATTENTION_MAX_HEAD)

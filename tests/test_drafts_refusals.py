@@ -151,3 +151,27 @@ def test_verify_drafts_refuses_outputs_in_its_inputs():
         for at, bad in ((0, True), (396, True), (400, False), (600 - 32, False), (600 - 28, True), (3 * 600 + 399, True), (3 * 600 + 400, False)):
             assert overlaps("pmm_verify_drafts", apart, **rows, path=base + at) == bad, at
     assert overlaps("pmm_verify_drafts", apart, **{"parents": apart["path"]})
+
+
+TREE = dict(q=A, ldq=512, k=A, ldk=128, v=A, ldv=128, pool=A, pages=4, block_table=A, max_blocks=2, held=A, cu=A, positions=None, mask=None, words=0,
+            sink=None, out=A, scale=0.125, window=0, page_size=64, n_seq=2, T=6, Hq=8, Hkv=2, Dh=64)
+
+
+@pytest.mark.parametrize("name,elem,last", [("pmm_tree_attention", 4, dict(dtype=0, sms=148, stream=None)), ("pmm_tree_attention", 2, dict(dtype=1, sms=148, stream=None)),
+                                            ("pmm_tree_attention_tc", 2, dict(wide=0, scratch=A, sms=148, status=A, stream=None))])
+def test_tree_attention_refuses_outputs_in_its_inputs(name, elem, last):
+    """Six rows of 512 values beside keys and values of 128."""
+    M = 1 << 24
+    apart = {**TREE, **last, "q": M, "k": 2 * M, "v": 3 * M, "pool": 4 * M, "out": 5 * M}
+    if "scratch" in last:
+        apart["scratch"] = 6 * M
+    assert not overlaps(name, apart)
+    row, kv = 512 * elem, 128 * elem
+    for at, bad in ((4 * M, True), (4 * M + 4 * 2 * 64 * kv - 16, True), (4 * M + 4 * 2 * 64 * kv, False), (4 * M - 6 * row + 16, True), (4 * M - 6 * row, False),
+                    (2 * M + 6 * kv - 16, True), (2 * M + 6 * kv, False), (3 * M, True), (M, False), (M + row, True), (M - 16, True), (M + 6 * row, False)):
+        assert overlaps(name, apart, out=at) == bad, (at / M, at % M)
+    # q a slice of rows twice as wide: not in place
+    assert overlaps(name, apart, ldq=1024, out=M) and not overlaps(name, apart, ldq=1024, out=M, T=1)
+    # one row: its neighbours in the same row are free
+    assert not overlaps(name, apart, T=1, q=M, ldq=4096, k=M + row, ldk=4096, v=M + row + kv, ldv=4096, out=M + row + 2 * kv)
+    assert overlaps(name, apart, T=1, q=M, ldq=4096, k=M + row, ldk=4096, v=M + row + kv, ldv=4096, out=M + row + kv)

@@ -187,3 +187,16 @@ def test_tree_attention_of_one_row_of_any_stride(dtype, heads):
         assert getattr(c, name).stride(0) % 2 == 1
     c.run()
     c.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (64, 8, 128), (2, 1, 256), (2, 1, 512)])
+def test_tree_attention_in_the_place_of_the_queries(dtype, heads):
+    """Results written over q: units of one block, units that shares cut, wide ones."""
+    for held, new in (([3000, 40], [33, 9]), ([20] * 300, [5] * 300), ([0], [1])):
+        c = Case(held, new, heads, dtype, 64, seed=17)
+        first = c.q.clone()
+        c.out = c.q
+        c.run()
+        c.q = first
+        c.check()
