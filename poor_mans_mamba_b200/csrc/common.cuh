@@ -159,6 +159,14 @@ inline bool overlap(const Extent (&a)[N], const Extent (&b)[M]) {
 // pdl_launch_dependents() lets the next kernel of the stream start its own preamble early.
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// The other way round, for a kernel that writes what later launches read ahead of their wait (tables, tokens, cached rows) and therefore
+// never calls pdl_launch_dependents(): the launch behind it begins once all of its blocks have ended, which alone does not say that what
+// they wrote has arrived.  The whole block calls this behind its last stores (one thread's fence stands for all that the barrier has put in
+// front of it; one for every thread costs a copy of 23 MB 1.7 us).
+__device__ __forceinline__ void pdl_arrived() {
+  __syncthreads();
+  if (threadIdx.x == 0) __threadfence();
+}
 // In a kernel with code before its wait: what is read through a `const T* __restrict__` parameter counts as never written, so
 // the compiler may move such a load above pdl_wait().  Called behind the wait for every such parameter that earlier
 // launches write, this makes the pointer a value that is only known there.

@@ -12,7 +12,7 @@
 // A copy: a block per (some layers and planes, request), a warp a row, up to eight pieces of a lane asked for before the first is stored.
 //
 // What these kernels write, later launches read ahead of their wait (sequence bounds, tables, cached keys): neither lets the
-// launch behind it begin early.
+// launch behind it begin early, and both wait for their stores (pdl_arrived).
 #include "common.cuh"
 
 namespace pmm {
@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(const StepT
     }
     a.positions[t] = saturated(static_cast<long long>(held) + depth);
   }
+  pdl_arrived();
 }
 
 constexpr int kKeepThreads = 256;
@@ -180,6 +181,7 @@ __global__ void __launch_bounds__(kKeepThreads)
           if (r[k].src != nullptr && base + 32 * u < width) r[k].dst[base + 32 * u] = v[k][u];
     }
   }
+  pdl_arrived();
 }
 
 }  // namespace pmm

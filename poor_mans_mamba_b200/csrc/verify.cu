@@ -404,6 +404,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_walk_kernel(const Verify
     if (rank == 0) {
       for (int j = tid; j < a.width; j += kVfThreads) out[j] = path[j] = -1;
       if (tid == 0) a.count[s] = 0;
+      pdl_arrived();
     }
     return;
   }
@@ -458,6 +459,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_walk_kernel(const Verify
     }
     for (int j = kept + 1 + lane; j < a.width; j += 32) out[j] = path[j] = -1;
     if (lane == 0) a.count[s] = kept + 1;
+    __threadfence();  // (as pdl_arrived: all that is left of the block is this warp)
     return;
   }
 
@@ -722,6 +724,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_walk_kernel(const Verify
     path[j] = j <= kept ? j : -1;
   }
   if (tid == 0) a.count[s] = kept + 1;
+  pdl_arrived();
 }
 
 }  // namespace pmm

@@ -200,3 +200,42 @@ def test_tree_attention_in_the_place_of_the_queries(dtype, heads):
         c.run()
         c.q = first
         c.check()
+
+
+# ----------------------------------------------------------------------------- launches directly behind
+def test_launches_directly_behind_find_tables_and_kept_rows():
+    """Attention of a decode step reads positions, block tables and cached keys ahead of its wait for the launch before it: directly behind
+    the tables' launch, and behind the kept rows', it reads what those have written."""
+    ops, n, page, hq, hkv, d, P_ = K(), 64, 64, 8, 2, 64, 600
+    g = torch.Generator(device=DEV).manual_seed(1)
+    bf = dict(dtype=torch.bfloat16, device=DEV)
+    pool = torch.randn(1, P_ + 1, 2, page, hkv * d, generator=g, **bf)
+    q, k, v = torch.randn(n, hq * d, generator=g, **bf), torch.randn(n, hkv * d, generator=g, **bf), torch.randn(n, hkv * d, generator=g, **bf)
+    one, free = i32([1] * n), torch.randperm(P_, device=DEV, generator=g).int()
+    cu, seq, pos, slots, blocks, taken = i32([0] * (n + 1)), i32([0] * n), i32([0] * n), i32([0] * n), i32([0] * n), i32([0])
+    table, zero = i32([[P_] * 9] * n), i32([0] * n)
+
+    def attend(to):
+        ops.flash_decode_attention(q, k, v, 1.0, 1.0, 1.0, None, pool[0], table, pos, to, hq, hkv, d, d ** -0.5)
+
+    for i in range(60):
+        held = torch.randint(0, 8 * page, (n,), generator=g, device=DEV, dtype=torch.int32)
+        free = free[torch.randperm(P_, generator=g, device=DEV)]
+        got, again = (torch.zeros(n, hq * d, **bf) for _ in range(2))
+        torch.cuda.synchronize()
+        ops.step_tables(held, one, zero, table, free, page, P_, cu, seq, pos, slots, blocks, taken)
+        attend(got)
+        torch.cuda.synchronize()
+        assert torch.equal(pos, held)
+        attend(again)
+        assert torch.equal(got, again), i
+        # kept rows: a token of every request, into places that the step behind them reads
+        rows = torch.randn(1, 2, n, hkv * d, generator=g, **bf)
+        place = (table[torch.arange(n, device=DEV), 0] * page + held.clamp_max(page - 1) // 2).int()
+        path, count = i32([[0]] * n), one
+        torch.cuda.synchronize()
+        ops.keep_accepted(rows, pool, place, cu, path, count)
+        attend(got)
+        torch.cuda.synchronize()
+        attend(again)
+        assert torch.equal(got, again), i
