@@ -1,6 +1,6 @@
 // Attention of drafted tokens over a paged cache: token i of request s sees the request's held[s] cached keys (the last
 // `window` positions up to its own, where there is a window) and, among the request's own tokens of this step, those whose
-// bits its mask holds (without masks: those in front of it, and itself).
+// bits its mask holds (without masks: those in front of it, and itself), with `window_step` only as far as the window reaches.
 //   sc[j] = (q.K[j]) * scale;  p = exp(sc - max);  o = sum p V / sum p,   0 for a row that sees no key
 // The step's own keys and values lie densely in k and v: the cache takes only those that are kept in the end.
 //
@@ -35,7 +35,9 @@ struct TreeAttnArgs {
   const float* sink;               // [Hq] or nullptr
   S* out;
   float scale;
-  int window, page_size, n_seq, Hq, Hkv, Dh;
+  int window;
+  int window_step;                 // the window limits the step's own tokens too, by their positions
+  int page_size, n_seq, Hq, Hkv, Dh;
 };
 
 __device__ __forceinline__ float ta_dot(const float* qw, const float* kr, int Dh) {
@@ -74,7 +76,7 @@ __device__ __forceinline__ bool ta_sees(const unsigned long long* mask, int word
 // Head sizes beyond 256.  A block per (token, query head); its eight warps share the keys in pieces of 32 (a key per lane for the scores, a
 // slice of the head per lane for the values) and merge their maxima, sums and results at the end.
 template <typename S, int ACC>
-__global__ void __launch_bounds__(kTaWarps * 32) tree_attention_kernel(const TreeAttnArgs<S> a, int T) {
+__global__ void __launch_bounds__(kTaWarps * 32, 3) tree_attention_kernel(const TreeAttnArgs<S> a, int T) {
   extern __shared__ float qs[];  // the query, then every warp's result
   __shared__ float s_m[kTaWarps], s_l[kTaWarps];
   pdl_launch_dependents();
@@ -108,7 +110,7 @@ __global__ void __launch_bounds__(kTaWarps * 32) tree_attention_kernel(const Tre
     const int begin = part == 0 ? lo : 0, end = part == 0 ? held : n_new;
     for (int base = begin + warp * 32; base < end; base += kTaWarps * 32) {
       const int j = base + lane;
-      const bool valid = j < end && (part == 0 || (mask ? ta_sees(mask, a.words, j) : j <= t - t0));
+      const bool valid = j < end && (part == 0 || ((mask ? ta_sees(mask, a.words, j) : j <= t - t0) && (!a.window_step || a.positions[t0 + j] >= lo)));
       const S *kr = nullptr, *vr = nullptr;
       float sc = -CUDART_INF_F;
       if (valid) {
@@ -368,6 +370,9 @@ __global__ void __launch_bounds__(kTfThreads, ACC <= 4 ? 2 : 1) tree_rows_kernel
     const bool own = j >= ctx_tiles;
     const int base = (own ? (j - ctx_tiles) * kTfKeys : first + j * kTfKeys) + 32 * half;
     const int n_keys = min(32, (own ? n_new : held) - base);  // of this warp's half
+    const int key = base + lane;
+    // what a window is compared with: the place of a cached key, the position of one of the step's, or none where the mask alone decides
+    const int at = !own ? key : a.window_step && lane < n_keys ? a.positions[t0 + key] : 0x7fffffff;
     asm volatile("cp.async.wait_all;\n" ::: "memory");
     __syncthreads();
     // N of the warp's rows, or more than it has: the last one again, whose results nobody reads (a question per row and step costs
@@ -386,8 +391,9 @@ __global__ void __launch_bounds__(kTfThreads, ACC <= 4 ? 2 : 1) tree_rows_kernel
       bool all = true;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int r = wr + 4 * min(i, mine - 1), tok = s_tok[r], key = base + lane;
-        const bool see = lane < n_keys && (!own ? key >= s_lo[r] : a.mask ? ta_sees(a.mask + static_cast<size_t>(t0 + tok) * a.words, a.words, key) : key <= tok);
+        const int r = wr + 4 * min(i, mine - 1), tok = s_tok[r];
+        const bool see = lane < n_keys && at >= s_lo[r] &&
+                         (!own || (a.mask ? ta_sees(a.mask + static_cast<size_t>(t0 + tok) * a.words, a.words, key) : key <= tok));
         sees[i] = __ballot_sync(0xffffffffu, see);
         all = all && sees[i] == 0xffffffffu;
         const float sc = see ? s[i] * a.scale : -CUDART_INF_F;
@@ -545,8 +551,8 @@ int launch_tree_rows(const TreeAttnArgs<S>& a, int T, int sms, cudaStream_t stre
 // Hq*Dh].  Rows behind the last request (cu[n_seq] and further) are left as they are.
 PMM_EXPORT int pmm_tree_attention(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* pool, int pages,
                                   const int* block_table, int max_blocks, const int* held, const int* cu, const int* positions, const void* mask,
-                                  int words, const float* sink, void* out, float scale, int window, int page_size, int n_seq, int T, int Hq,
-                                  int Hkv, int Dh, int dtype, int sms, cudaStream_t stream) {
+                                  int words, const float* sink, void* out, float scale, int window, int window_step, int page_size, int n_seq, int T,
+                                  int Hq, int Hkv, int Dh, int dtype, int sms, cudaStream_t stream) {
   if (T <= 0 || n_seq <= 0) return 0;
   if (Dh <= 0 || Dh % 16 || Dh > 512 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq > 65535 || page_size <= 0 || sms < 1 || max_blocks <= 0 || pages <= 0 || !(scale > 0.f) ||
       (window != 0 && !positions) || (mask && words < 1))
@@ -555,7 +561,7 @@ PMM_EXPORT int pmm_tree_attention(const void* q, long long ldq, const void* k, l
   PMM_DISPATCH_DTYPE(dtype, S, {
     pmm::TreeAttnArgs<S> a{static_cast<const S*>(q), ldq, static_cast<const S*>(k), ldk, static_cast<const S*>(v), ldv, static_cast<const S*>(pool),
                            block_table, max_blocks, pages, held, cu, positions, static_cast<const unsigned long long*>(mask), words, sink,
-                           static_cast<S*>(out), scale, window, page_size, n_seq, Hq, Hkv, Dh};
+                           static_cast<S*>(out), scale, window, window != 0 && window_step, page_size, n_seq, Hq, Hkv, Dh};
     if (Dh <= 64) return pmm::launch_tree_rows<S, 2>(a, T, sms, stream);
     if (Dh <= 128) return pmm::launch_tree_rows<S, 4>(a, T, sms, stream);
     if (Dh <= 256) return pmm::launch_tree_rows<S, 8>(a, T, sms, stream);

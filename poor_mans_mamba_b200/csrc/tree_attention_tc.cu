@@ -135,7 +135,9 @@ struct TreeTcArgs {
   float2* part_ml;      // [2 * blocks][rows]
   int* cuts;            // [blocks][8]: a unit that shares cut: its rows (0: none), first token, head, row tile, last block
   float scale_log2;
-  int window, page_size, box, n_seq, T, Hq, Hkv, shares;
+  int window;
+  int window_step;      // the window limits the step's own tokens too, by their positions
+  int page_size, box, n_seq, T, Hq, Hkv, shares;
   int rows;             // of a unit: 128 or 256
   int* status;
 };
@@ -734,24 +736,28 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
         // Half h of the scores to probabilities; masked: some rows may not see some of the keys.
         auto half = [&](int h, auto masked) {
           const unsigned here = s_tmem + kTtHalf * h;
-          unsigned v[kTtHalf];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) tmem_ld32(here + 32 * c, v + 32 * c);
-          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+          unsigned long long w = 0ull;  // the bits of the row's visible keys among these 64
           if (decltype(masked)::value) {
-            // the bits of the row's visible keys among these 64
             const int left = valid - kTtHalf * h;
-            unsigned long long w = left >= 64 ? ~0ull : (1ull << left) - 1ull;
+            w = left >= 64 ? ~0ull : (1ull << left) - 1ull;
             if (own) {  // of its mask, or up to the token itself
               const int k0 = (j - g.s.ctx_tiles) * kAtKeys + kTtHalf * h, upto = my_tok + 1 - k0;
               if (a.mask)
                 w &= k0 / 64 < a.words ? a.mask[static_cast<size_t>(g.s.t0 + my_tok) * a.words + k0 / 64] : 0ull;
               else
                 w &= upto <= 0 ? 0ull : upto >= 64 ? ~0ull : (1ull << upto) - 1ull;
+              if (a.window_step)  // (a place is one token for the whole warp)
+                for (int i = 0; i < min(left, 64); ++i) w &= ~(static_cast<unsigned long long>(a.positions[g.s.t0 + k0 + i] < my_lo) << i);
             } else {
               const int skip = my_lo - (base + kTtHalf * h);
               w &= skip <= 0 ? ~0ull : skip >= 64 ? 0ull : ~0ull << skip;
             }
+          }
+          unsigned v[kTtHalf];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) tmem_ld32(here + 32 * c, v + 32 * c);
+          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+          if (decltype(masked)::value) {
 #pragma unroll
             for (int i = 0; i < kTtHalf; ++i)
               if (!(static_cast<unsigned>(w >> (i & 32)) >> (i & 31) & 1u)) v[i] = __float_as_uint(-CUDART_INF_F);
@@ -907,6 +913,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
                   vr = a.v + (now.s.t0 + node) * a.ldv + now.hk * DH;
                   see = a.mask ? node < 64 * a.words && (a.mask[static_cast<size_t>(now.s.t0 + my_tok) * a.words + (node >> 6)] >> (node & 63) & 1ull)
                                : node <= my_tok;
+                  see = see && (!a.window_step || a.positions[now.s.t0 + node] >= my_lo);
                 } else {
                   const int page = min(max(a.block_table[static_cast<size_t>(now.seq) * a.max_blocks + key / a.page_size], 0), a.pages - 1);
                   vr = a.pool + ((static_cast<long long>(page) * 2 + 1) * a.page_size + key % a.page_size) * a.Hkv * DH + now.hk * DH;
@@ -1027,8 +1034,8 @@ PMM_EXPORT long long pmm_tree_attention_scratch(int sms) { return static_cast<lo
 
 PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* pool,
                                      int pages, const int* block_table, int max_blocks, const int* held, const int* cu, const int* positions,
-                                     const void* mask, int words, const float* sink, void* out, float scale, int window, int page_size, int n_seq,
-                                     int T, int Hq, int Hkv, int Dh, int wide, float* scratch, int sms, int* status, cudaStream_t stream) {
+                                     const void* mask, int words, const float* sink, void* out, float scale, int window, int window_step, int page_size,
+                                     int n_seq, int T, int Hq, int Hkv, int Dh, int wide, float* scratch, int sms, int* status, cudaStream_t stream) {
   if (T <= 0 || n_seq <= 0) return 0;
   if (!tree_tc_supported(Hq, Hkv, Dh, page_size, pages, n_seq) || max_blocks <= 0 || !(scale > 0.f) || (window != 0 && !positions) ||
       (mask && words < 1) || !scratch || sms < 1 || !status)
@@ -1082,6 +1089,7 @@ PMM_EXPORT int pmm_tree_attention_tc(const void* q, long long ldq, const void* k
   a.cuts = reinterpret_cast<int*>(scratch + static_cast<size_t>(a.shares) * 2 * a.rows * (Dh + 2));
   a.scale_log2 = scale * 1.4426950408889634f;
   a.window = window;
+  a.window_step = window != 0 && window_step;
   a.page_size = page_size;
   a.box = box;
   a.n_seq = n_seq;

@@ -188,11 +188,11 @@ _SIGNATURES = {
                           c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p],
     "pmm_tree_attention": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p,
                            c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
-                           c_int, c_int, c_int, c_int, c_void_p],
+                           c_int, c_int, c_int, c_int, c_int, c_void_p],
     "pmm_tree_attention_scratch": [c_int],
     "pmm_tree_attention_tc": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p,
                               c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int, c_int,
-                              c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
+                              c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
     "pmm_verify_scratch": [c_longlong, c_int],
     "pmm_verify_drafts": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
                           c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p],
@@ -2441,13 +2441,15 @@ def _aligned_rows(what: str, name: str, t: Tensor, rows: int, width: int) -> int
 def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: Tensor, held: Tensor, cu_seqlens: Tensor, out: Tensor,
                    n_q_heads: int, n_kv_heads: int, head_dim: int, softmax_scale: float, scratch: Tensor,
                    mask: Optional[Tensor] = None, positions: Optional[Tensor] = None, window: int = 0,
-                   sink: Optional[Tensor] = None) -> None:
+                   sink: Optional[Tensor] = None, window_step: bool = False) -> None:
     """Attention of a step's drafted tokens: token t of request s (``cu_seqlens`` int32 [n + 1]) over the request's ``held``
     [n] cached keys and, of the request's own tokens in this step, those whose bits ``mask`` [T, words] holds (`step_tables`;
     None: those in front of it and itself).  ``k``/``v`` [T, Hkv*Dh] are the step's keys and values, rotated and scaled as the
     cache holds them (`qkv_rope_store` without a pool leaves them so); they are not in the cache yet.  ``q``, ``k``, ``v`` may
     be column slices of wider rows.  ``window`` limits the cached keys as in `paged_attention`, counted from ``positions`` [T];
-    among the step's tokens the mask alone decides.  ``sink``: see `paged_attention`.
+    among the step's tokens the mask alone decides.  With ``window_step`` the window limits those too, each by its position: what
+    `paged_attention` has in steps of one token, so a layer with a window (or with chunks, ``window`` below zero) wants it;
+    without, the tokens that a window or a chunk's border hides have to be out of the mask.  ``sink``: see `paged_attention`.
     A row that sees no key is zero; rows behind the last request (cu_seqlens[n] and further) are left as they are.  ``out`` may
     be ``q`` itself, where that is contiguous; no other part of it lies in what is read."""
     what = "tree_attention"
@@ -2486,7 +2488,7 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: T
         raise KernelError(f"{what}: scratch comes from tree_attention_scratch")
     pages, page_size = pool_shape[0], pool_shape[2]
     args = (q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, pool.data_ptr(), pages, block_table.data_ptr(), block_table.shape[1],
-            held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words, _ptr(sink), out.data_ptr(), softmax_scale, window,
+            held.data_ptr(), cu_seqlens.data_ptr(), _ptr(positions), _ptr(mask), words, _ptr(sink), out.data_ptr(), softmax_scale, window, window_step,
             page_size, n_seq, T, n_q_heads, n_kv_heads, head_dim)
     # (the rule of pmm_tree_attention_tc, which refuses what does not keep it)
     if (dtype is torch.bfloat16 and head_dim in (64, 128) and page_size % 8 == 0 and n_seq <= TREE_TC_MAX_SEQS

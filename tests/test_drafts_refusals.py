@@ -154,7 +154,7 @@ def test_verify_drafts_refuses_outputs_in_its_inputs():
 
 
 TREE = dict(q=A, ldq=512, k=A, ldk=128, v=A, ldv=128, pool=A, pages=4, block_table=A, max_blocks=2, held=A, cu=A, positions=None, mask=None, words=0,
-            sink=None, out=A, scale=0.125, window=0, page_size=64, n_seq=2, T=6, Hq=8, Hkv=2, Dh=64)
+            sink=None, out=A, scale=0.125, window=0, window_step=0, page_size=64, n_seq=2, T=6, Hq=8, Hkv=2, Dh=64)
 
 
 @pytest.mark.parametrize("name,elem,last", [("pmm_tree_attention", 4, dict(dtype=0, sms=148, stream=None)), ("pmm_tree_attention", 2, dict(dtype=1, sms=148, stream=None)),

@@ -239,3 +239,76 @@ def test_launches_directly_behind_find_tables_and_kept_rows():
         torch.cuda.synchronize()
         attend(again)
         assert torch.equal(got, again), i
+
+
+# ----------------------------------------------------------------------------- windows over the step's own tokens
+def windowed(c, window):
+    """Keeps the mask, and takes what `window` hides among the step's own tokens out of what the plain form sees."""
+    pos = c.positions.tolist()
+    for s, see in enumerate(c.see):
+        own = torch.tensor(pos[c.cu[s]:c.cu[s + 1]])
+        first = own - window + 1 if window > 0 else own - own % -window
+        see &= own[None, :] >= first[:, None]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (6, 2, 128), (16, 1, 128), (16, 1, 64), (2, 1, 256), (2, 1, 512)])
+@pytest.mark.parametrize("window", [1, 2, 5, 30, 200, -1, -8, -50, -64])
+@pytest.mark.parametrize("parents", ["tree", None])
+def test_tree_attention_window_over_the_step(dtype, heads, window, parents):
+    """Paths deeper than the window, chunks whose border lies among the step's tokens; hidden values that are not numbers harm nobody."""
+    c = Case([300, 62, 0, 130], [14, 9, 40, 61], heads, dtype, 64, seed=23, parents=parents, extra_rows=2)
+    sink = torch.randn(heads[0], generator=torch.Generator().manual_seed(2)).to(DEV)
+    windowed(c, window)
+    c.run(window, sink, window_step=True)
+    c.check(window, sink)
+    hidden = [(s, j) for s, see in enumerate(c.see) for j in range(see.shape[0]) if int(see[:, j].sum()) <= 1]
+    for s, j in hidden[::3]:   # (a token that sees itself alone may spoil its own row)
+        c.v[c.cu[s] + j, ::3] = math.inf
+    c.run(window, None, window_step=True)
+    c.check(window)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("window", [7, 64, 300, -16, -64])
+def test_tree_attention_window_over_long_chains(dtype, window):
+    c = Case([100, 0, 700], [300, 513, 1], (4, 2, 64), dtype, 64, parents=None, seed=3)
+    windowed(c, window)
+    c.run(window, window_step=True)
+    c.check(window)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("window", [3, 40, -8, -64])
+def test_tree_attention_with_a_window_is_paged_attention_along_every_path(dtype, window):
+    """Every node of a tree against the framework's attention of single tokens: the path down to it is put into the cache, and the
+    node's row attends over it there."""
+    hq, hkv, d, page = 8, 2, 64, 16
+    held, new = [57, 6], [12, 9]
+    c = Case(held, new, (hq, hkv, d), dtype, page, seed=41, extra_pages=12)
+    c.run(window, window_step=True)
+    for s, m in enumerate(new):
+        t0, h = c.cu[s], held[s]
+        depth = [int(x) - h for x in c.positions[t0:t0 + m]]
+        table = torch.full((1, 8), c.pages - 1, dtype=torch.int32, device=DEV)
+        used = -(-h // page)
+        table[0, :used] = c.table[s, :used]
+        spare = sorted(set(range(c.pages - 1)) - set(c.table[:, :].flatten().tolist()))
+        table[0, used:used + 2] = i32(spare[:2])
+        for i in range(m):
+            path = [i]
+            while c.parents[s][path[0]] >= 0:
+                path.insert(0, c.parents[s][path[0]])
+            assert len(path) == depth[i] + 1
+            pool = c.pool.clone()
+            for at, node in enumerate(path):
+                p = int(table[0, (h + at) // page])
+                pool[p, 0, (h + at) % page], pool[p, 1, (h + at) % page] = c.k[t0 + node], c.v[t0 + node]
+            one = torch.zeros(1, hq * d, dtype=dtype, device=DEV)
+            K().paged_attention(c.q[t0 + i:t0 + i + 1].contiguous(), pool, table, i32([h + depth[i]]), i32([0]), one, hq, hkv, d, c.scale, window=window)
+            got, want = c.out[t0 + i].double(), one[0].double()
+            # both are within their sums' errors of the formula (float32: some 100 terms, scores of size 4); bfloat16: the probabilities and
+            # the result are rounded to 2^-8 on one side, the result on both
+            size = c.v[t0:t0 + m].abs().max().double().clamp_min(4.0)
+            off = 3 * 2.0 ** -8 * size if dtype == torch.bfloat16 else 200 * 2.0 ** -24 * 4 * size
+            assert float((got - want).abs().max()) <= float(off), (s, i)
