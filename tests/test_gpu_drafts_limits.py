@@ -312,3 +312,88 @@ def test_tree_attention_with_a_window_is_paged_attention_along_every_path(dtype,
             size = c.v[t0:t0 + m].abs().max().double().clamp_min(4.0)
             off = 3 * 2.0 ** -8 * size if dtype == torch.bfloat16 else 200 * 2.0 ** -24 * 4 * size
             assert float((got - want).abs().max()) <= float(off), (s, i)
+
+
+# ----------------------------------------------------------------------------- units of 256 rows
+# 16 query heads a key/value head: 9 tokens fill the second set of 128 rows with 16, 20 leave a last unit whose second set has none.
+WIDE = [([333, 1500, 0, 70], [20, 9, 17, 40]), ([(37 * s) % 300 for s in range(90)], [(9, 20, 8, 16)[s % 4] for s in range(90)])]
+
+
+def wide(held, new, d, page=64, **kw):
+    c = Case(held, new, (16, 1, d), torch.bfloat16, page, **kw)
+    assert sum(new) * 16 > 128 * len(new)
+    return c
+
+
+def some(new):
+    """Of many requests every seventh is looked at."""
+    return set(range(0, len(new), 7)) if len(new) > 8 else None
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("held,new", WIDE)
+@pytest.mark.parametrize("window", [0, 5, 100, -64])
+def test_wide_units_windows_and_sinks(d, held, new, window):
+    c = wide(held, new, d, seed=51, extra_rows=3)
+    sink = torch.randn(16, generator=torch.Generator().manual_seed(4)).to(DEV)
+    for s in (None, sink):
+        c.run(window, s)
+        c.check(window, s, some(new))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("held,new", WIDE)
+@pytest.mark.parametrize("window", [0, 1])
+def test_wide_units_empty_rows_and_any_mask(d, held, new, window):
+    """(A window of 1 hides the whole cache: rows that see nothing at all.)"""
+    c = wide(held, new, d, seed=52)
+    g = torch.Generator().manual_seed(1)
+    for see in c.see:
+        see[:] = torch.rand(see.shape, generator=g) < 0.4
+        see[::3] = False
+        see[:, 2:4] = False
+    c.write_mask()
+    for s in (None, torch.randn(16, generator=g).to(DEV)):
+        c.run(window, s)
+        c.check(window, s, some(new))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("held,new", WIDE)
+@pytest.mark.parametrize("window", [0, 90])
+def test_wide_units_values_that_are_not_numbers(d, held, new, window):
+    """Both sets of rows take what is not finite out of the one tile of values that they share."""
+    c = wide(held, new, d, seed=53)
+    for s, m in enumerate(new):
+        t0 = c.cu[s]
+        if m > 8:
+            c.k[t0 + 3] = math.nan
+            c.v[t0 + 5, :3] = math.inf
+            c.v[t0 + 7, d // 2:] = -math.inf
+            c.v[t0 + m - 1, 1::2] = math.nan
+        if held[s] > 80:    # a cached value and a cached key
+            for place, plane, row in ((70, 1, slice(4, 6)), (held[s] - 2, 0, slice(0, d))):
+                c.pool[int(c.table[s, place // 64]), plane, place % 64, row] = math.inf if plane else math.nan
+                c.ctx[s][plane, place, row] = math.inf if plane else math.nan
+    c.q[c.cu[1] + 4, :d] = math.nan
+    c.run(window)
+    c.check(window, only=some(new))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("page", [8, 24, 48, 200, 256])
+@pytest.mark.parametrize("window", [0, 70])
+def test_wide_units_page_sizes(d, page, window):
+    for held, new in (WIDE[0], ([301, 64, 17], [33, 16, 5])):
+        c = wide(held, new, d, page, seed=page, extra_pages=2)
+        c.run(window)
+        c.check(window)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_wide_units_of_as_many_requests_as_there_may_be(d):
+    """1,024 requests: the most whose lengths lie in shared memory beside the tiles."""
+    n = 1024
+    c = wide([s % 7 for s in range(n)], [10 - s % 2 for s in range(n)], d, 8, seed=6)
+    c.run()
+    c.check(only=set(range(0, n, 60)))
