@@ -1,6 +1,7 @@
 """The operators of a drafted step at the ends of what they take: temperatures, scores and lengths of every size, tensors that lie in one
 another, bounds beyond the step; against the plain forms in 64 bits."""
 import math
+import random
 
 import pytest
 import torch
@@ -397,3 +398,128 @@ def test_wide_units_of_as_many_requests_as_there_may_be(d):
     c = wide([s % 7 for s in range(n)], [10 - s % 2 for s in range(n)], d, 8, seed=6)
     c.run()
     c.check(only=set(range(0, n, 60)))
+
+
+# ----------------------------------------------------------------------------- the operators together
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("window", [0, 3, 20, -8])
+def test_drafted_steps_row_by_row(dtype, tree, window):
+    """A layer of attention whose tokens come from 16 columns of its rows, greedy: drafted steps against one token a step through the
+    framework's paged attention.  Every kept node's attention row is the single step's within both sides' roundings, and every token is
+    the single step's wherever its two best logits are further apart than those roundings can move them."""
+    hq, hkv, d, V, page, n, total = 4, 2, 64, 97, 16, 3, 30
+    ops, w, rng = K(), hkv * d, random.Random(3)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    E = torch.randn(V, 64, generator=g, device=DEV, dtype=torch.float64)
+    W = torch.randn(64, (hq + 2 * hkv) * d, generator=g, device=DEV, dtype=torch.float64) / 8
+    columns = torch.randperm(hq * d, generator=g, device=DEV)[:16]
+    R = torch.randn(16, V, generator=g, device=DEV, dtype=torch.float64)
+    inv = (1e4 ** (-torch.arange(0, d, 2) / d)).to(DEV)
+    prompts = [[rng.randrange(V) for _ in range(m)] for m in (5, 30, 17)]
+    rows_of = (E @ W).to(dtype)                                      # a token's q, k and v, the same whoever asks
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+    # (a rotation keeps a row's length up to its rounding; |q||k| bounds a score's sum of magnitudes)
+    norm = lambda x: float(x.double().view(V, -1, d).norm(dim=-1).max()) * 1.02
+    size = norm(rows_of[:, :hq * d]) * norm(rows_of[:, hq * d:hq * d + w]) * d ** -0.5
+    vmax = rows_of[:, hq * d + w:].double().abs().amax(0).view(hkv, 1, d).expand(hkv, hq // hkv, d).reshape(-1)
+    # per side: scores, exponentials and sums in float; in bfloat16 the probabilities (one side's) and both results are rounded
+    err = 2 * (2 * (d + 2) * 2.0 ** -24 * size + 100 * 2.0 ** -24 + 2.0 ** -21) * vmax + (3 if dtype == torch.bfloat16 else 2) * half * vmax
+    move = float((err[columns][:, None] * R.abs()).sum(0).max())     # of a logit
+
+    # ---- one token a step
+    pool, table = torch.zeros(40, 2, page, w, dtype=dtype, device=DEV), torch.arange(n * 10, device=DEV).view(n, 10).int()
+    lens, want, best = [0] * n, [{} for _ in range(n)], [{} for _ in range(n)]   # by place: the row, (token behind it, gap)
+
+    def plain(tokens):
+        seq, pos = [s for s in range(n) for _ in tokens[s]], [lens[s] + i for s in range(n) for i in range(len(tokens[s]))]
+        x = rows_of[torch.tensor([t for f in tokens for t in f], device=DEV)]
+        q, o = torch.empty(len(seq), hq * d, dtype=dtype, device=DEV), torch.empty(len(seq), hq * d, dtype=dtype, device=DEV)
+        ops.qkv_rope_store(x[:, :hq * d], x[:, hq * d:hq * d + w], x[:, hq * d + w:], 1, 1, 1, inv, i32(pos), i32(seq), table, pool, q, None, None, hq, hkv, d)
+        ops.paged_attention(q, pool, table, i32(pos), i32(seq), o, hq, hkv, d, d ** -0.5, window=window, use_tensor_cores=False)
+        top = (o.double()[:, columns] @ R).topk(2)
+        for i, (s, p) in enumerate(zip(seq, pos)):
+            want[s][p] = o[i].double()
+            best[s][p] = (int(top.indices[i, 0]), float(top.values[i, 0] - top.values[i, 1]))
+        for s in range(n):
+            lens[s] += len(tokens[s])
+        return [[best[s][lens[s] - 1][0]] for s in range(n)]
+
+    nxt = plain(prompts)
+    out = [list(x) for x in nxt]                                     # out[s][i]: the token at place len(prompt) + i
+    for _ in range(total + 6):
+        nxt = plain(nxt)
+        for s in range(n):
+            out[s] += nxt[s]
+
+    # ---- drafted steps
+    pages, room, width = 40, 64, 8
+    pool = torch.zeros(1, pages + 1, 2, page, w, dtype=dtype, device=DEV)
+    free, blocks, blocks_out = rng.sample(range(pages), pages), i32([0] * n), i32([0] * n)
+    table = torch.full((n, 10), pages, dtype=torch.int32, device=DEV)
+    held, got = [0] * n, [0] * n                                     # got: tokens of out that are known
+    scratch, vscratch = ops.tree_attention_scratch(DEV), ops.verify_drafts_scratch(room, V, DEV)
+    feed, parents = [list(p) for p in prompts], [list(range(-1, len(p) - 1)) for p in prompts]
+    steps = compared = close = 0
+    while min(got) < total:
+        steps += 1
+        new = [len(f) for f in feed]
+        first = steps == 1
+        cu, taken, seq = i32([0] * (n + 1)), i32([0]), i32([0] * room)
+        pos, slots, masks = torch.zeros_like(seq), torch.full_like(seq, -1), torch.zeros(room, 1, dtype=torch.int64, device=DEV)
+        up = i32([p for f in parents for p in f] + [-1] * (room - sum(new)))
+        ops.step_tables(i32(held), i32(new), blocks, table, i32(free), page, pages, cu, seq, pos, slots, blocks_out, taken, parents=up, masks=masks)
+        blocks.copy_(blocks_out)
+        free = free[int(taken):]
+        tokens = i32([x for f in feed for x in f] + [0] * (room - sum(new)))
+        x, rows = rows_of[tokens.long()], torch.zeros(1, 2, room, w, dtype=dtype, device=DEV)
+        q, o = torch.empty(room, hq * d, dtype=dtype, device=DEV), torch.zeros(room, hq * d, dtype=dtype, device=DEV)
+        ops.qkv_rope_store(x[:, :hq * d], x[:, hq * d:hq * d + w], x[:, hq * d + w:], 1, 1, 1, inv, pos, seq, None, None, q, rows[0, 0], rows[0, 1], hq, hkv, d)
+        ops.tree_attention(q, rows[0, 0], rows[0, 1], pool[0], table, i32(held), cu, o, hq, hkv, d, d ** -0.5, scratch, mask=None if first else masks,
+                           positions=pos, window=window, window_step=True)
+        logits = (o.double()[:, columns] @ R).float()
+        tokens_out, path, count = (torch.full(size_, -1, dtype=torch.int32, device=DEV) for size_ in ((n, width), (n, width), (n,)))
+        if first:                                                    # a prompt: all of it is kept
+            path, count = i32([list(range(m)) + [-1] * (30 - m) for m in new]), i32(new)
+        else:
+            ops.verify_drafts(logits, tokens, cu, torch.zeros(room, device=DEV), tokens_out, path, count, vscratch, parents=up)
+        kept, nodes, said = count.tolist(), path.tolist(), tokens_out.tolist()
+        for s in range(n):
+            t0 = int(cu[s])
+            for j in range(kept[s]):
+                node, place = nodes[s][j], held[s] + j
+                assert ((o[t0 + node].double() - want[s][place]).abs() <= err).all(), (steps, s, j)
+                compared += 1
+                token, gap = best[s][place]
+                if first and j < kept[s] - 1:
+                    continue
+                mine = int(logits[t0 + node].argmax())
+                assert first or mine == said[s][j]
+                if mine != token:
+                    assert gap <= 2 * move + 1e-6, (steps, s, j, gap, move)
+                    close += 1
+                    kept[s] = j + 1                                  # the single steps' token goes on
+                    break
+        ops.keep_accepted(rows, pool, slots, cu, path, i32(kept))
+        feed, parents = [], []
+        for s in range(n):
+            got[s] += 1 if first else kept[s]
+            held[s] += kept[s]
+            assert held[s] == len(prompts[s]) + got[s] - 1
+            if got[s] >= total:                                      # a request that has got all: no tokens in the steps left
+                feed.append([])
+                parents.append([])
+                continue
+            coming = out[s][got[s]:got[s] + 4]
+            f, p, at = [out[s][got[s] - 1]], [-1], 0
+            right = rng.randint(0, len(coming))
+            for i, c in enumerate(coming):
+                if tree:                                             # a wrong token beside every right one
+                    f.append((c + 1) % V)
+                    p.append(at)
+                f.append(c if i < right else (c + 2) % V)
+                p.append(at)
+                at = len(f) - 1
+            feed.append(f)
+            parents.append(p)
+    assert compared >= n * total and steps < total and close <= compared // 4
