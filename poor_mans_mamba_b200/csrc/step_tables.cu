@@ -135,10 +135,11 @@ __global__ void __launch_bounds__(kTablesThreads) step_tables_kernel(const StepT
 constexpr int kKeepThreads = 256;
 constexpr int kKeepLoads = 4;   // pieces of a row that a lane has in flight
 constexpr int kKeepPlanes = 4;  // layers and planes of a block where there are many
+constexpr int kKeepResident = 4 * 148;  // blocks on the device at once (64 registers a thread)
 
 // V: the piece that a thread copies at a time (16 bytes where rows begin on such boundaries).
 template <typename V>
-__global__ void __launch_bounds__(kKeepThreads)
+__global__ void __launch_bounds__(kKeepThreads, kKeepResident / 148)
     keep_accepted_kernel(const V* rows, long long ld_layer, long long ld_plane, long long ld_row, int n_rows, V* pool, long long pages,
                          int layers, int planes, int per_block, int page_size, int width, const int* slots, const int* cu, const int* path,
                          int path_width, const int* count) {
@@ -224,8 +225,12 @@ PMM_EXPORT int pmm_keep_accepted(const void* rows, long long ld_layer, long long
   // the widest piece that every row begins on
   const long long all = reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(pool) | (ld_layer * item) | (ld_plane * item) |
                         (ld_row * item) | (static_cast<long long>(width) * item);
-  // four planes a block where a thousand blocks are left: 64 requests of 8 tokens, 32 layers of 1,024, 11.1 us, with one plane a block 12.9
-  const int per_block = static_cast<long long>(layers) * planes * n >= 4096 ? pmm::kKeepPlanes : 1;
+  // One plane a block while all blocks are on the device at once, two while half as many are, else four: a block that comes later than the
+  // first ones waits for its three dependent reads once more.  5 of 8 tokens kept, us with one, two and four planes a block:
+  //   planes x requests  576: 3.6  3.7  3.9    640: 5.2  4.0  4.8    896: 5.8  4.5  5.2 (rows of 1,024);   1,024: 5.0  3.9  4.3
+  //   1,536: 6.9  5.9  4.9 (of 512);   2,048: 12.9  11.0  10.4    4,096: 22.5  19.2  18.7    8,192: 41.4  33.5  32.9 (of 1,024)
+  const long long blocks = static_cast<long long>(layers) * planes * n;
+  const int per_block = blocks <= pmm::kKeepResident ? 1 : blocks <= 2 * pmm::kKeepResident ? 2 : pmm::kKeepPlanes;
   const dim3 grid((layers * planes + per_block - 1) / per_block, n);
   auto go = [&](auto zero) {
     using V = decltype(zero);

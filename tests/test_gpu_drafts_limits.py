@@ -523,3 +523,22 @@ def test_drafted_steps_row_by_row(dtype, tree, window):
             feed.append(f)
             parents.append(p)
     assert compared >= n * total and steps < total and close <= compared // 4
+
+
+# ----------------------------------------------------------------------------- kept rows of many layers and requests
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layers,planes,n", [(7, 2, 42), (5, 1, 130), (7, 1, 100), (3, 2, 200), (5, 1, 301), (7, 2, 150)])
+@pytest.mark.parametrize("width", [8, 72])
+def test_keep_accepted_of_many_requests(dtype, layers, planes, n, width):
+    """One, two and four planes a block, also where they do not divide the planes."""
+    rng, g = random.Random(n), torch.Generator().manual_seed(n)
+    lens = [rng.choice([0, 1, 5, 8]) for _ in range(n)]
+    T, page, pages = sum(lens), 8, 3 * n
+    pool = torch.randn(layers, pages, planes, page, width, generator=g).to(dtype).to(DEV)
+    rows = torch.randn(layers, planes, T, width, generator=g).to(dtype).to(DEV)
+    slots = rng.sample(range(pages * page), T)
+    count = [rng.randint(0, m) for m in lens]
+    path = [sorted(rng.sample(range(m), c)) + [-1] * (8 - c) for m, c in zip(lens, count)]
+    want = P.keep(rows.cpu(), pool.cpu(), slots, cumulate(lens), path, count)
+    K().keep_accepted(rows, pool, i32(slots), i32(cumulate(lens)), i32(path), i32(count))
+    assert torch.equal(pool.cpu(), want)
