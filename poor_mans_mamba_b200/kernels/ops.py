@@ -2405,6 +2405,7 @@ def tree_attention_scratch(device) -> Tensor:
 
 
 _SIZES: Dict[tuple, int] = {}
+_SIZES_KEPT = 1024  # (a step's number of rows changes from call to call)
 
 
 def _sized(name: str, *args: int) -> int:
@@ -2414,6 +2415,8 @@ def _sized(name: str, *args: int) -> int:
     if size is None:
         f = _fn(name)
         f.restype = c_longlong
+        if len(_SIZES) >= _SIZES_KEPT:
+            _SIZES.clear()
         size = _SIZES[key] = f(*args)
     return size
 

@@ -175,3 +175,9 @@ def test_tree_attention_refuses_outputs_in_its_inputs(name, elem, last):
     # one row: its neighbours in the same row are free
     assert not overlaps(name, apart, T=1, q=M, ldq=4096, k=M + row, ldk=4096, v=M + row + kv, ldv=4096, out=M + row + 2 * kv)
     assert overlaps(name, apart, T=1, q=M, ldq=4096, k=M + row, ldk=4096, v=M + row + kv, ldv=4096, out=M + row + kv)
+
+
+def test_sizes_of_scratch_are_not_remembered_without_end():
+    for rows in range(1, 3 * K._SIZES_KEPT):
+        assert K._sized("pmm_verify_scratch", rows, 5000) == 2 * rows * 5 * 16 + 4 * rows
+        assert len(K._SIZES) <= K._SIZES_KEPT
