@@ -260,7 +260,8 @@ __device__ __forceinline__ void tf_scores(float (&s)[N], const float* const (&q)
   }
 }
 
-template <typename S, int ACC>
+// STEP: the window limits the step's own tokens too (in a form of its own: asked of every row it costs the others 3 %).
+template <typename S, int ACC, bool STEP>
 __global__ void __launch_bounds__(kTfThreads, ACC <= 4 ? 2 : 1) tree_rows_kernel(const TreeAttnArgs<S> a, int T, int cluster) {
   extern __shared__ __align__(16) unsigned char tf_mem[];
   __shared__ float2 s_ml[2][kTfRows];
@@ -370,9 +371,6 @@ __global__ void __launch_bounds__(kTfThreads, ACC <= 4 ? 2 : 1) tree_rows_kernel
     const bool own = j >= ctx_tiles;
     const int base = (own ? (j - ctx_tiles) * kTfKeys : first + j * kTfKeys) + 32 * half;
     const int n_keys = min(32, (own ? n_new : held) - base);  // of this warp's half
-    const int key = base + lane;
-    // what a window is compared with: the place of a cached key, the position of one of the step's, or none where the mask alone decides
-    const int at = !own ? key : a.window_step && lane < n_keys ? a.positions[t0 + key] : 0x7fffffff;
     asm volatile("cp.async.wait_all;\n" ::: "memory");
     __syncthreads();
     // N of the warp's rows, or more than it has: the last one again, whose results nobody reads (a question per row and step costs
@@ -391,9 +389,9 @@ __global__ void __launch_bounds__(kTfThreads, ACC <= 4 ? 2 : 1) tree_rows_kernel
       bool all = true;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int r = wr + 4 * min(i, mine - 1), tok = s_tok[r];
-        const bool see = lane < n_keys && at >= s_lo[r] &&
-                         (!own || (a.mask ? ta_sees(a.mask + static_cast<size_t>(t0 + tok) * a.words, a.words, key) : key <= tok));
+        const int r = wr + 4 * min(i, mine - 1), tok = s_tok[r], key = base + lane;
+        const bool see = lane < n_keys && (!own ? key >= s_lo[r] : a.mask ? ta_sees(a.mask + static_cast<size_t>(t0 + tok) * a.words, a.words, key) : key <= tok) &&
+                         (!STEP || !own || a.positions[t0 + key] >= s_lo[r]);
         sees[i] = __ballot_sync(0xffffffffu, see);
         all = all && sees[i] == 0xffffffffu;
         const float sc = see ? s[i] * a.scale : -CUDART_INF_F;
@@ -524,7 +522,7 @@ int launch_tree_rows(const TreeAttnArgs<S>& a, int T, int sms, cudaStream_t stre
   while (cluster > 1 && (blocks * cluster > 4ll * sms || cluster > keys || (blocks * cluster > 2ll * sms && 2 * cluster > keys))) cluster /= 2;
   if (tiles * cluster > 0x7fffffffll) return PMM_ERR_BAD_ARGUMENT;
   const size_t smem = tf_smem(a.Dh, sizeof(S));
-  auto kern = tree_rows_kernel<S, ACC>;
+  auto kern = a.window_step ? tree_rows_kernel<S, ACC, true> : tree_rows_kernel<S, ACC, false>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));  // (of the current device: at every call)
   if (e != cudaSuccess) return static_cast<int>(e);
   cudaLaunchConfig_t cfg{};
