@@ -197,12 +197,13 @@ __global__ void __launch_bounds__(kTaWarps * 32, 3) tree_attention_kernel(const 
 }
 
 // Head sizes up to 256.  A cluster of blocks takes up to 32 rows of one request and key/value head; its blocks take the keys in tiles of 64 in
-// turn.  A tile of K and V lies in shared memory once for all rows (a block per row read the keys anew: 8 requests of 19 tokens with 32 / 8 heads
-// of 128 over 433 keys took 123 us, so 52; 12 requests of a token over 53 keys
-// 10 either way).  A warp has up to eight rows and 32 of a tile's keys: a lane a key for the scores, a slice of the head a lane for the values, so maxima, sums
-// and results stay in its registers.  In the end every block leaves (maximum, sum, unnormalised result) in its shared memory, and the cluster's
-// blocks join a share of the rows each, in the order of the blocks.  What bounds it: shared memory, 12 reads of 128 bytes for 32 products of a warp's scores,
-// 24 for 128 of its values.
+// turn.  A tile of K and V lies in shared memory once for all rows (with a block per row, as beyond 256, 8 requests of up to 19 tokens, 32 / 8
+// heads of 128, over up to 433 keys took 123 us, so 55).  A warp has up to eight rows and 32 of a tile's keys: a lane a key for the
+// scores, a slice of the head a lane for the values, so maxima, sums and results stay in its registers.  In the end every block leaves
+// (maximum, sum, unnormalised result) in its shared memory, and the cluster's blocks join a share of the rows each, in the order of the
+// blocks.  What bounds it: shared memory, 12 reads of 128 bytes for 32 products of a warp's scores, 24 for 128 of its values, and one tile at
+// a time, so that copies and products do not overlap: 14 requests of 5 over 2,340 keys, 32 / 8 heads of 128 in float32, take 262 us where
+// the keys' bytes are 41; shared memory is busy for 42 % of the time there, the float units for 29.
 constexpr int kTfRows = 32, kTfKeys = 64, kTfThreads = 256, kTfPer = 8;
 constexpr int kTfCluster = 8;  // blocks of a cluster at most
 
@@ -513,8 +514,10 @@ int launch_tree_rows(const TreeAttnArgs<S>& a, int T, int sms, cudaStream_t stre
   const int G = a.Hq / a.Hkv;
   const long long tiles = (static_cast<long long>(T) * G + kTfRows - 1) / kTfRows + min(T, a.n_seq);  // (at most)
   // Blocks of a cluster: the tables' width tells how many tiles of keys there may be, and requests of equal size how many tiles of rows.  Up
-  // to four blocks a multiprocessor (19 requests of 8 tokens over 608 keys, 32 / 8 heads of 128: 129 us with one, 77 with two), and from
-  // two on at least two tiles a block (6 of 2 over 514 keys: 30 us with eight, 21 with four).
+  // to four blocks a multiprocessor, and from two on at least two tiles a block.  Float32, us with 1, 2, 4 and 8 blocks, the rule's in brackets:
+  // 8 / 2 heads of 64: 1 request of 5 over 700 keys 73, 40, 23, [18]; 4 of 12 over 300 40, 23, [18], 15; 14 of 5 over 2,340 221, 129, 86, [48];
+  // 64 of 4 over 500 49, 29, [36], 54; 100 of 2 over 200 20, [27], 31, 54; 32 / 8 heads of 128: 6 of 2 over 514 43, 32, [21], 29; 12 of 1 over
+  // 53 11, [10], 16, 29; 19 of 8 over 608 145, [135], 121, 162.  Of 20 shapes 11 get the best, 6 more come within 16 %, the last are 24 and 36 % off.
   const long long each = (static_cast<long long>(T) * G + a.n_seq - 1) / a.n_seq, blocks = a.n_seq * ((each + kTfRows - 1) / kTfRows) * a.Hkv;
   long long keys = static_cast<long long>(a.max_blocks) * a.page_size / kTfKeys + 1;
   if (a.window != 0) keys = min(keys, llabs(static_cast<long long>(a.window)) / kTfKeys + 4);

@@ -20,10 +20,14 @@
 // 48 each instead of 32), exponentials 1,024 (16 a clock), 32 KB from L2 at 5.4 TB/s of all blocks 1,450; it takes 2,250, of them 2,000 a
 // warp's own way through load, maximum, exponentials and store: two warps a scheduler do not cover each other's latencies.  With
 // units of 128 rows memory bounds it: 32 x 16,384 takes 245 us, the copies alone 237.
+// (These figures are of replayed graphs on a card that has not heated up.  Among other calls the card is at its 1,000 W and the clock
+// falls: 32 x 16,384 takes 298 us there, 16 x 8,192 with trees of 64 360.)
+// P is rounded to bfloat16 for the product, the sum it is divided by is not: beside the formula in 64 bits a result is off by 0.0023 of
+// its size, of which its own rounding is 0.0017.
 // Of a tile's values only the 16 keys at a time that hold a valid one are multiplied; rows behind the last valid one (stale
 // places of a page, other requests' tokens) are set to zero first, for 0 * NaN is NaN.  Where a tile's keys are not seen by
 // all rows alike (the step's own tokens, a window's edge) values that are not finite are taken out of the product and added
-// by hand to the rows that see them.
+// by hand to the rows that see them.  (In units of 256 rows both sets do that in the tile that they share, and write the same bytes.)
 // Every mbarrier wait is bounded (status codes 41..45, see attention_tc.cu).  No cluster multicast.
 #include "attention_tc.cuh"
 #include "tree_attention.cuh"
@@ -289,7 +293,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_attention_tc_kernel(const 
   constexpr int kQSub = tree_q_sub();
   extern __shared__ unsigned char smem_raw[];
   // the queries are in place / have been read by a unit's last S; a slot is full / empty; a set's S and P are there; a unit's last
-  // products are done; both sets' maxima and sums are there; both have read their O; it is a set's turn to make its exponentials
+  // products are done; both sets' maxima and sums are there; both have read their O
   __shared__ __align__(8) unsigned long long bar_q, bar_qfree, bar_full[kBars], bar_empty[kRing], bar_s[2][2], bar_p[2][2], bar_o[2], bar_done, bar_ml, bar_read;
   __shared__ float2 s_ml[2][2][kTtRows];  // (of two stretches in turn: one set may be a stretch ahead)
   __shared__ unsigned s_tmem_base;

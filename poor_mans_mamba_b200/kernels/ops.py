@@ -2374,7 +2374,8 @@ def step_tables(held: Tensor, new: Tensor, blocks: Tensor, table: Tensor, free_p
     of a fixed size: what lies behind the last token is left as it was.
     ``parents`` [room], with ``masks`` int64 [room, words]: a token's parent as a place among its request's tokens, in front of
     it (anything else: none, as -1).  ``positions`` are then held + depth, and bit j of a token's mask says that token j of its
-    request is the token itself or above it (64 * words tokens a request; further ones have no bit).  Without: held + i.
+    request is the token itself or above it (64 * words tokens a request; further ones have no bit, not even their own, and
+    `tree_attention` then leaves them out).  Without: held + i.
     What it writes, a launch directly behind may read ahead of its wait: this one lets none begin early."""
     what = "step_tables"
     stream = _launch_stream(what, held, new, blocks, table, free_pages, cu, seq_of, positions, slots, blocks_out, taken, parents, masks)
@@ -2453,6 +2454,8 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, pool: Tensor, block_table: T
     among the step's tokens the mask alone decides.  With ``window_step`` the window limits those too, each by its position: what
     `paged_attention` has in steps of one token, so a layer with a window (or with chunks, ``window`` below zero) wants it;
     without, the tokens that a window or a chunk's border hides have to be out of the mask.  ``sink``: see `paged_attention`.
+    bfloat16 of head size 64 or 128 in pages of a multiple of 8, up to 1,024 requests, runs on the tensor cores, with
+    probabilities rounded to bfloat16; everything else in float on the CUDA cores, which takes three to five times as long.
     A row that sees no key is zero; rows behind the last request (cu_seqlens[n] and further) are left as they are.  ``out`` may
     be ``q`` itself, where that is contiguous; no other part of it lies in what is read."""
     what = "tree_attention"
