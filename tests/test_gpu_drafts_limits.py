@@ -542,3 +542,84 @@ def test_keep_accepted_of_many_requests(dtype, layers, planes, n, width):
     want = P.keep(rows.cpu(), pool.cpu(), slots, cumulate(lens), path, count)
     K().keep_accepted(rows, pool, i32(slots), i32(cumulate(lens)), i32(path), i32(count))
     assert torch.equal(pool.cpu(), want)
+
+
+# ----------------------------------------------------------------------------- the largest and the smallest calls
+@pytest.mark.parametrize("V", [600001, 1500000, 2097152])
+@pytest.mark.parametrize("mode", ["tree", "drawn"])
+def test_verify_drafts_of_the_largest_vocabularies(V, mode):
+    """Up to 2,048 pieces of a row, whose sums take 64 KB of every block's shared memory."""
+    lens, temps = [3, 1], [0.75, 1.0]
+    logits, draft, parents, tokens, u = drafts_of(lens, V, 3, temps, mode == "tree", near=0.3)
+    if mode == "drawn":   # (a draft that is refused, and one that is not)
+        tokens[1], u[1], u[2] = int(logits[0].argmax()), 0.0, 1 - 2.0 ** -24
+    verify(logits, tokens, lens, u, 3, temps, parents if mode == "tree" else None, draft if mode == "drawn" else None)
+    with pytest.raises(K().KernelError):
+        wide = torch.zeros(1, 2097153, device=DEV)
+        K().verify_drafts(wide, i32([0]), i32([0, 1]), u[:1].to(DEV), i32([[0]]), i32([[0]]), i32([0]), torch.empty(1 << 20, dtype=torch.uint8, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(300, 1, 64), (129, 1, 128), (1, 1, 64), (33, 33, 64)])
+def test_tree_attention_groups_of_any_size(dtype, heads):
+    """Groups of more rows than a unit or a block holds: a token's rows lie in several."""
+    c = Case([70, 0, 200], [3, 1, 2], heads, dtype, 64, seed=9, extra_rows=1)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("page", [1024, 4096, 4104])
+def test_tree_attention_large_pages(dtype, page):
+    c = Case([5000, 17, 0], [20, 3, 1], (8, 2, 64), dtype, page, seed=8)
+    c.run(300, window_step=True)
+    windowed(c, 300)
+    c.check(300)
+
+
+def test_calls_without_tokens():
+    """No rows at all: nothing is written but counts of zero, bounds and tables."""
+    ops, none = K(), torch.zeros(0, dtype=torch.int32, device=DEV)
+    out, path, count = i32([[7, 7]] * 2), i32([[7, 7]] * 2), i32([7, 7])
+    for draft in (None, torch.zeros(0, 50, device=DEV)):
+        ops.verify_drafts(torch.zeros(0, 50, device=DEV), none, i32([0, 0, 0]), torch.zeros(0, device=DEV), out, path, count, ops.verify_drafts_scratch(0, 50, DEV),
+                          draft_logits=draft)
+        assert out.tolist() == path.tolist() == [[-1, -1]] * 2 and count.tolist() == [0, 0]
+        out.fill_(7), path.fill_(7), count.fill_(7)
+    for d in (64, 512):
+        q, kv = torch.zeros(0, 2 * d, dtype=torch.bfloat16, device=DEV), torch.zeros(0, d, dtype=torch.bfloat16, device=DEV)
+        ops.tree_attention(q, kv, kv, torch.zeros(2, 2, 8, d, dtype=torch.bfloat16, device=DEV), i32([[0]]), i32([3]), i32([0, 0]), torch.empty_like(q), 2, 1, d, 0.1,
+                           ops.tree_attention_scratch(DEV))
+    pool = torch.ones(1, 2, 2, 8, 64, device=DEV)
+    ops.keep_accepted(torch.zeros(1, 2, 0, 64, device=DEV), pool, none, i32([0, 0]), i32([[0]]), i32([1]))
+    assert (pool == 1).all()
+    cu, table, taken, after = i32([5] * 3), i32([[4, 9], [9, 9]]), i32([5]), i32([5, 5])
+    ops.step_tables(i32([8, 0]), i32([0, 0]), i32([1, 0]), table, none, 8, 9, cu, none, none.clone(), none.clone(), after, taken)
+    assert cu.tolist() == [0, 0, 0] and table.tolist() == [[4, 9], [9, 9]] and taken.tolist() == [0] and after.tolist() == [1, 0]
+    ops.step_tables(i32([8, 3]), i32([1, 9]), i32([1, 1]), table, none, 8, 9, cu, none, none.clone(), none.clone(), after, taken)   # no room, no page
+    assert cu.tolist() == [0, 1, 10] and table.tolist() == [[4, 9], [9, 9]] and taken.tolist() == [2] and after.tolist() == [2, 2]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_verify_and_keep_side_by_side_on_two_streams(dtype):
+    """Two requests' batches at once, tensors of their own each."""
+    sets = []
+    for seed in (1, 2):
+        lens, temps = [5, 3, 8], [0.8, 0.0, 1.1]
+        logits, draft, _, tokens, u = drafts_of(lens, 33000, seed, temps, False)
+        rows, pool = torch.randn(4, 2, 16, 64, device=DEV).to(dtype), torch.zeros(4, 9, 2, 8, 64, dtype=dtype, device=DEV)
+        out = [i32([[0] * 8] * 3), i32([[0] * 8] * 3), i32([0] * 3)]
+        sets.append((lens, temps, logits, draft, tokens, u, rows, pool, random.Random(seed).sample(range(72), 16), out, K().verify_drafts_scratch(16, 33000, DEV),
+                     i32(tokens), i32(cumulate(lens)), u.to(DEV), torch.tensor(temps, device=DEV), torch.cuda.Stream()))
+    places = [i32(s[8]) for s in sets]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (lens, temps, logits, draft, tokens, u, rows, pool, slots, out, scratch, tok, cu, uni, temp, stream), at in zip(sets, places):
+            with torch.cuda.stream(stream):
+                K().verify_drafts(logits, tok, cu, uni, *out, scratch, temperature=temp, draft_logits=draft)
+                K().keep_accepted(rows, pool, at, cu, out[1], out[2])
+    torch.cuda.synchronize()
+    for lens, temps, logits, draft, tokens, u, rows, pool, slots, out, *_ in sets:
+        want = P.verify(logits.cpu(), tokens, cumulate(lens), u, 8, temps, None, draft.cpu())
+        assert dict(tokens=out[0].tolist(), path=out[1].tolist(), count=out[2].tolist()) == want
+        assert torch.equal(pool.cpu(), P.keep(rows.cpu(), torch.zeros_like(pool).cpu(), slots, cumulate(lens), want["path"], want["count"]))
