@@ -191,7 +191,7 @@ def test_tree_attention_of_one_row_of_any_stride(dtype, heads):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("heads", [(8, 2, 64), (64, 8, 128), (2, 1, 256), (2, 1, 512)])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (16, 1, 128), (2, 1, 256), (2, 1, 512)])
 def test_tree_attention_in_the_place_of_the_queries(dtype, heads):
     """Results written over q: units of one block, units that shares cut, wide ones."""
     for held, new in (([3000, 40], [33, 9]), ([20] * 300, [5] * 300), ([0], [1])):
@@ -254,7 +254,7 @@ def windowed(c, window):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("heads", [(8, 2, 64), (6, 2, 128), (16, 1, 128), (16, 1, 64), (2, 1, 256), (2, 1, 512)])
-@pytest.mark.parametrize("window", [1, 2, 5, 30, 200, -1, -8, -50, -64])
+@pytest.mark.parametrize("window", [1, 5, 200, -8, -64])
 @pytest.mark.parametrize("parents", ["tree", None])
 def test_tree_attention_window_over_the_step(dtype, heads, window, parents):
     """Paths deeper than the window, chunks whose border lies among the step's tokens; hidden values that are not numbers harm nobody."""
